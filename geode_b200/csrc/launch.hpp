@@ -1,104 +1,16 @@
-// launch.hpp - host-side launch helpers: the static GEMV's launch (shared-memory opt-in, grid sized to the SMs,
-// optionally as a programmatic dependent launch), a process-wide launch counter and the operators' status word.
-// What depends on the GPU (its SM count, the kernels' shared-memory opt-in, the status word) is kept per device and
-// set up the first time a launch on that device (the current one) needs it, so handles on several GPUs of one
-// process each get their own.
+// launch.hpp - host-side launch helpers of the GEMVs: the static GEMV's launch (shared-memory opt-in, grid sized to the
+// SMs, optionally as a programmatic dependent launch) and the bf16 GEMV's.
 #pragma once
 
 #include <cuda_runtime.h>
 
 #include <algorithm>
-#include <atomic>
-#include <cstdint>
-#include <mutex>
 
 #include "../../include/geode_cuda.h"
+#include "device.hpp"
 #include "gemv_kernels.cuh"
 
 namespace gcu {
-
-inline std::atomic<uint64_t> &launch_counter() {
-    static std::atomic<uint64_t> n{0};
-    return n;
-}
-inline void count_launch(uint64_t k = 1) { launch_counter().fetch_add(k, std::memory_order_relaxed); }
-
-// Per-device set-up state, filled lazily under one mutex. gemv_rc / bf16_rc: 0 = not tried yet, else the outcome
-// (GCUDA_OK or GCUDA_E_CUDA) of the shared-memory opt-in on that device.
-constexpr int kMaxDevices = 64;
-struct DeviceState {
-    std::mutex mu;
-    int sms[kMaxDevices] = {};
-    int gemv_rc[kMaxDevices] = {};
-    int bf16_rc[kMaxDevices] = {};
-    int umma_rc[kMaxDevices] = {};
-    int lane_rc[kMaxDevices] = {};
-    size_t lane_avail[kMaxDevices] = {};   // the expert lane kernels' dynamic shared memory limit
-    uint32_t *status[kMaxDevices] = {};
-};
-inline DeviceState &device_state() {
-    static DeviceState d;
-    return d;
-}
-inline int current_device() {
-    int dev = -1;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return -1;
-    return dev;
-}
-
-inline int sm_count() {
-    const int dev = current_device();
-    if (dev < 0) return 148;
-    DeviceState &d = device_state();
-    std::lock_guard<std::mutex> lock(d.mu);
-    if (!d.sms[dev]) {
-        int c = 0;
-        if (cudaDeviceGetAttribute(&c, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || c <= 0) c = 148;
-        d.sms[dev] = c;
-    }
-    return d.sms[dev];
-}
-
-// The operators' status word on the current device (device memory, zeroed once): kernels OR error flags into it.
-inline uint32_t *device_status() {
-    const int dev = current_device();
-    if (dev < 0) return nullptr;
-    DeviceState &d = device_state();
-    std::lock_guard<std::mutex> lock(d.mu);
-    if (!d.status[dev]) {
-        void *q = nullptr;
-        if (cudaMalloc(&q, 4) != cudaSuccess) return nullptr;
-        if (cudaMemset(q, 0, 4) != cudaSuccess) {
-            cudaFree(q);
-            return nullptr;
-        }
-        d.status[dev] = static_cast<uint32_t *>(q);
-    }
-    return d.status[dev];
-}
-
-// Launch with the programmatic-stream-serialization attribute when pdl: the kernel may begin (its prologue, the
-// weight stream) before the previous kernel on the stream ends; it waits for it at griddepcontrol.wait.
-template <typename Kern, typename... Args>
-inline cudaError_t launch_ex(Kern kern, dim3 grid, dim3 block, size_t smem, cudaStream_t st, bool pdl, Args... args) {
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = grid;
-    cfg.blockDim = block;
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    int na = 0;
-    if (pdl) {
-        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr[0].val.programmaticStreamSerializationAllowed = 1;
-        na = 1;
-    }
-    cfg.attrs = attr;
-    cfg.numAttrs = na;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, args...);
-    count_launch();
-    return e;
-}
 
 // The GEMV kernels' shared-memory opt-in: the largest any launch shape takes (plan_gemv caps it there).
 // (cudaFuncSetAttribute acts on the current device's context, so each device opts in once.)
