@@ -52,6 +52,11 @@ def cuda_lib() -> C.CDLL:
         "gcuda_op_moe_umma_relayout": (i32, [vp, sz, i32, i32, i32, vp, vp]),
         "gcuda_op_moe_umma": (i32, [vp, vp, i32, i32, i32, vp, vp, vp, i32, vp, i32, vp, vp, sz, vp]),
         "gcuda_debug_expf_table": (i32, [C.c_uint32, i64, vp, vp]),
+        # many conversations at once (descriptors: geode_b200.batch)
+        "gcuda_op_paged_append": (i32, [vp, vp, vp, vp]),
+        "gcuda_op_paged_attn_work_bytes": (sz, [vp, vp, i32]),
+        "gcuda_op_paged_attn": (i32, [vp, vp, vp, vp, sz, vp]),
+        "gcuda_op_logits_adjust": (i32, [vp, vp, vp, i32, i32, i32, i32, i64, i64, vp]),
     }
     for name, (res, args) in sig.items():
         if hasattr(L, name):

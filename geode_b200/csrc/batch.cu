@@ -1,0 +1,130 @@
+// batch.cu - the operators for many conversations at once (gcuda_op_paged_append, gcuda_op_paged_attn,
+// gcuda_op_logits_adjust): argument checks and launches. A translation unit of its own.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <type_traits>
+
+#include "../../include/geode_cuda.h"
+#include "device.hpp"
+#include "logits_adjust.cuh"
+#include "paged.cuh"
+#include "paged_attn.cuh"
+
+using namespace gcu;
+
+namespace {
+
+bool activation(int type) { return type == GCUDA_F32 || type == GCUDA_BF16 || type == GCUDA_F16; }
+bool misaligned(const void *p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n != 0; }
+size_t value_bytes(int type) { return type == GCUDA_F32 ? 4 : type == GCUDA_I8 ? 1 : 2; }
+
+// The geometry alone (what the scratch's size follows from); then with the pointers
+bool good_geometry(const gcuda_paged_kv *kv, const gcuda_paged_batch *b) {
+    return kv && b && (kv->type == GCUDA_I8 || kv->type == GCUDA_BF16 || kv->type == GCUDA_F16) && kv->n_pages >= 1 &&
+           kv->page_size >= 1 && kv->n_kv_heads >= 1 && kv->n_kv_heads <= 1024 &&
+           (kv->head_dim == 64 || kv->head_dim == 128 || kv->head_dim == 256) && b->n_seq >= 1 && b->n_rows >= 1 &&
+           b->max_rows >= 1 && b->max_pages >= 1 && b->pages_stride >= 0;
+}
+bool good_cache(const gcuda_paged_kv *kv, const gcuda_paged_batch *b) {
+    if (!good_geometry(kv, b) || !kv->k || !kv->v || !b->row_start || !b->length || !b->pages) return false;
+    if ((kv->type == GCUDA_I8) != (kv->k_scale != nullptr) || (kv->type == GCUDA_I8) != (kv->v_scale != nullptr)) return false;
+    const int64_t unit = 16 / static_cast<int64_t>(value_bytes(kv->type));
+    return !misaligned(kv->k, 16) && !misaligned(kv->v, 16) && kv->page_stride % unit == 0 && kv->pos_stride % unit == 0 &&
+           kv->head_stride % unit == 0 && kv->page_stride >= 0 && kv->pos_stride >= 0 && kv->head_stride >= 0;
+}
+
+// f(activation type, cache type) for the call's types
+template <int CACHE, typename F>
+int by_activation(int act, F f) {
+    if (act == GCUDA_F32) return f(float{}, std::integral_constant<int, CACHE>{});
+    if (act == GCUDA_BF16) return f(__nv_bfloat16{}, std::integral_constant<int, CACHE>{});
+    return f(__half{}, std::integral_constant<int, CACHE>{});
+}
+template <typename F>
+int by_types(int act, int cache, F f) {
+    if (cache == GCUDA_I8) return by_activation<GCUDA_I8>(act, f);
+    if (cache == GCUDA_BF16) return by_activation<GCUDA_BF16>(act, f);
+    return by_activation<GCUDA_F16>(act, f);
+}
+template <typename F>
+int by_dim(int hd, F f) {
+    if (hd == 64) return f(std::integral_constant<int, 64>{});
+    if (hd == 128) return f(std::integral_constant<int, 128>{});
+    return f(std::integral_constant<int, 256>{});
+}
+int launched(cudaError_t e) { return e == cudaSuccess ? GCUDA_OK : GCUDA_E_CUDA; }
+
+}  // namespace
+
+extern "C" {
+
+int gcuda_op_paged_append(const gcuda_paged_kv *kv, const gcuda_paged_batch *b, const gcuda_append_rows *x, void *stream) {
+    if (!good_cache(kv, b) || !x || !activation(x->type) || !x->k || !x->v || x->n_heads < 0 || x->n_heads > 1024 ||
+        (x->n_heads > 0) != (x->q != nullptr) || (x->n_heads > 0) != (x->q_out != nullptr) || x->rope_dim < 0 ||
+        x->rope_dim % 2 || x->rope_dim > kv->head_dim || (x->rope_dim > 0 && !x->inv_freq) || !(x->eps >= 0.0f) ||
+        (x->q && x->q == x->q_out && (x->q_stride != x->q_out_stride || x->q_head_stride != kv->head_dim)))
+        return GCUDA_E_ARG;
+    AppendArgs a{*kv, *b, *x, device_status()};
+    if (!a.status) return GCUDA_E_CUDA;
+    return by_types(x->type, kv->type, [&](auto act, auto cache) {
+        return by_dim(kv->head_dim, [&](auto hd) {
+            return launched(launch_ex(k_paged_append<hd(), decltype(act), cache()>, dim3(b->n_rows), dim3(kAppendThreads), 0,
+                                      static_cast<cudaStream_t>(stream), false, a));
+        });
+    });
+}
+
+size_t gcuda_op_paged_attn_work_bytes(const gcuda_paged_kv *kv, const gcuda_paged_batch *b, int n_heads) {
+    if (!good_geometry(kv, b) || b->max_rows > kMaxTok || n_heads < 1 || n_heads > 1024 || n_heads % kv->n_kv_heads) return 0;
+    return 256;
+}
+
+int gcuda_op_paged_attn(const gcuda_paged_kv *kv, const gcuda_paged_batch *b, const gcuda_attn_rows *x, void *d_work,
+                        size_t work_bytes, void *stream) {
+    if (!good_cache(kv, b) || !x || !activation(x->type) || !x->q || !x->out || !d_work || misaligned(d_work, 256) ||
+        x->window < 0)
+        return GCUDA_E_ARG;
+    const size_t need = gcuda_op_paged_attn_work_bytes(kv, b, x->n_heads);
+    if (need == 0 || work_bytes < need) return GCUDA_E_ARG;
+    PagedAttnArgs a{*kv, *b, *x, device_status()};
+    if (!a.status) return GCUDA_E_CUDA;
+    return by_types(x->type, kv->type, [&](auto act, auto cache) {
+        return by_dim(kv->head_dim, [&](auto hd) {
+            return launched(launch_ex(k_paged_attn<hd(), decltype(act), cache()>, dim3(b->n_rows, x->n_heads),
+                                      dim3(kPagedAttnThreads), 0, static_cast<cudaStream_t>(stream), false, a));
+        });
+    });
+}
+
+int gcuda_op_logits_adjust(const gcuda_logit_rules *r, const void *d_in, void *d_out, int type, int S, int k, int V,
+                           int64_t in_stride, int64_t out_stride, void *stream) {
+    if (!r || !d_in || !d_out || !activation(type) || S < 1 || S > (1 << 20) || k < 0 || k > 64 || V < 1 || in_stride < V ||
+        out_stride < V)
+        return GCUDA_E_ARG;
+    const int64_t rows = static_cast<int64_t>(S) * (k + 1);
+    if ((r->history != nullptr) != (r->history_len != nullptr) || (r->bias_id != nullptr) != (r->bias != nullptr) ||
+        (r->bias_id != nullptr) != (r->bias_len != nullptr) || (r->drafts && k == 0) || r->history_stride < 0 ||
+        r->bias_stride < 0 || (r->mask_row && !r->mask) ||
+        (r->mask && (r->n_masks < 1 || r->mask_stride < (V + 31) / 32 || (!r->mask_row && r->n_masks < rows))))
+        return GCUDA_E_ARG;
+    // in place row for row, or apart
+    const char *i0 = static_cast<const char *>(d_in), *o0 = static_cast<const char *>(d_out);
+    const int64_t es = static_cast<int64_t>(value_bytes(type)), ib = ((rows - 1) * in_stride + V) * es,
+                  ob = ((rows - 1) * out_stride + V) * es;
+    if (i0 == o0 ? in_stride != out_stride : (i0 < o0 + ob && o0 < i0 + ib)) return GCUDA_E_ARG;
+    AdjustArgs a{*r, d_in, d_out, S, k, V, 0, 0, in_stride, out_stride, device_status()};
+    if (!a.status) return GCUDA_E_CUDA;
+    a.slice = 4096;
+    a.slices = (V + a.slice - 1) / a.slice;
+    if (static_cast<int64_t>(S) * a.slices > 0x7fffffff) return GCUDA_E_ARG;
+    const dim3 grid(S * a.slices);
+    const size_t smem = 2 * sizeof(int) * a.slice;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (type == GCUDA_F32) return launched(launch_ex(k_logits_adjust<float>, grid, dim3(kAdjustThreads), smem, st, false, a));
+    if (type == GCUDA_BF16)
+        return launched(launch_ex(k_logits_adjust<__nv_bfloat16>, grid, dim3(kAdjustThreads), smem, st, false, a));
+    return launched(launch_ex(k_logits_adjust<__half>, grid, dim3(kAdjustThreads), smem, st, false, a));
+}
+
+}  // extern "C"

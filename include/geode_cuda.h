@@ -350,6 +350,121 @@ int gcuda_op_greedy_verify(const float *d_target, const int *d_drafts, int S, in
 int gcuda_op_spec_reject_static(const float *d_target, const float *d_draft, const int *drafts, int S, int k, int V,
                                 const gcuda_sampling *s, uint64_t seed, int *accepted, int *next, void *stream);
 
+/* ------------------------------------------------------------------------------- many conversations at once ----
+ * The operators of a batched step over a paged KV cache: gcuda_op_paged_append puts the step's key and value rows into
+ * the cache (and norms and rotates the queries on the way), gcuda_op_paged_attn lets each sequence's new rows attend
+ * over its pages, gcuda_op_logits_adjust applies penalties, biases and grammar masks to the rows that
+ * gcuda_op_greedy_verify or the rejection samplers then accept from. No counterpart in the reference, which holds one
+ * conversation in one contiguous cache (its arithmetic per row: engine/src/model.cpp:3705-3797, 3815-4019, and the
+ * presence penalty of engine/src/geode.cpp:234-255).
+ *
+ * Types of values: activations and 16-bit cache rows are read and written as these; GCUDA_I8 rows are int8 codes with
+ * one float scale per (position, head), as the engine's cache (value = code * scale). */
+#define GCUDA_F32 0
+#define GCUDA_BF16 1
+#define GCUDA_F16 2
+#define GCUDA_I8 3
+
+/* A paged cache: n_pages pages of page_size positions, each position n_kv_heads rows of head_dim values (64, 128 or
+ * 256) in k and in v. Value (page, position, head, d) of either lies at page * page_stride + position * pos_stride +
+ * head * head_stride + d (strides in values, so heads may be inside or outside the positions, and k and v may be two
+ * halves of each page of one buffer); its scale likewise by the scale_* strides. k, v and the three strides in bytes
+ * are multiples of 16. type: GCUDA_I8 (k_scale and v_scale needed, scales >= 0), GCUDA_BF16 or GCUDA_F16 (both NULL). */
+typedef struct {
+    void *k, *v;
+    float *k_scale, *v_scale;
+    int type, n_pages, page_size, n_kv_heads, head_dim;
+    int64_t page_stride, pos_stride, head_stride;
+    int64_t scale_page_stride, scale_pos_stride, scale_head_stride;
+} gcuda_paged_kv;
+
+/* The step's rows: sequence s owns rows row_start[s] .. row_start[s+1]-1 (at most max_rows) of the step's buffers of
+ * n_rows rows; its cache holds length[s] positions, its rows the last of them; position p lies on page
+ * pages[s * pages_stride + p / page_size], p / page_size < max_pages. The three arrays are device memory (int32), so a
+ * captured step follows its plan from replay to replay. Rows of no sequence (behind row_start[n_seq]) are neither read
+ * nor written. What is out of range on the device raises the status word's flag 2 (gcuda_op_status): a sequence whose
+ * rows or length are out of range is left out whole; a position on a page id outside [0, n_pages) is not stored and
+ * not attended to. */
+typedef struct {
+    int n_seq, n_rows, max_rows, max_pages;
+    const int *row_start, *length, *pages;
+    int64_t pages_stride;
+} gcuda_paged_batch;
+
+/* The rows of gcuda_op_paged_append: k and v rows of n_kv_heads * head_dim values, k_stride / v_stride apart; q rows
+ * of n_heads heads q_head_stride apart (the engine's query | gate rows: 2 head_dim), q_stride from row to row. Query
+ * and key heads go through the zero-centred RMSNorm x / sqrt(mean x^2 + eps) * (1 + w) with w = q_norm / k_norm
+ * [head_dim] (NULL: no norm) and the rotate-half rotary embedding over the first rope_dim values (even; 0: none), the
+ * angle position * inv_freq[i] (float [rope_dim / 2]) taken in 64 bits. q_out [n_rows][n_heads][head_dim], rows
+ * q_out_stride apart: the queries after both, in `type` (q_out may be q itself with the same strides; n_heads 0, q and
+ * q_out NULL: keys and values only). Keys and values are rounded once to a 16-bit cache; into an int8 cache the row
+ * rounded to float, its scale amax / 127 and its codes the nearest of 127 x / amax, the even one of two (an all-zero
+ * row: zeros), computed in 64 bits. type: GCUDA_F32, GCUDA_BF16 or GCUDA_F16, of q, k, v and q_out alike. */
+typedef struct {
+    int type, n_heads, rope_dim;
+    float eps;
+    const void *q, *k, *v;
+    void *q_out;
+    int64_t q_stride, q_head_stride, k_stride, v_stride, q_out_stride;
+    const float *q_norm, *k_norm, *inv_freq;
+} gcuda_append_rows;
+/* Appends the step's rows: row i of sequence s (i-th of T) at position length[s] - T + i. Two sequences must not
+ * write one position's rows in the same call. */
+int gcuda_op_paged_append(const gcuda_paged_kv *kv, const gcuda_paged_batch *b, const gcuda_append_rows *x, void *stream);
+
+/* The rows of gcuda_op_paged_attn: q rows of n_heads heads (n_heads a multiple of n_kv_heads, query head h reads key
+ * head h / (n_heads / n_kv_heads)) q_head_stride apart; out [n_rows][n_heads][head_dim], rows out_stride apart; lse
+ * [n_rows][n_heads] float (NULL: not wanted). Row i of sequence s (i-th of its T <= max_rows <= 8) at position
+ * p = length[s] - T + i attends to the positions 0 .. p (the last `window` of them when window > 0):
+ * out = sum softmax(scale * q . k) v, lse = log sum exp(scale * q . k). A row that sees no position (an empty
+ * sequence, p < 0) gives zeros and lse -inf. Values at positions a row does not see do not touch it, whatever they
+ * are. type: of q and out. */
+typedef struct {
+    int type, n_heads, window;
+    float scale;
+    const void *q;
+    void *out;
+    float *lse;
+    int64_t q_stride, q_head_stride, out_stride;
+} gcuda_attn_rows;
+/* Scratch of the call: gcuda_op_paged_attn_work_bytes of the same cache geometry, batch sizes and n_heads on the
+ * current device (0: out of range), 256-byte aligned. Its contents need not be set and do not matter afterwards; two
+ * calls that may run at the same time need one each. */
+size_t gcuda_op_paged_attn_work_bytes(const gcuda_paged_kv *kv, const gcuda_paged_batch *b, int n_heads);
+int gcuda_op_paged_attn(const gcuda_paged_kv *kv, const gcuda_paged_batch *b, const gcuda_attn_rows *x, void *d_work,
+                        size_t work_bytes, void *stream);
+
+/* The rules of gcuda_op_logits_adjust, per sequence (device memory; any of them NULL: that rule is off):
+ *   bias_id / bias [n_seq][bias_stride], bias_len [n_seq] entries used: the last entry of an id is added to its logit;
+ *   history [n_seq][history_stride], history_len [n_seq] tokens used, duplicates and all: row i of a sequence counts
+ *   them and the sequence's drafts 0 .. i-1 (drafts [n_seq][k]; the samples of rows 0 .. i-1 when their drafts stood).
+ *   A token that occurs c > 0 times: l = l > 0 ? l / repetition : l * repetition, then l - frequency * c - presence
+ *   (repetition, frequency, presence: float [n_seq]; NULL: 1, 0, 0);
+ *   mask [n_masks] rows of ceil(V / 32) 32-bit words, mask_stride words apart, bit v % 32 of word v / 32 set where
+ *   token v is allowed: the others become -inf. mask_row [n_seq * (k+1)]: the mask of each row, negative: none
+ *   (NULL: row i has mask i, n_masks >= n_seq * (k+1)).
+ * Negative ids are padding and are passed over; ids >= V are left out and raise the status word's flag 4; a length
+ * outside [0, stride] is clamped, a mask_row >= n_masks leaves its row unmasked, and both raise flag 2. */
+typedef struct {
+    const int *history, *history_len;
+    int64_t history_stride;
+    const int *drafts;
+    const float *repetition, *frequency, *presence;
+    const int *bias_id;
+    const float *bias;
+    const int *bias_len;
+    int64_t bias_stride;
+    const uint32_t *mask;
+    const int *mask_row;
+    int n_masks;
+    int64_t mask_stride;
+} gcuda_logit_rules;
+/* d_out row = the rules in this order (biases, penalties, mask) on d_in row, for S sequences of k+1 rows of V logits
+ * (rows s * (k+1) + i, in_stride and out_stride values apart), computed in float and rounded once to `type`
+ * (GCUDA_F32, GCUDA_BF16 or GCUDA_F16). d_out may be d_in with the same stride; otherwise they must not overlap. */
+int gcuda_op_logits_adjust(const gcuda_logit_rules *r, const void *d_in, void *d_out, int type, int S, int k, int V,
+                           int64_t in_stride, int64_t out_stride, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
