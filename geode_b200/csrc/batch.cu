@@ -10,6 +10,7 @@
 #include "logits_adjust.cuh"
 #include "paged.cuh"
 #include "paged_attn.cuh"
+#include "paged_attn_plan.hpp"
 
 using namespace gcu;
 
@@ -77,7 +78,7 @@ int gcuda_op_paged_append(const gcuda_paged_kv *kv, const gcuda_paged_batch *b, 
 
 size_t gcuda_op_paged_attn_work_bytes(const gcuda_paged_kv *kv, const gcuda_paged_batch *b, int n_heads) {
     if (!good_geometry(kv, b) || b->max_rows > kMaxTok || n_heads < 1 || n_heads > 1024 || n_heads % kv->n_kv_heads) return 0;
-    return 256;
+    return plan_paged_attn(*kv, *b, n_heads).total;
 }
 
 int gcuda_op_paged_attn(const gcuda_paged_kv *kv, const gcuda_paged_batch *b, const gcuda_attn_rows *x, void *d_work,
@@ -87,14 +88,15 @@ int gcuda_op_paged_attn(const gcuda_paged_kv *kv, const gcuda_paged_batch *b, co
         return GCUDA_E_ARG;
     const size_t need = gcuda_op_paged_attn_work_bytes(kv, b, x->n_heads);
     if (need == 0 || work_bytes < need) return GCUDA_E_ARG;
-    PagedAttnArgs a{*kv, *b, *x, device_status()};
+    const PagedAttnPlan p = plan_paged_attn(*kv, *b, x->n_heads);
+    uint8_t *w = static_cast<uint8_t *>(d_work);
+    const PagedAttnArgs a{*kv, *b, *x, device_status(), reinterpret_cast<int4 *>(w + p.desc),
+                          reinterpret_cast<float4 *>(w + p.stats), reinterpret_cast<float4 *>(w + p.part)};
     if (!a.status) return GCUDA_E_CUDA;
-    return by_types(x->type, kv->type, [&](auto act, auto cache) {
-        return by_dim(kv->head_dim, [&](auto hd) {
-            return launched(launch_ex(k_paged_attn<hd(), decltype(act), cache()>, dim3(b->n_rows, x->n_heads),
-                                      dim3(kPagedAttnThreads), 0, static_cast<cudaStream_t>(stream), false, a));
-        });
-    });
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (kv->type == GCUDA_I8) return launch_paged_attn_i8(a, p, st);
+    if (kv->type == GCUDA_BF16) return launch_paged_attn_bf16(a, p, st);
+    return launch_paged_attn_f16(a, p, st);
 }
 
 int gcuda_op_logits_adjust(const gcuda_logit_rules *r, const void *d_in, void *d_out, int type, int S, int k, int V,

@@ -21,12 +21,12 @@ constexpr int kAdjustThreads = 256;
 // row i. Then one pass over each row's slice.
 template <typename T>
 __global__ void __launch_bounds__(kAdjustThreads) k_logits_adjust(AdjustArgs a) {
-    extern __shared__ int sm[];
-    int *count = sm, *entry = sm + a.slice;   // occurrences, 1 + the last bias entry
+    extern __shared__ int adjust_sm[];
+    int *count = adjust_sm, *entry = adjust_sm + a.slice;   // occurrences, 1 + the last bias entry
     const int tid = threadIdx.x, s = blockIdx.x / a.slices, v0 = (blockIdx.x % a.slices) * a.slice;
     const int nv = min(a.slice, a.V - v0), rows = a.k + 1;
     const gcuda_logit_rules &r = a.r;
-    for (int i = tid; i < 2 * a.slice; i += kAdjustThreads) sm[i] = 0;
+    for (int i = tid; i < 2 * a.slice; i += kAdjustThreads) adjust_sm[i] = 0;
     __syncthreads();
     auto checked = [&](int n, int64_t most) {
         if (n >= 0 && n <= most) return n;

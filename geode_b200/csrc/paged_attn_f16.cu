@@ -1,0 +1,6 @@
+// paged_attn_f16.cu - gcuda_op_paged_attn's kernels over a f16 cache.
+#include "paged_attn_launch.cuh"
+
+int gcu::launch_paged_attn_f16(const PagedAttnArgs &a, const PagedAttnPlan &p, cudaStream_t st) {
+    return launch_paged_cache<GCUDA_F16>(a, p, st);
+}

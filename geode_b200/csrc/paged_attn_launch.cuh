@@ -1,0 +1,49 @@
+// paged_attn_launch.cuh - the attention kernels' instantiations and launches for one cache type (included by the
+// paged_attn_*.cu files, one per type, which compile side by side).
+#pragma once
+
+#include <atomic>
+
+#include "device.hpp"
+#include "paged_attn.cuh"
+#include "paged_attn_plan.hpp"
+
+namespace gcu {
+
+template <typename S>
+int launch_paged_shape(const PagedAttnArgs &a, int grid, cudaStream_t st) {
+    static std::atomic<uint64_t> opted{0};   // devices whose shared-memory opt-in is done
+    const int dev = current_device();
+    if (dev < 0) return GCUDA_E_CUDA;
+    if (!(opted.load(std::memory_order_relaxed) >> dev & 1)) {
+        if (cudaFuncSetAttribute(k_paged_attn<S>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem) != cudaSuccess)
+            return GCUDA_E_CUDA;
+        opted.fetch_or(1ull << dev, std::memory_order_relaxed);
+    }
+    if (launch_ex(k_paged_attn<S>, dim3(grid), dim3(kPagedAttnThreads), S::kSmem, st, true, a) != cudaSuccess) return GCUDA_E_CUDA;
+    if (grid == 1) return GCUDA_OK;
+    const int units = (S::NTT * S::OM / 2 + 3) / 4;
+    return launch_ex(k_paged_attn_join<S>, dim3(grid - 1, units), dim3(kPagedAttnThreads), 0, st, true, a, grid) == cudaSuccess
+               ? GCUDA_OK
+               : GCUDA_E_CUDA;
+}
+
+template <int CACHE, int HD, bool SPLIT>
+int launch_paged_rows(const PagedAttnArgs &a, const PagedAttnPlan &p, cudaStream_t st) {
+    if (p.rows == 8) return launch_paged_shape<PagedShape<HD, CACHE, SPLIT, 1, 1>>(a, p.grid, st);
+    if (p.rows == 16) return launch_paged_shape<PagedShape<HD, CACHE, SPLIT, 2, 1>>(a, p.grid, st);
+    return launch_paged_shape<PagedShape<HD, CACHE, SPLIT, 2, 4>>(a, p.grid, st);
+}
+template <int CACHE, int HD>
+int launch_paged_split(const PagedAttnArgs &a, const PagedAttnPlan &p, cudaStream_t st) {
+    const bool split = a.x.type == GCUDA_F32 || (a.x.type == GCUDA_F16 && CACHE == GCUDA_BF16);
+    return split ? launch_paged_rows<CACHE, HD, true>(a, p, st) : launch_paged_rows<CACHE, HD, false>(a, p, st);
+}
+template <int CACHE>
+int launch_paged_cache(const PagedAttnArgs &a, const PagedAttnPlan &p, cudaStream_t st) {
+    if (a.kv.head_dim == 64) return launch_paged_split<CACHE, 64>(a, p, st);
+    if (a.kv.head_dim == 128) return launch_paged_split<CACHE, 128>(a, p, st);
+    return launch_paged_split<CACHE, 256>(a, p, st);
+}
+
+}  // namespace gcu

@@ -1,0 +1,48 @@
+// paged_attn_plan.hpp - the host's side of gcuda_op_paged_attn: which kernel shape takes the call, its grid and scratch.
+#pragma once
+
+#include <algorithm>
+
+#include "device.hpp"
+
+namespace gcu {
+
+struct PagedAttnArgs;
+struct PagedAttnPlan {
+    int rows;      // query rows of a block (8, 16: position groups of one warp; 64: four warps share the positions)
+    int grid;      // main CTAs
+    size_t desc, stats, part, total;   // scratch offsets
+};
+
+// Query rows sharing a key head, R = max_rows * n_heads / n_kv_heads, choose the shape: blocks of 8 or 16 rows leave all
+// four warps to the positions; more rows share each position's copy among four warps of 16 rows.
+inline PagedAttnPlan plan_paged_attn(const gcuda_paged_kv &kv, const gcuda_paged_batch &b, int n_heads) {
+    PagedAttnPlan p{};
+    const int64_t R = static_cast<int64_t>(b.max_rows) * (n_heads / kv.n_kv_heads);
+    p.rows = R <= 8 ? 8 : R <= 16 ? 16 : 64;
+    // two resident CTAs an SM; no more than there can be tiles of 16 positions
+    const int64_t per_seq = std::max<int64_t>(1, (static_cast<int64_t>(b.max_pages) * kv.page_size + 15) / 16);
+    const int64_t blocks = (R + p.rows - 1) / p.rows;
+    const int64_t most = 2 * static_cast<int64_t>(sm_count());
+    int64_t tiles = per_seq;
+    for (const int64_t f : {static_cast<int64_t>(b.n_seq), static_cast<int64_t>(kv.n_kv_heads), blocks})
+        tiles = std::min(most, tiles * std::min(most, f));   // (capped at each step: no overflow)
+    p.grid = static_cast<int>(std::min(most, tiles));
+    auto take = [&](size_t bytes) {
+        const size_t at = p.total;
+        p.total += (bytes + 255) / 256 * 256;
+        return at;
+    };
+    const size_t slots = 2 * static_cast<size_t>(p.grid);
+    p.desc = take(slots * 16);
+    p.stats = take(slots * p.rows * 16);
+    p.part = take(slots * p.rows * kv.head_dim * 4);
+    return p;
+}
+
+// one per cache type, each in a translation unit of its own
+int launch_paged_attn_i8(const PagedAttnArgs &a, const PagedAttnPlan &p, cudaStream_t st);
+int launch_paged_attn_bf16(const PagedAttnArgs &a, const PagedAttnPlan &p, cudaStream_t st);
+int launch_paged_attn_f16(const PagedAttnArgs &a, const PagedAttnPlan &p, cudaStream_t st);
+
+}  // namespace gcu
