@@ -3,6 +3,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 #include "../../include/geode_cuda.h"
@@ -55,6 +56,28 @@ int by_dim(int hd, F f) {
     return f(std::integral_constant<int, 256>{});
 }
 int launched(cudaError_t e) { return e == cudaSuccess ? GCUDA_OK : GCUDA_E_CUDA; }
+
+template <typename T, int U>
+int launch_adjust_slices(AdjustArgs a, cudaStream_t st) {
+    using P = AdjustShape<T, U>;
+    a.slices = (a.V + P::slice - 1) / P::slice;
+    if (static_cast<int64_t>(a.S) * a.slices > 0x7fffffff) return GCUDA_E_ARG;
+    static std::atomic<uint64_t> opted{0};   // devices whose shared-memory opt-in is done
+    const int dev = current_device();
+    if (dev < 0) return GCUDA_E_CUDA;
+    if (!(opted.load(std::memory_order_relaxed) >> dev & 1)) {
+        if (cudaFuncSetAttribute(k_logits_adjust<T, U>, cudaFuncAttributeMaxDynamicSharedMemorySize, P::smem) != cudaSuccess)
+            return GCUDA_E_CUDA;
+        opted.fetch_or(1ull << dev, std::memory_order_relaxed);
+    }
+    return launched(launch_ex(k_logits_adjust<T, U>, dim3(a.S * a.slices), dim3(kAdjustThreads), P::smem, st, true, a));
+}
+// Slices of four loads a thread where that makes two CTAs an SM or more, of one load otherwise
+template <typename T>
+int launch_adjust(const AdjustArgs &a, cudaStream_t st) {
+    const int64_t wide = static_cast<int64_t>(a.S) * ((a.V + AdjustShape<T, 4>::slice - 1) / AdjustShape<T, 4>::slice);
+    return wide >= 2 * sm_count() ? launch_adjust_slices<T, 4>(a, st) : launch_adjust_slices<T, 1>(a, st);
+}
 
 }  // namespace
 
@@ -115,18 +138,12 @@ int gcuda_op_logits_adjust(const gcuda_logit_rules *r, const void *d_in, void *d
     const int64_t es = static_cast<int64_t>(value_bytes(type)), ib = ((rows - 1) * in_stride + V) * es,
                   ob = ((rows - 1) * out_stride + V) * es;
     if (i0 == o0 ? in_stride != out_stride : (i0 < o0 + ob && o0 < i0 + ib)) return GCUDA_E_ARG;
-    AdjustArgs a{*r, d_in, d_out, S, k, V, 0, 0, in_stride, out_stride, device_status()};
+    AdjustArgs a{*r, d_in, d_out, S, k, V, 0, in_stride, out_stride, device_status()};
     if (!a.status) return GCUDA_E_CUDA;
-    a.slice = 4096;
-    a.slices = (V + a.slice - 1) / a.slice;
-    if (static_cast<int64_t>(S) * a.slices > 0x7fffffff) return GCUDA_E_ARG;
-    const dim3 grid(S * a.slices);
-    const size_t smem = 2 * sizeof(int) * a.slice;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (type == GCUDA_F32) return launched(launch_ex(k_logits_adjust<float>, grid, dim3(kAdjustThreads), smem, st, false, a));
-    if (type == GCUDA_BF16)
-        return launched(launch_ex(k_logits_adjust<__nv_bfloat16>, grid, dim3(kAdjustThreads), smem, st, false, a));
-    return launched(launch_ex(k_logits_adjust<__half>, grid, dim3(kAdjustThreads), smem, st, false, a));
+    if (type == GCUDA_F32) return launch_adjust<float>(a, st);
+    if (type == GCUDA_BF16) return launch_adjust<__nv_bfloat16>(a, st);
+    return launch_adjust<__half>(a, st);
 }
 
 }  // extern "C"

@@ -20,6 +20,7 @@
 #pragma once
 
 #include "paged.cuh"
+#include "paged_attn_plan.hpp"
 
 namespace gcu {
 
@@ -772,46 +773,62 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn(PagedAttnAr
     }
 }
 
-// The parts of each item that was cut, joined: CTA (c, y) does so for the item whose first cut is the start of main CTA
-// c's share - its parts are main CTA c-1's last, then those of c, c+1, .. up to the one that ends it - and the y-th
-// share of its values, a warp for each pair of m tiles of an n tile.
+// The parts of each item that was cut, joined. Main CTA c cuts an item when its share starts inside it; the item's first
+// cut stands for it: its parts are main CTA c-1's last, then the first of c, c+1, .. up to the one that ends it. CTA
+// (i, y) finds the i-th such c among the descriptors (all of them, in one round of loads) and joins the y-th pair of m
+// tiles of an n tile: a warp takes every 8th part, eight in flight, then the warps' sums are joined in shared memory.
+constexpr int kJoinThreads = 256;
+
 template <typename S>
-__global__ void __launch_bounds__(kPagedAttnThreads) k_paged_attn_join(PagedAttnArgs a, int grid) {
-    constexpr int OM = S::OM;
-    const int lane = threadIdx.x & 31, tig = lane & 3, gid = lane >> 2, c = blockIdx.x + 1;
+__global__ void __launch_bounds__(kJoinThreads) k_paged_attn_join(PagedAttnArgs a, int grid) {
+    constexpr int OM = S::OM, W = kJoinThreads / 32;
+    __shared__ uint32_t s_cut[kPagedMaxGrid / 32], s_end[kPagedMaxGrid / 32];
+    __shared__ float4 s_stat[W][2][4], s_v[W][2][32];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, tig = lane & 3, gid = lane >> 2;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;");
-    const int4 here = a.desc[2 * c];
-    const int4 p1 = a.desc[2 * c - 1], p0 = a.desc[2 * c - 2];
-    const int4 prev = (p1.x & kPartHeld) ? p1 : p0;
-    if (!(here.x & kPartHeld) || (here.x & kPartStarts) || !(prev.x & kPartStarts) || (prev.x & kPartEnds)) return;
-    int n = 0;   // parts: slot 2 c - 2 or - 1, then 2 c, 2 c + 2, .. up to the first that ends the item
-    for (int k = c; n == 0; k += 32) {
-        const uint32_t ends = __ballot_sync(0xffffffffu, k + lane >= grid || (a.desc[2 * (k + lane)].x & kPartEnds));
-        if (ends) n = k - c + __ffs(ends) + 1;
+    for (int c0 = 0; c0 < grid; c0 += kJoinThreads) {
+        const int c = c0 + tid;
+        int here = 0, prev = 0;
+        if (c < grid) {
+            here = a.desc[2 * c].x;
+            if (c > 0) prev = a.desc[2 * c - 1].x, prev = prev & kPartHeld ? prev : a.desc[2 * c - 2].x;
+        }
+        const uint32_t cut = __ballot_sync(0xffffffffu, (here & kPartHeld) && !(here & kPartStarts) && (prev & kPartStarts) && !(prev & kPartEnds));
+        const uint32_t end = __ballot_sync(0xffffffffu, c < grid && (here & kPartEnds));
+        if (lane == 0) s_cut[c >> 5] = cut, s_end[c >> 5] = end;
     }
-    const int slot0 = (p1.x & kPartHeld) ? 2 * c - 1 : 2 * c - 2;
+    __syncthreads();
+    const int words = (grid + 31) / 32;
+    int c = -1, left = blockIdx.x;
+    for (int w = 0; w < words; ++w) {
+        uint32_t bits = s_cut[w];
+        const int n = __popc(bits);
+        if (left >= n) {
+            left -= n;
+            continue;
+        }
+        for (; left > 0; --left) bits &= bits - 1;
+        c = 32 * w + __ffs(bits) - 1;
+        break;
+    }
+    if (c < 0) return;
+    int last = c >> 5;   // the CTA that ends the item
+    uint32_t ends = s_end[last] & (0xffffffffu << (c & 31));
+    while (ends == 0 && last + 1 < words) ends = s_end[++last];
+    last = ends ? 32 * last + __ffs(ends) - 1 : grid - 1;
+    const int n = last - c + 2;
+    const int4 item = a.desc[2 * c];
+    const int slot0 = 2 * c - 1 - ((a.desc[2 * c - 1].x & kPartHeld) ? 0 : 1);
     auto slot = [&](int k) { return static_cast<int64_t>(k == 0 ? slot0 : 2 * (c + k - 1)); };
-    const int unit = blockIdx.y * (kPagedAttnThreads / 32) + (threadIdx.x >> 5);   // (n tile, pair of m tiles)
-    if (unit >= S::NTT * OM / 2) return;
-    const int nt = unit / (OM / 2), k2 = unit % (OM / 2) * 2;
-    const int G = a.x.n_heads / a.kv.n_kv_heads, R = here.w * G, nrb = (R + S::kRows - 1) / S::kRows;
-    if (here.y % nrb * S::kRows + 8 * nt >= R) return;
+    const int nt = blockIdx.y / (OM / 2), k2 = blockIdx.y % (OM / 2) * 2;
+    const int G = a.x.n_heads / a.kv.n_kv_heads, R = item.w * G, nrb = (R + S::kRows - 1) / S::kRows;
+    if (item.y % nrb * S::kRows + 8 * nt >= R) return;
     constexpr int B = 8;   // parts whose loads are in flight together
     float M[2] = {-INFINITY, -INFINITY}, Mo[2] = {-INFINITY, -INFINITY}, L[2] = {0.0f, 0.0f};
     float4 v[2] = {make_float4(0.0f, 0.0f, 0.0f, 0.0f), make_float4(0.0f, 0.0f, 0.0f, 0.0f)};
-    for (int k0 = 0; k0 < n; k0 += B) {
-        float4 st[B][2], x[B][2];
-#pragma unroll
-        for (int b = 0; b < B; ++b) {
-            const bool in = k0 + b < n;
-            const int64_t s = slot(in ? k0 + b : 0);
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                st[b][h] = in ? a.stats[s * S::kRows + 8 * nt + 2 * tig + h] : make_float4(-INFINITY, 0.0f, -INFINITY, 0.0f);
-                x[b][h] = in ? a.part[((s * S::NTT + nt) * OM + k2 + h) * 32 + lane] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            }
-        }
+    // parts or warps b = 0 .. n-1 of (stats of the lane's two rows, values of two m tiles) into M, Mo, L, v
+    auto take = [&](const float4 (&st)[B][2], const float4 (&x)[B][2]) {
         float f0[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -836,11 +853,40 @@ __global__ void __launch_bounds__(kPagedAttnThreads) k_paged_attn_join(PagedAttn
 #pragma unroll
             for (int h = 0; h < 2; ++h) v[h].x += x[b][h].x * f[0], v[h].y += x[b][h].y * f[1], v[h].z += x[b][h].z * f[0], v[h].w += x[b][h].w * f[1];
         }
+    };
+    float4 st[B][2], x[B][2];
+    for (int k0 = warp; k0 < n; k0 += W * B) {
+#pragma unroll
+        for (int b = 0; b < B; ++b) {
+            const bool in = k0 + b * W < n;
+            const int64_t at = slot(in ? k0 + b * W : 0);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                st[b][h] = in ? a.stats[at * S::kRows + 8 * nt + 2 * tig + h] : make_float4(-INFINITY, 0.0f, -INFINITY, 0.0f);
+                x[b][h] = in ? a.part[((at * S::NTT + nt) * OM + k2 + h) * 32 + lane] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            }
+        }
+        take(st, x);
     }
-    write_out<S>(a, here.z, here.w, here.y, nt, k2, v[0], v[1], row_factor(M[0], L[0], Mo[0]), row_factor(M[1], L[1], Mo[1]));
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        s_v[warp][h][lane] = v[h];
+        if (gid == 0) s_stat[warp][h][tig] = make_float4(M[h], L[h], Mo[h], 0.0f);
+    }
+    __syncthreads();
+    if (warp != 0) return;
+    static_assert(W == B, "the warps' sums are one batch");
+#pragma unroll
+    for (int b = 0; b < B; ++b)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) st[b][h] = s_stat[b][h][tig], x[b][h] = s_v[b][h][lane];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) M[h] = Mo[h] = -INFINITY, L[h] = 0.0f, v[h] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    take(st, x);
+    write_out<S>(a, item.z, item.w, item.y, nt, k2, v[0], v[1], row_factor(M[0], L[0], Mo[0]), row_factor(M[1], L[1], Mo[1]));
     if (k2 == 0 && gid == 0)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) write_lse<S>(a, here.z, here.w, here.y, 8 * nt + 2 * tig + h, M[h], L[h]);
+        for (int h = 0; h < 2; ++h) write_lse<S>(a, item.z, item.w, item.y, 8 * nt + 2 * tig + h, M[h], L[h]);
 }
 
 }  // namespace gcu

@@ -11,7 +11,8 @@
 namespace gcu {
 
 template <typename S>
-int launch_paged_shape(const PagedAttnArgs &a, int grid, cudaStream_t st) {
+int launch_paged_shape(const PagedAttnArgs &a, const PagedAttnPlan &p, cudaStream_t st) {
+    const int grid = p.grid;
     static std::atomic<uint64_t> opted{0};   // devices whose shared-memory opt-in is done
     const int dev = current_device();
     if (dev < 0) return GCUDA_E_CUDA;
@@ -21,18 +22,17 @@ int launch_paged_shape(const PagedAttnArgs &a, int grid, cudaStream_t st) {
         opted.fetch_or(1ull << dev, std::memory_order_relaxed);
     }
     if (launch_ex(k_paged_attn<S>, dim3(grid), dim3(kPagedAttnThreads), S::kSmem, st, true, a) != cudaSuccess) return GCUDA_E_CUDA;
-    if (grid == 1) return GCUDA_OK;
-    const int units = (S::NTT * S::OM / 2 + 3) / 4;
-    return launch_ex(k_paged_attn_join<S>, dim3(grid - 1, units), dim3(kPagedAttnThreads), 0, st, true, a, grid) == cudaSuccess
+    if (grid == 1) return GCUDA_OK;   // (nothing is cut)
+    return launch_ex(k_paged_attn_join<S>, dim3(p.cuts, S::NTT * S::OM / 2), dim3(kJoinThreads), 0, st, true, a, grid) == cudaSuccess
                ? GCUDA_OK
                : GCUDA_E_CUDA;
 }
 
 template <int CACHE, int HD, bool SPLIT>
 int launch_paged_rows(const PagedAttnArgs &a, const PagedAttnPlan &p, cudaStream_t st) {
-    if (p.rows == 8) return launch_paged_shape<PagedShape<HD, CACHE, SPLIT, 1, 1>>(a, p.grid, st);
-    if (p.rows == 16) return launch_paged_shape<PagedShape<HD, CACHE, SPLIT, 2, 1>>(a, p.grid, st);
-    return launch_paged_shape<PagedShape<HD, CACHE, SPLIT, 2, 4>>(a, p.grid, st);
+    if (p.rows == 8) return launch_paged_shape<PagedShape<HD, CACHE, SPLIT, 1, 1>>(a, p, st);
+    if (p.rows == 16) return launch_paged_shape<PagedShape<HD, CACHE, SPLIT, 2, 1>>(a, p, st);
+    return launch_paged_shape<PagedShape<HD, CACHE, SPLIT, 2, 4>>(a, p, st);
 }
 template <int CACHE, int HD>
 int launch_paged_split(const PagedAttnArgs &a, const PagedAttnPlan &p, cudaStream_t st) {

@@ -7,10 +7,13 @@
 
 namespace gcu {
 
+constexpr int kPagedMaxGrid = 2048;   // main CTAs (the join keeps a bit for each)
+
 struct PagedAttnArgs;
 struct PagedAttnPlan {
     int rows;      // query rows of a block (8, 16: position groups of one warp; 64: four warps share the positions)
     int grid;      // main CTAs
+    int cuts;      // items that their shares can cut, at most
     size_t desc, stats, part, total;   // scratch offsets
 };
 
@@ -23,11 +26,12 @@ inline PagedAttnPlan plan_paged_attn(const gcuda_paged_kv &kv, const gcuda_paged
     // two resident CTAs an SM; no more than there can be tiles of 16 positions
     const int64_t per_seq = std::max<int64_t>(1, (static_cast<int64_t>(b.max_pages) * kv.page_size + 15) / 16);
     const int64_t blocks = (R + p.rows - 1) / p.rows;
-    const int64_t most = 2 * static_cast<int64_t>(sm_count());
-    int64_t tiles = per_seq;
+    const int64_t most = std::min<int64_t>(kPagedMaxGrid, 2 * static_cast<int64_t>(sm_count()));
+    int64_t items = 1;
     for (const int64_t f : {static_cast<int64_t>(b.n_seq), static_cast<int64_t>(kv.n_kv_heads), blocks})
-        tiles = std::min(most, tiles * std::min(most, f));   // (capped at each step: no overflow)
-    p.grid = static_cast<int>(std::min(most, tiles));
+        items = std::min(most, items * std::min(most, f));   // (capped at each step: no overflow)
+    p.grid = static_cast<int>(std::min(most, items * std::min(most, per_seq)));
+    p.cuts = static_cast<int>(std::min<int64_t>(items, p.grid - 1));
     auto take = [&](size_t bytes) {
         const size_t at = p.total;
         p.total += (bytes + 255) / 256 * 256;
