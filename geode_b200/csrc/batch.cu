@@ -113,7 +113,7 @@ int gcuda_op_paged_attn(const gcuda_paged_kv *kv, const gcuda_paged_batch *b, co
     if (need == 0 || work_bytes < need) return GCUDA_E_ARG;
     const PagedAttnPlan p = plan_paged_attn(*kv, *b, x->n_heads);
     uint8_t *w = static_cast<uint8_t *>(d_work);
-    const PagedAttnArgs a{*kv, *b, *x, device_status(), reinterpret_cast<int4 *>(w + p.desc),
+    const PagedAttnArgs a{*kv, *b, *x, device_status(), reinterpret_cast<int4 *>(w + p.cut),
                           reinterpret_cast<float4 *>(w + p.stats), reinterpret_cast<float4 *>(w + p.part)};
     if (!a.status) return GCUDA_E_CUDA;
     cudaStream_t st = static_cast<cudaStream_t>(stream);

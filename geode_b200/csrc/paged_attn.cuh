@@ -2,9 +2,10 @@
 //
 // An item is one (sequence, key head, block of query rows): the sequence's T rows times the G query heads that share the
 // key head, R = T * G rows in blocks of kRows. Items are cut into tiles of positions and the tiles of all items, laid end
-// to end, are dealt out evenly to the resident CTAs (each CTA finds its share by a scan over the lengths on the device:
-// whatever the lengths, every CTA reads the same number of tiles). What a CTA holds of an item that it does not finish
-// goes to the scratch and k_paged_attn_join adds the parts up.
+// to end with a few tiles' time for each item's beginning, are dealt out evenly to the resident CTAs (each CTA finds its
+// share by a scan over the lengths on the device: whatever the lengths, every CTA has the same work). What a CTA holds
+// of an item that it does not finish goes to the scratch and k_paged_attn_join adds the parts up. The copies run ahead
+// of the products across tiles and items alike, so memory is not left idle while an item ends and the next begins.
 //
 // Both products run on the tensor cores (mma.sync m16n8k16, float sums) with the cache as the 16-row operand and the
 // query rows as the 8-column one, so that one token's few rows fill the instruction: S^T = K Q^T, then O^T = V^T P^T.
@@ -29,38 +30,43 @@ struct PagedAttnArgs {
     gcuda_paged_batch b;
     gcuda_attn_rows x;
     uint32_t *status;
-    int4 *desc;      // [grid][2] the parts that CTAs left: {flags, item, first row, rows}
+    int4 *cut;       // [grid] the item that CTA c began and did not finish: {2 parts + the slot of c's own, item, first row, rows}
     float4 *stats;   // [grid][2][kRows] {m, l, m', -} of each row
     float4 *part;    // [grid][2][n tile][m tile][lane]
 };
 
 constexpr int kPagedAttnThreads = 128;
-constexpr int kPartHeld = 1, kPartStarts = 2, kPartEnds = 4;   // desc flags
 constexpr float kWeightBias = 14.0f;   // f16 weights reach up to 2^14: the smallest kept is 2^-39 of the largest
 
 // Shapes of one instantiation. NT: n tiles (8 query rows) a warp; WR: warps that share the positions (each with its own
-// rows; the CTA's other factor, 4 / WR, takes positions).
+// rows; the CTA's other factor, 4 / WR, takes positions). An entry of the ring is a tile's K or V rows, at most 256 bytes
+// of each (longer rows: in parts).
 template <int HD_, int CACHE_, bool SPLIT_, int NT_, int WR_>
 struct PagedShape {
     static constexpr int HD = HD_, CACHE = CACHE_, NT = NT_, WR = WR_;
     static constexpr bool SPLIT = SPLIT_, I8 = CACHE == GCUDA_I8, BF16 = CACHE == GCUDA_BF16;
     static constexpr int WP = 4 / WR;
     static constexpr int ES = I8 ? 1 : 2, RB = HD * ES;          // bytes of a value, of a row
-    static constexpr int MT = RB <= 128 || (RB == 256 && NT == 1) ? 2 : 1, TP = 16 * MT;   // positions of a warp's tile
+    static constexpr int RE = RB < 256 ? RB : 256, PARTS = RB / RE;
+    static constexpr int MT = RB <= 128 ? 2 : 1, TP = 16 * MT;    // positions of a warp's tile
     static constexpr int CT = TP * WP;                            // of a CTA's
+    // an item's beginning and end cost about what 64 KB of rows do
+    static constexpr int kItemCost = 65536 / (2 * CT * RB) > 0 ? 65536 / (2 * CT * RB) : 1;
     static constexpr int NTT = NT * WR, kRows = 8 * NTT;
     static constexpr int KS = HD / 16, OM = HD / 16;
-    static constexpr int kEntry = TP * RB;                        // a tile's K or V rows in shared memory
-    static constexpr int kRing = (WR > 1 ? 40 : NT == 1 || RB == 512 ? 24 : 20) * 1024;   // bytes of a position group's ring
+    static constexpr int kEntry = TP * RE;
+    static constexpr int kRing = (WR > 1 ? 40 : NT == 1 ? 16 : 12) * 1024;      // bytes of a position group's ring
     static constexpr int E = kRing / kEntry < 12 ? kRing / kEntry : 12;
-    static constexpr int kScale = 2 * TP * 4 + 16;                // a slot's scales and valid bits
+    static constexpr int TS = E / (2 * PARTS) + 2;                // tiles whose scales and valid bits are kept
+    static constexpr int kScale = (I8 ? 2 * TP * 4 : 0) + 16;
     static constexpr int kQ = KS * NTT * 32 * 8 * (SPLIT ? 2 : 1);
-    static constexpr int kJoin = WR == 1 ? 4 * NT * OM * 32 * 16 : 0;   // (over the ring, drained)
-    static constexpr int kRings = WP * E * kEntry > kJoin ? WP * E * kEntry : kJoin;
-    static constexpr int o_q = 0, o_ring = o_q + kQ, o_scale = o_ring + kRings;
-    static constexpr int o_col = o_scale + WP * E * kScale;       // [kRows] column factor
-    static constexpr int o_join = o_col + kRows * 4;              // [4][kRows] m, l, m' of each position group
-    static constexpr int kSmem = o_join + (WR == 1 ? 4 * kRows * 16 : 0);
+    static constexpr int o_q = 0, o_ring = o_q + kQ, o_scale = o_ring + WP * E * kEntry;
+    static constexpr int o_col = o_scale + WP * TS * kScale;      // [kRows] column factor
+    static constexpr int o_seg = o_col + kRows * 4;               // [warp][kSegs] segments looked up, not yet done
+    static constexpr int kSegs = E / (2 * PARTS) + 5;
+    static constexpr int o_stat = o_seg + 4 * kSegs * 48;         // [4][kRows] m, l, m' of each position group
+    static constexpr int o_join = o_stat + (WR == 1 ? 4 * kRows * 16 : 0);   // [group][m tile][lane] O of an n tile
+    static constexpr int kSmem = o_join + (WR == 1 ? 4 * OM * 32 * 16 : 0);
     static_assert(E >= 3, "two entries in flight");
 };
 
@@ -187,18 +193,28 @@ __device__ __forceinline__ int seq_tiles(const PagedAttnArgs &a, const SeqRows &
     lo = a.x.window > 0 ? max(0, q.length - q.rows + 1 - a.x.window) : 0;
     return max(1, (q.length - lo + S::CT - 1) / S::CT);
 }
+// a sequence's share of the work: for each of its items the beginning's cost and the tiles
 template <typename S>
-__device__ __forceinline__ int64_t all_tiles(const PagedAttnArgs &a, const SeqRows &q) {
+__device__ __forceinline__ int64_t seq_cost(const PagedAttnArgs &a, const SeqRows &q) {
     if (q.rows == 0) return 0;
     int lo;
-    const int64_t t = seq_tiles<S>(a, q, lo);
+    const int64_t t = S::kItemCost + seq_tiles<S>(a, q, lo);
     return t * a.kv.n_kv_heads * ((q.rows * (a.x.n_heads / a.kv.n_kv_heads) + S::kRows - 1) / S::kRows);
 }
 
+struct PagedSegment {   // what a CTA does of one item (48 bytes)
+    int r0, rows, length;
+    int lo, tps;        // the item's first position and tiles
+    int item, t0, n;    // the item within its sequence; this CTA's tiles
+    int parts;          // the CTAs that share the item, where it begins here and ends elsewhere (else 0)
+    int no;             // how many segments came before it in this CTA
+    int kh, rb;         // its key head, its block of rows
+};
+
 template <typename S>
 __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn(PagedAttnArgs a) {
-    constexpr int HD = S::HD, NT = S::NT, WR = S::WR, TP = S::TP, MT = S::MT, RB = S::RB, E = S::E, OM = S::OM;
-    constexpr int A = E / 2 + 1;   // tiles whose pages are looked up ahead
+    constexpr int HD = S::HD, NT = S::NT, WR = S::WR, TP = S::TP, MT = S::MT, RB = S::RB, RE = S::RE, E = S::E, OM = S::OM;
+    constexpr int PARTS = S::PARTS, KPC = S::I8 ? 4 : 2;   // (k steps of a 16-byte piece)
     constexpr bool I8 = S::I8, BF16 = S::BF16, SPLIT = S::SPLIT;
     extern __shared__ __align__(128) uint8_t sm[];
     __shared__ int64_t s_sum[4], s_base;
@@ -209,12 +225,12 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn(PagedAttnAr
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;");
 
-    // this CTA's share [u, end) of all tiles: each thread sums a run of sequences, then a scan over the threads
-    if (tid < 2) a.desc[2 * cta + tid] = make_int4(0, 0, 0, 0);
+    // this CTA's share [begin, end) of all work: each thread sums a run of sequences, then a scan over the threads
+    if (tid == 0) a.cut[cta] = make_int4(0, 0, 0, 0);
     const int run = (a.b.n_seq + kPagedAttnThreads - 1) / kPagedAttnThreads;
     const int s_lo = min(tid * run, a.b.n_seq), s_hi = min(s_lo + run, a.b.n_seq);
     int64_t mine = 0;
-    for (int s = s_lo; s < s_hi; ++s) mine += all_tiles<S>(a, seq_rows(a.b, a.kv.page_size, s, a.status));
+    for (int s = s_lo; s < s_hi; ++s) mine += seq_cost<S>(a, seq_rows(a.b, a.kv.page_size, s, a.status));
     int64_t before = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -237,7 +253,7 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn(PagedAttnAr
         int64_t base = before;
         int s = s_lo;
         for (; s < s_hi; ++s) {
-            const int64_t n = all_tiles<S>(a, seq_rows(a.b, a.kv.page_size, s, a.status));
+            const int64_t n = seq_cost<S>(a, seq_rows(a.b, a.kv.page_size, s, a.status));
             if (begin < base + n) break;
             base += n;
         }
@@ -245,96 +261,170 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn(PagedAttnAr
         s_base = base;
     }
     __syncthreads();
-    int seq = s_seq;
-    int64_t base = s_base, u = begin;
 
     uint2 *q_hi = reinterpret_cast<uint2 *>(sm + S::o_q);       // fragments (b0, b1) [k step][n tile][lane]; SPLIT: uint4
     uint4 *q_both = reinterpret_cast<uint4 *>(sm + S::o_q);
     float *col_s = reinterpret_cast<float *>(sm + S::o_col);
-    float4 *join_s = reinterpret_cast<float4 *>(sm + S::o_join);
     uint8_t *ring = sm + S::o_ring + wp * E * S::kEntry;
-    uint8_t *scales = sm + S::o_scale + wp * E * S::kScale;
+    uint8_t *scales = sm + S::o_scale + wp * S::TS * S::kScale;
+    PagedSegment *segs = reinterpret_cast<PagedSegment *>(sm + S::o_seg) + warp * S::kSegs;
     const uint32_t ring_a = smem_addr(ring), scales_a = smem_addr(scales);
-    const uint8_t *kb = static_cast<const uint8_t *>(a.kv.k), *vb = static_cast<const uint8_t *>(a.kv.v);
 
-    while (u < end) {
-        const SeqRows q = seq_rows(a.b, a.kv.page_size, seq, a.status);
-        if (q.rows == 0) {
+    // ---- looking ahead: the next tile of this CTA's share, and the page of this lane's position in it. A warp does this
+    // for itself (all alike); the segments it opens wait in shared memory until the products reach them. The following
+    // sequence's plan is loaded a sequence ahead.
+    int seq = s_seq, opened = 0;
+    int64_t base = s_base, u = begin;
+    auto load_seq = [&](int s) { return s < a.b.n_seq ? seq_rows(a.b, a.kv.page_size, s, a.status) : SeqRows{0, 0, 0}; };
+    SeqRows sq = load_seq(seq), sq_next = load_seq(seq + 1);
+    int at_p0 = 0, at_n = 0, at_length = 0, at_kh = 0;   // the segment being looked up: next tile's position, tiles left
+    const int *at_pages = nullptr;
+    auto open = [&]() {   // the next segment with tiles (none left: at_n 0)
+        while (at_n == 0 && u < end) {
+            if (sq.rows > 0) {
+                PagedSegment g;
+                g.r0 = sq.r0, g.rows = sq.rows, g.length = sq.length;
+                g.tps = seq_tiles<S>(a, sq, g.lo);
+                const int nrb = (sq.rows * G + S::kRows - 1) / S::kRows, per = S::kItemCost + g.tps;
+                const int64_t off = u - base;
+                g.item = static_cast<int>(off / per);
+                const int o = static_cast<int>(off % per), n = static_cast<int>(min(static_cast<int64_t>(per - o), end - u));
+                g.t0 = max(0, o - S::kItemCost);
+                g.n = max(0, o + n - S::kItemCost) - g.t0;
+                // (the CTA that holds the item's last tile, by the shares' own division)
+                g.parts = g.t0 == 0 && g.n < g.tps ? static_cast<int>(((u - o + per) * ctas - 1) / total) - cta + 1 : 0;
+                g.no = opened;
+                g.kh = g.item / nrb;
+                g.rb = g.item % nrb;
+                if (g.n > 0) {
+                    at_n = g.n;
+                    at_p0 = g.lo + g.t0 * S::CT + wp * TP;
+                    at_length = g.length;
+                    at_kh = g.kh;
+                    at_pages = a.b.pages + seq * a.b.pages_stride;
+                    if (lane == 0) segs[opened % S::kSegs] = g;
+                    ++opened;
+                }
+                u += n;
+                if (u - base < static_cast<int64_t>(per) * a.kv.n_kv_heads * nrb) continue;
+                base = u;
+            }
             ++seq;
-            continue;
+            sq = sq_next;
+            sq_next = load_seq(seq + 1);
         }
-        int lo;
-        const int tps = seq_tiles<S>(a, q, lo), R = q.rows * G, nrb = (R + S::kRows - 1) / S::kRows;
-        const int item = static_cast<int>((u - base) / tps), t0 = static_cast<int>((u - base) % tps);
-        const int t1 = static_cast<int>(min(static_cast<int64_t>(tps), t0 + (end - u)));
-        const int kh = item / nrb, rb = item % nrb;
-        const int *pages = a.b.pages + seq * a.b.pages_stride;
+    };
+    struct Tile {
+        int page;    // of this lane's position (-2: it has none)
+        int p0;      // the tile's first position (-1: no tile)
+        int kh;
+    };
+    auto look = [&]() {
+        open();
+        if (at_n == 0) return Tile{-2, -1, 0};
+        Tile t{-2, at_p0, at_kh};
+        const int p = at_p0 + lane;
+        if (lane < TP && p < at_length) t.page = at_pages[p / a.kv.page_size];
+        at_p0 += S::CT;
+        --at_n;
+        return t;
+    };
+    Tile ahead0 = look(), ahead1 = look();
 
-        // ---- the copies: entry 2 i is tile i's K rows, entry 2 i + 1 its V rows; a lane knows one position's place
-        const int n_tiles = t1 - t0, first = lo + t0 * S::CT + wp * TP;   // this group's first position
-        int64_t place = 0;    // value offset of this lane's position (of the tile whose K was last issued)
-        bool there = false;
-        int page[A] = {};     // the pages of this lane's positions in the tiles whose K is issued next
-        auto load_page = [&](int i) {
-            const int p = first + i * S::CT + lane;
-            return (i < n_tiles && lane < TP && p < q.length) ? pages[p / a.kv.page_size] : -1;
-        };
-        auto issue = [&](int e) {
-            if (e < 2 * n_tiles) {
-                const int slot = e % E, i = e >> 1;
-                if (!(e & 1)) {
-                    const int p = first + i * S::CT + lane;
-                    const int pg = page[0];
-#pragma unroll
-                    for (int k = 0; k + 1 < A; ++k) page[k] = page[k + 1];
-                    page[A - 1] = load_page(i + A);
-                    there = pg >= 0 && pg < a.kv.n_pages;
-                    if (lane < TP && p < q.length && !there) atomicOr(a.status, kErrBadShape);
-                    const int ip = p % a.kv.page_size;
-                    place = there ? pg * a.kv.page_stride + ip * a.kv.pos_stride + kh * a.kv.head_stride : 0;
-                    const uint32_t bits = __ballot_sync(0xffffffffu, there);
-                    if (wr == 0) {
-                        uint8_t *sc = scales + slot * S::kScale;
-                        if (lane == 0) *reinterpret_cast<uint32_t *>(sc + 2 * TP * 4) = bits;
-                        if constexpr (I8) {
-                            if (lane < TP) {
-                                const int64_t sp = there ? pg * a.kv.scale_page_stride + ip * a.kv.scale_pos_stride + kh * a.kv.scale_head_stride : 0;
-                                const uint32_t d = scales_a + slot * S::kScale + lane * 4;
-                                copy4(d, a.kv.k_scale + sp, there ? 4 : 0);
-                                copy4(d + TP * 4, a.kv.v_scale + sp, there ? 4 : 0);
-                            }
+    // ---- the copies: entry by entry through the tiles looked up (K's parts, then V's)
+    int in_slot = 0, in_entry = 0, in_tile = 0;   // the ring slot, the entry within its tile, the tile's place among scales
+    bool in_any = true, there = false, one_page = false;
+    int64_t place = 0;    // value offset of this lane's position
+    uint32_t ok = 0;      // the tile's positions that are on a page
+    auto issue = [&]() {
+        if (in_entry == 0 && in_any) {
+            const Tile t = ahead0;
+            ahead0 = ahead1;
+            ahead1 = look();
+            in_any = t.p0 >= 0;
+            if (in_any) {
+                there = t.page >= 0 && t.page < a.kv.n_pages;
+                if (t.page != -2 && !there) atomicOr(a.status, kErrBadShape);
+                const int ip = (t.p0 + lane) % a.kv.page_size;
+                place = there ? t.page * a.kv.page_stride + ip * a.kv.pos_stride + t.kh * a.kv.head_stride : 0;
+                ok = __ballot_sync(0xffffffffu, there);
+                // positions one after the other on one page: their rows are pos_stride apart
+                const int ip0 = __shfl_sync(0xffffffffu, ip, 0);
+                one_page = ok == static_cast<uint32_t>((1ull << TP) - 1) && ip0 + TP <= a.kv.page_size;
+                if (wr == 0) {
+                    const uint32_t d = scales_a + in_tile * S::kScale;
+                    if (lane == 0) *reinterpret_cast<uint32_t *>(scales + in_tile * S::kScale) = ok;
+                    if constexpr (I8) {
+                        if (lane < TP) {
+                            const int64_t sp = there ? t.page * a.kv.scale_page_stride + ip * a.kv.scale_pos_stride + t.kh * a.kv.scale_head_stride : 0;
+                            copy4(d + 16 + lane * 4, a.kv.k_scale + sp, there ? 4 : 0);
+                            copy4(d + 16 + (TP + lane) * 4, a.kv.v_scale + sp, there ? 4 : 0);
                         }
                     }
                 }
-                const uint8_t *src = (e & 1) ? vb : kb;
-                constexpr int CH = RB / 16;   // 16-byte pieces of a row
-                const uint32_t ok = __ballot_sync(0xffffffffu, there);
+            }
+        }
+        if (in_any) {
+            const bool is_v = in_entry >= PARTS;
+            const uint8_t *src = static_cast<const uint8_t *>(is_v ? a.kv.v : a.kv.k) + (in_entry - (is_v ? PARTS : 0)) * RE;
+            constexpr int CH = RE / 16, PR = 32 / CH;   // 16-byte pieces of a row, rows of a warp's copy
+            const int c = lane % CH;
+            const uint32_t dst = ring_a + in_slot * S::kEntry;
+            // pieces swapped within a row so that the fragment loads of K (8 rows x 4 neighbouring pieces) and of V (every
+            // second row x 2 pieces) meet no bank twice
+            auto put = [&](int k, const uint8_t *from, uint32_t bytes) {
+                const int p = (k * WR + wr) * PR + lane / CH;
+                int sw;
+                if (is_v) sw = RE == 64 ? c ^ ((p >> 1 & 1) << 1) : c ^ ((p >> 1 & 3) << 1);
+                else sw = RE == 64 ? c : c ^ ((p & 1) << 2);
+                copy16(dst + p * RE + sw * 16, from, bytes);
+            };
+            constexpr int N = TP * CH / (32 * WR);
+            if (one_page) {
+                const int64_t first = __shfl_sync(0xffffffffu, place, 0), step = a.kv.pos_stride * S::ES;
+                const uint8_t *from = src + first * S::ES + (wr * PR + lane / CH) * step + c * 16;
 #pragma unroll
-                for (int k = 0; k < TP * CH / (32 * WR); ++k) {
-                    const int idx = (k * WR + wr) * 32 + lane, p = idx / CH, c = idx % CH;
-                    const int64_t at = __shfl_sync(0xffffffffu, place, p);
-                    // pieces swapped within a row so that the fragment loads of K (8 rows x 4 pieces of 4 neighbouring
-                    // lanes) and of V (every second row x 2 pieces) meet no bank twice
-                    int sw;
-                    if (e & 1) sw = RB == 64 ? c ^ ((p >> 1 & 1) << 1) : c ^ ((p >> 1 & 3) << 1);
-                    else sw = RB == 64 ? c : c ^ ((p & 1) << 2);
-                    copy16(ring_a + slot * S::kEntry + p * RB + sw * 16, src + at * S::ES + c * 16, (ok >> p & 1) ? 16 : 0);
+                for (int k = 0; k < N; ++k) put(k, from, 16), from += step * (PR * WR);
+            } else {
+#pragma unroll
+                for (int k = 0; k < N; ++k) {
+                    const int p = (k * WR + wr) * PR + lane / CH;
+                    const int64_t x = __shfl_sync(0xffffffffu, place, p);
+                    put(k, src + x * S::ES + c * 16, (ok >> p & 1) ? 16 : 0);
                 }
             }
-            asm volatile("cp.async.commit_group;" ::: "memory");
-        };
-#pragma unroll
-        for (int k = 0; k < A; ++k) page[k] = load_page(k);
-        __syncthreads();   // the last segment's shared memory is free
-#pragma unroll
-        for (int e = 0; e < E - 1; ++e) issue(e);
+            if (++in_entry == 2 * PARTS) {
+                in_entry = 0;
+                in_tile = in_tile + 1 == S::TS ? 0 : in_tile + 1;
+            }
+        }
+        in_slot = in_slot + 1 == E ? 0 : in_slot + 1;
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll 1
+    for (int e = 0; e < E - 1; ++e) issue();
+    __syncwarp();   // (the first segments are written)
 
+    int slot = 0, tile_at = 0;   // the products' place in the ring and among the scales
+    auto next_entry = [&]() {    // the entry at `slot` has landed, and the one before it is free for a new copy
+        asm volatile("cp.async.wait_group %0;" ::"n"(E - 2) : "memory");
+        if constexpr (WR == 1) __syncwarp();
+        else __syncthreads();
+        issue();
+        const uint8_t *ent = ring + slot * S::kEntry;
+        slot = slot + 1 == E ? 0 : slot + 1;
+        return ent;
+    };
+
+    for (int done = 0; done < opened; ++done) {
+        const PagedSegment g = segs[done % S::kSegs];
+        const int R = g.rows * G;
         // ---- the queries as fragments: warp w takes rows w, w + 4, ..; lane HD / 32 neighbouring dims
         for (int i = warp; i < S::kRows; i += 4) {
             constexpr int N = HD / 32;
-            const int r = rb * S::kRows + i;
+            const int r = g.rb * S::kRows + i;
             float v[N], top = 0.0f;
-            const int64_t at = r < R ? static_cast<int64_t>(q.r0 + r / G) * a.x.q_stride + static_cast<int64_t>(kh * G + r % G) * a.x.q_head_stride + lane * N : 0;
+            const int64_t at = r < R ? static_cast<int64_t>(g.r0 + r / G) * a.x.q_stride + static_cast<int64_t>(g.kh * G + r % G) * a.x.q_head_stride + lane * N : 0;
 #pragma unroll
             for (int k = 0; k < N; ++k) v[k] = r < R ? load_act(a.x.q, a.x.type, at + k) : 0.0f;
             int ex = 0;
@@ -374,16 +464,16 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn(PagedAttnAr
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                const int i = 8 * (wr * NT + nt) + 2 * tig + c, r = rb * S::kRows + i;
+                const int i = 8 * (wr * NT + nt) + 2 * tig + c, r = g.rb * S::kRows + i;
                 col[nt][c] = col_s[i];
-                lim[nt][c] = r < R ? q.length - q.rows + r / G : -1;
+                lim[nt][c] = r < R ? g.length - g.rows + r / G : -1;
                 m[nt][c] = mo[nt][c] = -INFINITY;
                 l[nt][c] = 0.0f;
             }
         // rows of this block: all see [all_lo, all_hi]
-        const int t_first = rb * S::kRows / G, t_last = (min(R, (rb + 1) * S::kRows) - 1) / G;
-        const int all_hi = q.length - q.rows + t_first;
-        const int all_lo = a.x.window > 0 ? q.length - q.rows + t_last + 1 - a.x.window : 0;
+        const int t_first = g.rb * S::kRows / G, t_last = (min(R, (g.rb + 1) * S::kRows) - 1) / G;
+        const int all_hi = g.length - g.rows + t_first;
+        const int all_lo = a.x.window > 0 ? g.length - g.rows + t_last + 1 - a.x.window : 0;
         float o[OM][NT][4];
 #pragma unroll
         for (int k = 0; k < OM; ++k)
@@ -391,19 +481,13 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn(PagedAttnAr
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int c = 0; c < 4; ++c) o[k][nt][c] = 0.0f;
-        const bool busy = rb * S::kRows + 8 * wr * NT < R;   // this warp has rows
+        const bool busy = g.rb * S::kRows + 8 * wr * NT < R;   // this warp has rows
 
-        uint32_t ph[MT][NT][2], pl[MT][NT][2];   // the weights as fragments: (b0, b1), and what is left of them
-        bool edge = false;
-        for (int e = 0; e < 2 * n_tiles; ++e) {
-            asm volatile("cp.async.wait_group %0;" ::"n"(E - 2) : "memory");
-            if constexpr (WR == 1) __syncwarp();
-            else __syncthreads();
-            issue(e + E - 1);
-            if (!busy) continue;
-            const int slot = e % E, p0 = first + (e >> 1) * S::CT;
-            const uint8_t *ent = ring + slot * S::kEntry;
-            if (!(e & 1)) {
+        for (int i = 0; i < g.n; ++i) {
+            const int p0 = g.lo + (g.t0 + i) * S::CT + wp * TP;
+            uint32_t ph[MT][NT][2], pl[MT][NT][2];   // the weights as fragments: (b0, b1), and what is left of them
+            bool edge;
+            {
                 // ---- S^T = K Q^T
                 float s[MT][NT][4], s2[MT][NT][4];
 #pragma unroll
@@ -413,51 +497,58 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn(PagedAttnAr
 #pragma unroll
                         for (int c = 0; c < 4; ++c) s[mt][nt][c] = s2[mt][nt][c] = 0.0f;
 #pragma unroll
-                for (int j = 0; j < RB / 64; ++j) {
-                    uint4 kg[MT][2];
+                for (int part = 0; part < PARTS; ++part) {
+                    const uint8_t *ent = next_entry();
+                    if (!busy) continue;
 #pragma unroll
-                    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            const int p = 16 * mt + 8 * h + gid, c = 4 * j + tig, sw = RB == 64 ? c : c ^ ((p & 1) << 2);
-                            kg[mt][h] = *reinterpret_cast<const uint4 *>(ent + p * RB + sw * 16);
-                        }
-#pragma unroll
-                    for (int w = 0; w < (I8 ? 4 : 2); ++w) {
-                        const int ks = j * (I8 ? 4 : 2) + w;
-                        uint32_t ka[MT][4];
+                    for (int j = 0; j < RE / 64; ++j) {
+                        uint4 kg[MT][2];
 #pragma unroll
                         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
                             for (int h = 0; h < 2; ++h) {
-                                const uint32_t *x = reinterpret_cast<const uint32_t *>(&kg[mt][h]);
-                                if constexpr (I8) widen4(x[w], ka[mt][h], ka[mt][2 + h]);
-                                else ka[mt][h] = x[2 * w], ka[mt][2 + h] = x[2 * w + 1];
+                                const int p = 16 * mt + 8 * h + gid, c = 4 * j + tig, sw = RE == 64 ? c : c ^ ((p & 1) << 2);
+                                kg[mt][h] = *reinterpret_cast<const uint4 *>(ent + p * RE + sw * 16);
                             }
 #pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) {
-                            const int f = (ks * S::NTT + wr * NT + nt) * 32 + lane;
-                            if constexpr (SPLIT) {
-                                const uint4 b = q_both[f];
+                        for (int w = 0; w < KPC; ++w) {
+                            const int ks = (part * (RE / 64) + j) * KPC + w;
+                            uint32_t ka[MT][4];
 #pragma unroll
-                                for (int mt = 0; mt < MT; ++mt) {
-                                    mma_16816<BF16>(s[mt][nt], ka[mt][0], ka[mt][1], ka[mt][2], ka[mt][3], b.x, b.y);
-                                    mma_16816<BF16>(s2[mt][nt], ka[mt][0], ka[mt][1], ka[mt][2], ka[mt][3], b.z, b.w);
+                            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                                for (int h = 0; h < 2; ++h) {
+                                    const uint32_t *x = reinterpret_cast<const uint32_t *>(&kg[mt][h]);
+                                    if constexpr (I8) widen4(x[w], ka[mt][h], ka[mt][2 + h]);
+                                    else ka[mt][h] = x[2 * w], ka[mt][2 + h] = x[2 * w + 1];
                                 }
-                            } else {
-                                const uint2 b = q_hi[f];
 #pragma unroll
-                                for (int mt = 0; mt < MT; ++mt)
-                                    mma_16816<BF16>(s[mt][nt], ka[mt][0], ka[mt][1], ka[mt][2], ka[mt][3], b.x, b.y);
+                            for (int nt = 0; nt < NT; ++nt) {
+                                const int f = (ks * S::NTT + wr * NT + nt) * 32 + lane;
+                                if constexpr (SPLIT) {
+                                    const uint4 b = q_both[f];
+#pragma unroll
+                                    for (int mt = 0; mt < MT; ++mt) {
+                                        mma_16816<BF16>(s[mt][nt], ka[mt][0], ka[mt][1], ka[mt][2], ka[mt][3], b.x, b.y);
+                                        mma_16816<BF16>(s2[mt][nt], ka[mt][0], ka[mt][1], ka[mt][2], ka[mt][3], b.z, b.w);
+                                    }
+                                } else {
+                                    const uint2 b = q_hi[f];
+#pragma unroll
+                                    for (int mt = 0; mt < MT; ++mt)
+                                        mma_16816<BF16>(s[mt][nt], ka[mt][0], ka[mt][1], ka[mt][2], ka[mt][3], b.x, b.y);
+                                }
                             }
                         }
                     }
                 }
                 // ---- scores in bits, masks, running maxima
-                const uint8_t *sc = scales + slot * S::kScale;
-                const uint32_t bits = *reinterpret_cast<const uint32_t *>(sc + 2 * TP * 4);
+                const uint8_t *sc = scales + tile_at * S::kScale;
+                tile_at = tile_at + 1 == S::TS ? 0 : tile_at + 1;
+                const uint32_t bits = *reinterpret_cast<const uint32_t *>(sc);
+                const float *sv = reinterpret_cast<const float *>(sc + 16);
                 edge = p0 < all_lo || p0 + TP - 1 > all_hi;
-                const bool masked = edge || bits != (TP == 32 ? 0xffffffffu : (1u << (TP & 31)) - 1u);
+                const bool masked = edge || bits != static_cast<uint32_t>((1ull << TP) - 1);
                 float y[MT][NT][4];   // int8: s + log2 vs (masked on its own: an unseen scale may be anything)
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt)
@@ -466,8 +557,8 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn(PagedAttnAr
                         const int p = 16 * mt + 8 * h + gid;
                         float ks = 1.0f, lv = 0.0f;
                         if constexpr (I8) {
-                            ks = reinterpret_cast<const float *>(sc)[p];
-                            lv = lg2(reinterpret_cast<const float *>(sc)[TP + p]);
+                            ks = sv[p];
+                            lv = lg2(sv[TP + p]);
                         }
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt)
@@ -550,113 +641,117 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn(PagedAttnAr
                         }
                     }
                 }
-                continue;
             }
             // ---- O^T += V^T P^T
-            constexpr int PB = RB / 8 < 16 ? RB / 8 : 16, NP = RB / 8 / PB, NW = PB / 4;
-            auto v_words = [&](int mt, int np, uint32_t (&x)[4][NW]) {   // positions 2 tig, + 1, + 8, + 9
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const int p = 16 * mt + 2 * tig + (k & 1) + 8 * (k >> 1);
-                    const uint8_t *row = ent + p * RB;
-                    if constexpr (PB == 16) {
-                        const int c = np * 8 + gid, sw = c ^ ((p >> 1 & 3) << 1);
-                        const uint4 t = *reinterpret_cast<const uint4 *>(row + sw * 16);
-                        x[k][0] = t.x, x[k][1] = t.y, x[k][2] = t.z, x[k][3] = t.w;
-                    } else {
-                        const int c = gid >> 1, sw = c ^ ((p >> 1 & 1) << 1);
-                        const uint2 t = *reinterpret_cast<const uint2 *>(row + sw * 16 + (gid & 1) * 8);
-                        x[k][0] = t.x, x[k][1] = t.y;
+            for (int part = 0; part < PARTS; ++part) {
+                const uint8_t *ent = next_entry();
+                if (!busy) continue;
+                constexpr int PB = RE / 8 < 16 ? RE / 8 : 16, NP = RE / 8 / PB, NW = PB / 4;
+                constexpr int MW = I8 ? 2 : 1;   // m tiles of a word
+                auto v_words = [&](int mt, int np, uint32_t (&x)[4][NW]) {   // positions 2 tig, + 1, + 8, + 9
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const int p = 16 * mt + 2 * tig + (k & 1) + 8 * (k >> 1);
+                        const uint8_t *row = ent + p * RE;
+                        if constexpr (PB == 16) {
+                            const int c = np * 8 + gid, sw = c ^ ((p >> 1 & 3) << 1);
+                            const uint4 t = *reinterpret_cast<const uint4 *>(row + sw * 16);
+                            x[k][0] = t.x, x[k][1] = t.y, x[k][2] = t.z, x[k][3] = t.w;
+                        } else {
+                            const int c = gid >> 1, sw = c ^ ((p >> 1 & 1) << 1);
+                            const uint2 t = *reinterpret_cast<const uint2 *>(row + sw * 16 + (gid & 1) * 8);
+                            x[k][0] = t.x, x[k][1] = t.y;
+                        }
+                    }
+                };
+                // a row must not be touched by values that it does not see, and zero times an infinity is not zero: at
+                // the edges of what the rows see a 16-bit tile that holds such values goes a token at a time
+                bool apart = false;
+                if constexpr (!I8) {
+                    if (edge && g.rows > 1) {
+                        bool odd = false;
+#pragma unroll
+                        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                            for (int np = 0; np < NP; ++np) {
+                                uint32_t x[4][NW];
+                                v_words(mt, np, x);
+                                constexpr uint32_t kExp = BF16 ? 0x7f80u : 0x7c00u;
+#pragma unroll
+                                for (int k = 0; k < 4; ++k)
+#pragma unroll
+                                    for (int w = 0; w < NW; ++w)
+                                        odd = odd || (x[k][w] & kExp) == kExp || (x[k][w] & (kExp << 16)) == (kExp << 16);
+                            }
+                        apart = __any_sync(0xffffffffu, odd);
                     }
                 }
-            };
-            // a row must not be touched by values that it does not see, and zero times an infinity is not zero: at the
-            // edges of what the rows see a 16-bit tile that holds such values goes a token at a time
-            bool apart = false;
-            if constexpr (!I8) {
-                if (edge && q.rows > 1) {
-                    bool odd = false;
+                if (!apart) {
 #pragma unroll
                     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
                         for (int np = 0; np < NP; ++np) {
                             uint32_t x[4][NW];
                             v_words(mt, np, x);
-                            constexpr uint32_t kExp = BF16 ? 0x7f80u : 0x7c00u;
-#pragma unroll
-                            for (int k = 0; k < 4; ++k)
-#pragma unroll
-                                for (int w = 0; w < NW; ++w)
-                                    odd = odd || (x[k][w] & kExp) == kExp || (x[k][w] & (kExp << 16)) == (kExp << 16);
-                        }
-                    apart = __any_sync(0xffffffffu, odd);
-                }
-            }
-            if (!apart) {
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                    for (int np = 0; np < NP; ++np) {
-                        uint32_t x[4][NW];
-                        v_words(mt, np, x);
-#pragma unroll
-                        for (int w = 0; w < NW; ++w) {
-                            constexpr int MW = I8 ? 2 : 1;   // m tiles of a word
-                            uint32_t va[MW][4];
-#pragma unroll
-                            for (int h = 0; h < 2; ++h) {
-                                const uint32_t xa = x[2 * h][w], xb = x[2 * h + 1][w];
-                                if constexpr (I8) {
-                                    widen4(__byte_perm(xa, xb, 0x5140), va[0][2 * h], va[0][2 * h + 1]);
-                                    widen4(__byte_perm(xa, xb, 0x7362), va[MW - 1][2 * h], va[MW - 1][2 * h + 1]);
-                                } else {
-                                    va[0][2 * h] = __byte_perm(xa, xb, 0x5410);
-                                    va[0][2 * h + 1] = __byte_perm(xa, xb, 0x7632);
-                                }
-                            }
-#pragma unroll
-                            for (int k = 0; k < MW; ++k) {
-                                const int mo_i = (np * NW + w) * MW + k;
-#pragma unroll
-                                for (int nt = 0; nt < NT; ++nt) {
-                                    mma_16816<BF16>(o[mo_i][nt], va[k][0], va[k][1], va[k][2], va[k][3], ph[mt][nt][0], ph[mt][nt][1]);
-                                    if constexpr (SPLIT)
-                                        mma_16816<BF16>(o[mo_i][nt], va[k][0], va[k][1], va[k][2], va[k][3], pl[mt][nt][0], pl[mt][nt][1]);
-                                }
-                            }
-                        }
-                    }
-            } else if constexpr (!I8) {
-                for (int t = 0; t < q.rows; ++t) {
-                    const int hi_p = q.length - q.rows + t - p0, lo_p = a.x.window > 0 ? hi_p - a.x.window + 1 : -(1 << 30);
-#pragma unroll
-                    for (int mt = 0; mt < MT; ++mt) {
-                        uint32_t keep[2];   // the halves of positions 2 tig, 2 tig + 1 (and + 8) that token t sees
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            const int p = 16 * mt + 2 * tig + 8 * h;
-                            keep[h] = (p >= lo_p && p <= hi_p ? 0xffffu : 0u) | (p + 1 >= lo_p && p + 1 <= hi_p ? 0xffff0000u : 0u);
-                        }
-#pragma unroll
-                        for (int np = 0; np < NP; ++np) {
-                            uint32_t x[4][NW];
-                            v_words(mt, np, x);
 #pragma unroll
                             for (int w = 0; w < NW; ++w) {
-                                uint32_t va[4];
+                                uint32_t va[MW][4];
 #pragma unroll
                                 for (int h = 0; h < 2; ++h) {
-                                    va[2 * h] = __byte_perm(x[2 * h][w], x[2 * h + 1][w], 0x5410) & keep[h];
-                                    va[2 * h + 1] = __byte_perm(x[2 * h][w], x[2 * h + 1][w], 0x7632) & keep[h];
+                                    const uint32_t xa = x[2 * h][w], xb = x[2 * h + 1][w];
+                                    if constexpr (I8) {
+                                        widen4(__byte_perm(xa, xb, 0x5140), va[0][2 * h], va[0][2 * h + 1]);
+                                        widen4(__byte_perm(xa, xb, 0x7362), va[MW - 1][2 * h], va[MW - 1][2 * h + 1]);
+                                    } else {
+                                        va[0][2 * h] = __byte_perm(xa, xb, 0x5410);
+                                        va[0][2 * h + 1] = __byte_perm(xa, xb, 0x7632);
+                                    }
                                 }
 #pragma unroll
-                                for (int nt = 0; nt < NT; ++nt) {
-                                    float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                                    mma_16816<BF16>(d, va[0], va[1], va[2], va[3], ph[mt][nt][0], ph[mt][nt][1]);
-                                    if constexpr (SPLIT) mma_16816<BF16>(d, va[0], va[1], va[2], va[3], pl[mt][nt][0], pl[mt][nt][1]);
+                                for (int k = 0; k < MW; ++k) {
+                                    const int om = ((part * NP + np) * NW + w) * MW + k;
 #pragma unroll
-                                    for (int x4 = 0; x4 < 4; ++x4)
-                                        if (lim[nt][x4 & 1] - p0 == hi_p && lim[nt][x4 & 1] >= 0) o[np * NW + w][nt][x4] += d[x4];
+                                    for (int nt = 0; nt < NT; ++nt) {
+                                        mma_16816<BF16>(o[om][nt], va[k][0], va[k][1], va[k][2], va[k][3], ph[mt][nt][0], ph[mt][nt][1]);
+                                        if constexpr (SPLIT)
+                                            mma_16816<BF16>(o[om][nt], va[k][0], va[k][1], va[k][2], va[k][3], pl[mt][nt][0], pl[mt][nt][1]);
+                                    }
+                                }
+                            }
+                        }
+                } else if constexpr (!I8) {
+                    for (int t = 0; t < g.rows; ++t) {
+                        const int hi_p = g.length - g.rows + t - p0, lo_p = a.x.window > 0 ? hi_p - a.x.window + 1 : -(1 << 30);
+#pragma unroll
+                        for (int mt = 0; mt < MT; ++mt) {
+                            uint32_t keep[2];   // the halves of positions 2 tig, 2 tig + 1 (and + 8) that token t sees
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                const int p = 16 * mt + 2 * tig + 8 * h;
+                                keep[h] = (p >= lo_p && p <= hi_p ? 0xffffu : 0u) | (p + 1 >= lo_p && p + 1 <= hi_p ? 0xffff0000u : 0u);
+                            }
+#pragma unroll
+                            for (int np = 0; np < NP; ++np) {
+                                uint32_t x[4][NW];
+                                v_words(mt, np, x);
+#pragma unroll
+                                for (int w = 0; w < NW; ++w) {
+                                    uint32_t va[4];
+#pragma unroll
+                                    for (int h = 0; h < 2; ++h) {
+                                        va[2 * h] = __byte_perm(x[2 * h][w], x[2 * h + 1][w], 0x5410) & keep[h];
+                                        va[2 * h + 1] = __byte_perm(x[2 * h][w], x[2 * h + 1][w], 0x7632) & keep[h];
+                                    }
+#pragma unroll
+                                    for (int nt = 0; nt < NT; ++nt) {
+                                        float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                                        mma_16816<BF16>(d, va[0], va[1], va[2], va[3], ph[mt][nt][0], ph[mt][nt][1]);
+                                        if constexpr (SPLIT) mma_16816<BF16>(d, va[0], va[1], va[2], va[3], pl[mt][nt][0], pl[mt][nt][1]);
+#pragma unroll
+                                        for (int x4 = 0; x4 < 4; ++x4)
+                                            if (lim[nt][x4 & 1] - p0 == hi_p && lim[nt][x4 & 1] >= 0) o[(part * NP + np) * NW + w][nt][x4] += d[x4];
+                                    }
                                 }
                             }
                         }
@@ -673,34 +768,31 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn(PagedAttnAr
                 for (int x = 4; x < 32; x <<= 1) l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], x);
 
         // ---- the segment's end: the position groups joined, then out or to the scratch
-        const bool whole = t0 == 0 && t1 == tps;
-        const int keep_slot = 2 * cta + (u == begin ? 0 : 1);
-        if (!whole && tid == 0)
-            a.desc[keep_slot] = make_int4(kPartHeld | (t0 == 0 ? kPartStarts : 0) | (t1 == tps ? kPartEnds : 0), item, q.r0, q.rows);
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        const bool whole = g.t0 == 0 && g.n == g.tps;
+        const int keep_slot = 2 * cta + (g.no == 0 ? 0 : 1);
+        if (g.parts > 0 && tid == 0) a.cut[cta] = make_int4(2 * g.parts + (keep_slot & 1), g.item, g.r0, g.rows);
         if constexpr (WR == 1) {
-            __syncthreads();   // every warp is through with its ring
-            float4 *buf = reinterpret_cast<float4 *>(sm + S::o_ring);   // [group][n tile][m tile][lane]
+            float4 *stat = reinterpret_cast<float4 *>(sm + S::o_stat);
+            float4 *buf = reinterpret_cast<float4 *>(sm + S::o_join);   // [group][m tile][lane], an n tile at a time
             if (gid == 0)
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                    for (int c = 0; c < 2; ++c) join_s[warp * S::kRows + 8 * nt + 2 * tig + c] = make_float4(m[nt][c], l[nt][c], mo[nt][c], 0.0f);
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int k = 0; k < OM; ++k)
-                    buf[((warp * NT + nt) * OM + k) * 32 + lane] = make_float4(o[k][nt][0], o[k][nt][1], o[k][nt][2], o[k][nt][3]);
-            __syncthreads();
+                    for (int c = 0; c < 2; ++c) stat[warp * S::kRows + 8 * nt + 2 * tig + c] = make_float4(m[nt][c], l[nt][c], mo[nt][c], 0.0f);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
+                if (nt > 0) __syncthreads();
+#pragma unroll
+                for (int k = 0; k < OM; ++k)
+                    buf[(warp * OM + k) * 32 + lane] = make_float4(o[k][nt][0], o[k][nt][1], o[k][nt][2], o[k][nt][3]);
+                __syncthreads();   // (the queries' fragments are free from here, the buffer after the next barrier)
                 float M[2] = {-INFINITY, -INFINITY}, Mo[2] = {-INFINITY, -INFINITY}, Ls[2] = {0.0f, 0.0f}, f[4][2];
                 float4 st[4][2];
 #pragma unroll
                 for (int w = 0; w < 4; ++w)
 #pragma unroll
                     for (int c = 0; c < 2; ++c) {
-                        st[w][c] = join_s[w * S::kRows + 8 * nt + 2 * tig + c];
+                        st[w][c] = stat[w * S::kRows + 8 * nt + 2 * tig + c];
                         M[c] = fmaxf(M[c], st[w][c].x);
                         Mo[c] = fmaxf(Mo[c], st[w][c].z);
                     }
@@ -719,12 +811,12 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn(PagedAttnAr
                         v[h] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
                         for (int w = 0; w < 4; ++w) {
-                            const float4 x = buf[((w * NT + nt) * OM + k + h) * 32 + lane];
+                            const float4 x = buf[(w * OM + k + h) * 32 + lane];
                             v[h].x += x.x * f[w][0], v[h].y += x.y * f[w][1], v[h].z += x.z * f[w][0], v[h].w += x.w * f[w][1];
                         }
                     }
                     if (whole) {
-                        write_out<S>(a, q.r0, q.rows, item, nt, k, v[0], v[1], inv0, inv1);
+                        write_out<S>(a, g.r0, g.rows, g.item, nt, k, v[0], v[1], inv0, inv1);
                     } else {
                         float4 *d = a.part + ((static_cast<int64_t>(keep_slot) * NT + nt) * OM + k) * 32 + lane;
                         d[0] = v[0];
@@ -735,96 +827,86 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn(PagedAttnAr
 #pragma unroll
                     for (int c = 0; c < 2; ++c) {
                         const int i = 8 * nt + 2 * tig + c;
-                        if (whole) write_lse<S>(a, q.r0, q.rows, item, i, M[c], Ls[c]);
+                        if (whole) write_lse<S>(a, g.r0, g.rows, g.item, i, M[c], Ls[c]);
                         else a.stats[static_cast<int64_t>(keep_slot) * S::kRows + i] = make_float4(M[c], Ls[c], Mo[c], 0.0f);
                     }
             }
-        } else if (busy) {
+        } else {
+            if (busy) {
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                const int n = wr * NT + nt;
-                const float inv0 = row_factor(m[nt][0], l[nt][0], mo[nt][0]), inv1 = row_factor(m[nt][1], l[nt][1], mo[nt][1]);
+                for (int nt = 0; nt < NT; ++nt) {
+                    const int n = wr * NT + nt;
+                    const float inv0 = row_factor(m[nt][0], l[nt][0], mo[nt][0]), inv1 = row_factor(m[nt][1], l[nt][1], mo[nt][1]);
 #pragma unroll
-                for (int k = 0; k < OM; k += 2) {
-                    const float4 v0 = make_float4(o[k][nt][0], o[k][nt][1], o[k][nt][2], o[k][nt][3]);
-                    const float4 v1 = make_float4(o[k + 1][nt][0], o[k + 1][nt][1], o[k + 1][nt][2], o[k + 1][nt][3]);
-                    if (whole) {
-                        write_out<S>(a, q.r0, q.rows, item, n, k, v0, v1, inv0, inv1);
-                    } else {
-                        float4 *d = a.part + ((static_cast<int64_t>(keep_slot) * S::NTT + n) * OM + k) * 32 + lane;
-                        d[0] = v0;
-                        d[32] = v1;
+                    for (int k = 0; k < OM; k += 2) {
+                        const float4 v0 = make_float4(o[k][nt][0], o[k][nt][1], o[k][nt][2], o[k][nt][3]);
+                        const float4 v1 = make_float4(o[k + 1][nt][0], o[k + 1][nt][1], o[k + 1][nt][2], o[k + 1][nt][3]);
+                        if (whole) {
+                            write_out<S>(a, g.r0, g.rows, g.item, n, k, v0, v1, inv0, inv1);
+                        } else {
+                            float4 *d = a.part + ((static_cast<int64_t>(keep_slot) * S::NTT + n) * OM + k) * 32 + lane;
+                            d[0] = v0;
+                            d[32] = v1;
+                        }
                     }
+                    if (gid == 0)
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) {
+                            const int i = 8 * n + 2 * tig + c;
+                            if (whole) write_lse<S>(a, g.r0, g.rows, g.item, i, m[nt][c], l[nt][c]);
+                            else a.stats[static_cast<int64_t>(keep_slot) * S::kRows + i] = make_float4(m[nt][c], l[nt][c], mo[nt][c], 0.0f);
+                        }
                 }
-                if (gid == 0)
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        const int i = 8 * n + 2 * tig + c;
-                        if (whole) write_lse<S>(a, q.r0, q.rows, item, i, m[nt][c], l[nt][c]);
-                        else a.stats[static_cast<int64_t>(keep_slot) * S::kRows + i] = make_float4(m[nt][c], l[nt][c], mo[nt][c], 0.0f);
-                    }
             }
-        }
-        u += n_tiles;
-        if (u - base == static_cast<int64_t>(tps) * a.kv.n_kv_heads * nrb) {
-            base = u;
-            ++seq;
+            __syncthreads();   // every warp is through with the queries' fragments
         }
     }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
-// The parts of each item that was cut, joined. Main CTA c cuts an item when its share starts inside it; the item's first
-// cut stands for it: its parts are main CTA c-1's last, then the first of c, c+1, .. up to the one that ends it. CTA
-// (i, y) finds the i-th such c among the descriptors (all of them, in one round of loads) and joins the y-th pair of m
-// tiles of an n tile: a warp takes every 8th part, eight in flight, then the warps' sums are joined in shared memory.
+// The parts of each item that was cut, joined: CTA (c, y) has the one that main CTA c began, if there is one - its parts
+// are c's last and the first of c + 1, c + 2, .. - and a share of its values, `split` warps to a pair of m tiles of an
+// n tile: they take every split-th part, B in flight, and join their sums in shared memory.
 constexpr int kJoinThreads = 256;
 
 template <typename S>
-__global__ void __launch_bounds__(kJoinThreads) k_paged_attn_join(PagedAttnArgs a, int grid) {
+__global__ void __launch_bounds__(kJoinThreads, 2) k_paged_attn_join(PagedAttnArgs a, int split, int grid) {
     constexpr int OM = S::OM, W = kJoinThreads / 32;
-    __shared__ uint32_t s_cut[kPagedMaxGrid / 32], s_end[kPagedMaxGrid / 32];
     __shared__ float4 s_stat[W][2][4], s_v[W][2][32];
+    __shared__ uint32_t s_cut[W];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, tig = lane & 3, gid = lane >> 2;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;");
-    for (int c0 = 0; c0 < grid; c0 += kJoinThreads) {
-        const int c = c0 + tid;
-        int here = 0, prev = 0;
-        if (c < grid) {
-            here = a.desc[2 * c].x;
-            if (c > 0) prev = a.desc[2 * c - 1].x, prev = prev & kPartHeld ? prev : a.desc[2 * c - 2].x;
+    int c = blockIdx.x;
+    if (split > 1) {   // (few items: a CTA for each of them, not for each main CTA)
+        int left = blockIdx.x;
+        c = -1;
+        for (int c0 = 0; c0 < grid && c < 0; c0 += kJoinThreads) {
+            const uint32_t held = __ballot_sync(0xffffffffu, c0 + tid < grid && a.cut[c0 + tid].x != 0);
+            if (lane == 0) s_cut[warp] = held;
+            __syncthreads();
+            for (int w = 0; w < W && c < 0; ++w) {
+                uint32_t bits = s_cut[w];
+                const int m = __popc(bits);
+                if (left < m) {
+                    for (; left > 0; --left) bits &= bits - 1;
+                    c = c0 + 32 * w + __ffs(bits) - 1;
+                } else {
+                    left -= m;
+                }
+            }
+            __syncthreads();
         }
-        const uint32_t cut = __ballot_sync(0xffffffffu, (here & kPartHeld) && !(here & kPartStarts) && (prev & kPartStarts) && !(prev & kPartEnds));
-        const uint32_t end = __ballot_sync(0xffffffffu, c < grid && (here & kPartEnds));
-        if (lane == 0) s_cut[c >> 5] = cut, s_end[c >> 5] = end;
+        if (c < 0) return;
     }
-    __syncthreads();
-    const int words = (grid + 31) / 32;
-    int c = -1, left = blockIdx.x;
-    for (int w = 0; w < words; ++w) {
-        uint32_t bits = s_cut[w];
-        const int n = __popc(bits);
-        if (left >= n) {
-            left -= n;
-            continue;
-        }
-        for (; left > 0; --left) bits &= bits - 1;
-        c = 32 * w + __ffs(bits) - 1;
-        break;
-    }
-    if (c < 0) return;
-    int last = c >> 5;   // the CTA that ends the item
-    uint32_t ends = s_end[last] & (0xffffffffu << (c & 31));
-    while (ends == 0 && last + 1 < words) ends = s_end[++last];
-    last = ends ? 32 * last + __ffs(ends) - 1 : grid - 1;
-    const int n = last - c + 2;
-    const int4 item = a.desc[2 * c];
-    const int slot0 = 2 * c - 1 - ((a.desc[2 * c - 1].x & kPartHeld) ? 0 : 1);
-    auto slot = [&](int k) { return static_cast<int64_t>(k == 0 ? slot0 : 2 * (c + k - 1)); };
-    const int nt = blockIdx.y / (OM / 2), k2 = blockIdx.y % (OM / 2) * 2;
+    const int4 item = a.cut[c];
+    const int n = item.x >> 1, unit = blockIdx.y * (W / split) + warp / split, sub = warp % split;
+    if (n == 0) return;
+    auto slot = [&](int k) { return static_cast<int64_t>(2 * (c + k) + (k == 0 ? item.x & 1 : 0)); };
+    const int nt = unit / (OM / 2), k2 = unit % (OM / 2) * 2;
     const int G = a.x.n_heads / a.kv.n_kv_heads, R = item.w * G, nrb = (R + S::kRows - 1) / S::kRows;
-    if (item.y % nrb * S::kRows + 8 * nt >= R) return;
-    constexpr int B = 8;   // parts whose loads are in flight together
+    const bool live = nt < S::NTT && item.y % nrb * S::kRows + 8 * nt < R;
+    constexpr int B = 4;   // parts whose loads are in flight together
     float M[2] = {-INFINITY, -INFINITY}, Mo[2] = {-INFINITY, -INFINITY}, L[2] = {0.0f, 0.0f};
     float4 v[2] = {make_float4(0.0f, 0.0f, 0.0f, 0.0f), make_float4(0.0f, 0.0f, 0.0f, 0.0f)};
     // parts or warps b = 0 .. n-1 of (stats of the lane's two rows, values of two m tiles) into M, Mo, L, v
@@ -855,11 +937,11 @@ __global__ void __launch_bounds__(kJoinThreads) k_paged_attn_join(PagedAttnArgs 
         }
     };
     float4 st[B][2], x[B][2];
-    for (int k0 = warp; k0 < n; k0 += W * B) {
+    for (int k0 = live ? sub : n; k0 < n; k0 += split * B) {
 #pragma unroll
         for (int b = 0; b < B; ++b) {
-            const bool in = k0 + b * W < n;
-            const int64_t at = slot(in ? k0 + b * W : 0);
+            const bool in = k0 + b * split < n;
+            const int64_t at = slot(in ? k0 + b * split : 0);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 st[b][h] = in ? a.stats[at * S::kRows + 8 * nt + 2 * tig + h] : make_float4(-INFINITY, 0.0f, -INFINITY, 0.0f);
@@ -868,21 +950,25 @@ __global__ void __launch_bounds__(kJoinThreads) k_paged_attn_join(PagedAttnArgs 
         }
         take(st, x);
     }
+    if (split > 1) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        s_v[warp][h][lane] = v[h];
-        if (gid == 0) s_stat[warp][h][tig] = make_float4(M[h], L[h], Mo[h], 0.0f);
+        for (int h = 0; h < 2; ++h) {
+            s_v[warp][h][lane] = v[h];
+            if (gid == 0) s_stat[warp][h][tig] = make_float4(M[h], L[h], Mo[h], 0.0f);
+        }
+        __syncthreads();
+        if (sub != 0) return;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) M[h] = Mo[h] = -INFINITY, L[h] = 0.0f, v[h] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int b0 = 0; b0 < split; b0 += B) {   // (split a multiple of B)
+#pragma unroll
+            for (int b = 0; b < B; ++b)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) st[b][h] = s_stat[warp + b0 + b][h][tig], x[b][h] = s_v[warp + b0 + b][h][lane];
+            take(st, x);
+        }
     }
-    __syncthreads();
-    if (warp != 0) return;
-    static_assert(W == B, "the warps' sums are one batch");
-#pragma unroll
-    for (int b = 0; b < B; ++b)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) st[b][h] = s_stat[b][h][tig], x[b][h] = s_v[b][h][lane];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) M[h] = Mo[h] = -INFINITY, L[h] = 0.0f, v[h] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    take(st, x);
+    if (!live) return;
     write_out<S>(a, item.z, item.w, item.y, nt, k2, v[0], v[1], row_factor(M[0], L[0], Mo[0]), row_factor(M[1], L[1], Mo[1]));
     if (k2 == 0 && gid == 0)
 #pragma unroll

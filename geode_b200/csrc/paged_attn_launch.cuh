@@ -23,7 +23,9 @@ int launch_paged_shape(const PagedAttnArgs &a, const PagedAttnPlan &p, cudaStrea
     }
     if (launch_ex(k_paged_attn<S>, dim3(grid), dim3(kPagedAttnThreads), S::kSmem, st, true, a) != cudaSuccess) return GCUDA_E_CUDA;
     if (grid == 1) return GCUDA_OK;   // (nothing is cut)
-    return launch_ex(k_paged_attn_join<S>, dim3(p.cuts, S::NTT * S::OM / 2), dim3(kJoinThreads), 0, st, true, a, grid) == cudaSuccess
+    const int units = S::NTT * S::OM / 2, per = kJoinThreads / 32 / p.split;
+    return launch_ex(k_paged_attn_join<S>, dim3(p.cuts, (units + per - 1) / per), dim3(kJoinThreads), 0, st, true, a, p.split, grid) ==
+                   cudaSuccess
                ? GCUDA_OK
                : GCUDA_E_CUDA;
 }

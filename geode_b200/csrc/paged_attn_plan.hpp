@@ -7,14 +7,13 @@
 
 namespace gcu {
 
-constexpr int kPagedMaxGrid = 2048;   // main CTAs (the join keeps a bit for each)
-
 struct PagedAttnArgs;
 struct PagedAttnPlan {
     int rows;      // query rows of a block (8, 16: position groups of one warp; 64: four warps share the positions)
     int grid;      // main CTAs
-    int cuts;      // items that their shares can cut, at most
-    size_t desc, stats, part, total;   // scratch offsets
+    int split;     // warps that share an item's parts in the join
+    int cuts;      // the join's CTAs: one for each item that may be cut, or (many items, split 1) for each main CTA
+    size_t cut, stats, part, total;   // scratch offsets
 };
 
 // Query rows sharing a key head, R = max_rows * n_heads / n_kv_heads, choose the shape: blocks of 8 or 16 rows leave all
@@ -23,22 +22,24 @@ inline PagedAttnPlan plan_paged_attn(const gcuda_paged_kv &kv, const gcuda_paged
     PagedAttnPlan p{};
     const int64_t R = static_cast<int64_t>(b.max_rows) * (n_heads / kv.n_kv_heads);
     p.rows = R <= 8 ? 8 : R <= 16 ? 16 : 64;
-    // two resident CTAs an SM; no more than there can be tiles of 16 positions
+    // two resident CTAs an SM; no more than there can be work: a tile of 16 positions and an item's cost of up to 32 each
     const int64_t per_seq = std::max<int64_t>(1, (static_cast<int64_t>(b.max_pages) * kv.page_size + 15) / 16);
     const int64_t blocks = (R + p.rows - 1) / p.rows;
-    const int64_t most = std::min<int64_t>(kPagedMaxGrid, 2 * static_cast<int64_t>(sm_count()));
+    const int64_t most = 2 * static_cast<int64_t>(sm_count());
     int64_t items = 1;
     for (const int64_t f : {static_cast<int64_t>(b.n_seq), static_cast<int64_t>(kv.n_kv_heads), blocks})
         items = std::min(most, items * std::min(most, f));   // (capped at each step: no overflow)
-    p.grid = static_cast<int>(std::min(most, items * std::min(most, per_seq)));
-    p.cuts = static_cast<int>(std::min<int64_t>(items, p.grid - 1));
+    p.grid = static_cast<int>(std::min(most, items * std::min(most, per_seq + 32)));
+    // (few items: many parts each)
+    p.split = items >= 64 ? 1 : items >= 16 ? 4 : 8;
+    p.cuts = std::max(1, static_cast<int>(p.split == 1 ? p.grid - 1 : std::min<int64_t>(items, p.grid - 1)));
     auto take = [&](size_t bytes) {
         const size_t at = p.total;
         p.total += (bytes + 255) / 256 * 256;
         return at;
     };
     const size_t slots = 2 * static_cast<size_t>(p.grid);
-    p.desc = take(slots * 16);
+    p.cut = take(static_cast<size_t>(p.grid) * 16);
     p.stats = take(slots * p.rows * 16);
     p.part = take(slots * p.rows * kv.head_dim * 4);
     return p;
