@@ -26,7 +26,8 @@ bool good_geometry(const gcuda_paged_kv *kv, const gcuda_paged_batch *b) {
     return kv && b && (kv->type == GCUDA_I8 || kv->type == GCUDA_BF16 || kv->type == GCUDA_F16) && kv->n_pages >= 1 &&
            kv->page_size >= 1 && kv->n_kv_heads >= 1 && kv->n_kv_heads <= 1024 &&
            (kv->head_dim == 64 || kv->head_dim == 128 || kv->head_dim == 256) && b->n_seq >= 1 && b->n_rows >= 1 &&
-           b->max_rows >= 1 && b->max_pages >= 1 && b->pages_stride >= 0;
+           b->max_rows >= 1 && b->max_pages >= 1 && b->pages_stride >= 0 &&
+           static_cast<int64_t>(b->max_pages) * kv->page_size <= (1ll << 30);
 }
 bool good_cache(const gcuda_paged_kv *kv, const gcuda_paged_batch *b) {
     if (!good_geometry(kv, b) || !kv->k || !kv->v || !b->row_start || !b->length || !b->pages) return false;
@@ -113,7 +114,13 @@ int gcuda_op_paged_attn(const gcuda_paged_kv *kv, const gcuda_paged_batch *b, co
     if (need == 0 || work_bytes < need) return GCUDA_E_ARG;
     const PagedAttnPlan p = plan_paged_attn(*kv, *b, x->n_heads);
     uint8_t *w = static_cast<uint8_t *>(d_work);
-    const PagedAttnArgs a{*kv, *b, *x, device_status(), reinterpret_cast<int4 *>(w + p.cut),
+    // p / page_size by a multiplication, exact for p < 2^31: with 2^l >= page_size the multiplier is less than
+    // page_size / 2^(31 + l) too large, which p < 2^31 does not carry over the next integer
+    int l = 0;
+    while ((1ll << l) < kv->page_size) ++l;
+    const uint64_t d = static_cast<uint64_t>(kv->page_size);
+    const uint32_t mul = static_cast<uint32_t>(((1ull << (31 + l)) + d - 1) / d);
+    const PagedAttnArgs a{*kv, *b, *x, device_status(), mul, 31 + l, reinterpret_cast<int4 *>(w + p.cut),
                           reinterpret_cast<float4 *>(w + p.stats), reinterpret_cast<float4 *>(w + p.part)};
     if (!a.status) return GCUDA_E_CUDA;
     cudaStream_t st = static_cast<cudaStream_t>(stream);

@@ -10,15 +10,19 @@
 // Both products run on the tensor cores (mma.sync m16n8k16, float sums) with the cache as the 16-row operand and the
 // query rows as the 8-column one, so that one token's few rows fill the instruction: S^T = K Q^T, then O^T = V^T P^T.
 // The order of dims inside a product is free as long as both operands agree, so a lane takes 16 consecutive bytes of a
-// cache row as its fragments of several products: no transposition, no staging of widened rows. int8 codes are widened
-// to f16 in registers (exact).
+// cache row as its fragments of several products: no transposition, no staging of widened rows. int8 keys are multiplied
+// as they are (m16n8k32, integer sums); int8 values are widened to f16 in registers (exact).
 //
-// Arithmetic: queries are f16 scaled by a power of two per row (bf16 for a bf16 cache). Float activations, and f16 ones
-// over a bf16 cache, are held as a sum of two such numbers, the weights too: 22 bits (16 for bf16). Otherwise a weight
-// is rounded once to 16 bits, an error of at most half a step relative to each weight, below the output's own rounding.
+// Arithmetic: over an int8 cache a query row is its largest value times (a + (b + c / 254) / 254) / 127 with int8 a, b, c:
+// every value to 2^-24 of the row's largest, each sum of products exact. Over a 16-bit cache queries are in the cache's
+// type (f16: scaled by a power of two per row); float activations, and f16 ones over bf16, are held as a sum of two such
+// numbers. Weights are rounded once to 16 bits, an error of at most half a step relative to each, below the output's own
+// rounding; for float activations they are a sum of two (22 bits, 16 for bf16).
 // int8 rows' value scales go into the weight's exponent: w = 2^(s + log2 vs - m'), with a maximum m' of its own, so that
 // rows of any scale keep their bits. Scores, sums, maxima and outputs are float.
 #pragma once
+
+#include <utility>
 
 #include "paged.cuh"
 #include "paged_attn_plan.hpp"
@@ -30,6 +34,8 @@ struct PagedAttnArgs {
     gcuda_paged_batch b;
     gcuda_attn_rows x;
     uint32_t *status;
+    uint32_t page_mul;   // p / page_size = (p * page_mul) >> page_shift for p < 2^31
+    int page_shift;
     int4 *cut;       // [grid] the item that CTA c began and did not finish: {2 parts + the slot of c's own, item, first row, rows}
     float4 *stats;   // [grid][2][kRows] {m, l, m', -} of each row
     float4 *part;    // [grid][2][n tile][m tile][lane]
@@ -39,8 +45,8 @@ constexpr int kPagedAttnThreads = 128;
 constexpr float kWeightBias = 14.0f;   // f16 weights reach up to 2^14: the smallest kept is 2^-39 of the largest
 
 // Shapes of one instantiation. NT: n tiles (8 query rows) a warp; WR: warps that share the positions (each with its own
-// rows; the CTA's other factor, 4 / WR, takes positions). An entry of the ring is a tile's K or V rows, at most 256 bytes
-// of each (longer rows: in parts).
+// rows; the CTA's other factor, 4 / WR, takes positions). An entry of the ring is K's or V's rows of ME m tiles (16
+// positions each), at most 256 bytes of a row; a tile is EPO entries of K, then as many of V.
 template <int HD_, int CACHE_, bool SPLIT_, int NT_, int WR_>
 struct PagedShape {
     static constexpr int HD = HD_, CACHE = CACHE_, NT = NT_, WR = WR_;
@@ -48,22 +54,23 @@ struct PagedShape {
     static constexpr int WP = 4 / WR;
     static constexpr int ES = I8 ? 1 : 2, RB = HD * ES;          // bytes of a value, of a row
     static constexpr int RE = RB < 256 ? RB : 256, PARTS = RB / RE;
-    static constexpr int MT = RB <= 128 ? 2 : 1, TP = 16 * MT;    // positions of a warp's tile
-    static constexpr int CT = TP * WP;                            // of a CTA's
+    static constexpr int MT = 2, TP = 16 * MT;                    // m tiles, positions of a warp's tile
+    static constexpr int ME = RB < 256 ? 2 : 1, EM = MT / ME, EPO = EM * PARTS;
+    static constexpr int CT = TP * WP;                            // positions of a CTA's tile
     // an item's beginning and end cost about what 64 KB of rows do
     static constexpr int kItemCost = 65536 / (2 * CT * RB) > 0 ? 65536 / (2 * CT * RB) : 1;
     static constexpr int NTT = NT * WR, kRows = 8 * NTT;
     static constexpr int KS = HD / 16, OM = HD / 16;
-    static constexpr int kEntry = TP * RE;
+    static constexpr int kEntry = 16 * ME * RE;
     static constexpr int kRing = (WR > 1 ? 40 : NT == 1 ? 16 : 12) * 1024;      // bytes of a position group's ring
     static constexpr int E = kRing / kEntry < 12 ? kRing / kEntry : 12;
-    static constexpr int TS = E / (2 * PARTS) + 2;                // tiles whose scales and valid bits are kept
+    static constexpr int TS = E / (2 * EPO) + 2;                // tiles whose scales and valid bits are kept
     static constexpr int kScale = (I8 ? 2 * TP * 4 : 0) + 16;
-    static constexpr int kQ = KS * NTT * 32 * 8 * (SPLIT ? 2 : 1);
+    static constexpr int kQ = I8 ? KS / 2 * NTT * 32 * 24 : KS * NTT * 32 * 8 * (SPLIT ? 2 : 1);
     static constexpr int o_q = 0, o_ring = o_q + kQ, o_scale = o_ring + WP * E * kEntry;
     static constexpr int o_col = o_scale + WP * TS * kScale;      // [kRows] column factor
     static constexpr int o_seg = o_col + kRows * 4;               // [warp][kSegs] segments looked up, not yet done
-    static constexpr int kSegs = E / (2 * PARTS) + 5;
+    static constexpr int kSegs = E / (2 * EPO) + 5;
     static constexpr int o_stat = o_seg + 4 * kSegs * 48;         // [4][kRows] m, l, m' of each position group
     static constexpr int o_join = o_stat + (WR == 1 ? 4 * kRows * 16 : 0);   // [group][m tile][lane] O of an n tile
     static constexpr int kSmem = o_join + (WR == 1 ? 4 * OM * 32 * 16 : 0);
@@ -90,6 +97,11 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a
         asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
             : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
             : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_s8_16832(int32_t (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t move_trans(uint32_t x) {   // an 8x8 matrix of 16-bit values, transposed
     uint32_t y;
@@ -202,6 +214,12 @@ __device__ __forceinline__ int64_t seq_cost(const PagedAttnArgs &a, const SeqRow
     return t * a.kv.n_kv_heads * ((q.rows * (a.x.n_heads / a.kv.n_kv_heads) + S::kRows - 1) / S::kRows);
 }
 
+// f(kind) for the kinds first, first + 1, ..
+template <int first = 0, typename F, int... e>
+__device__ __forceinline__ void for_kinds(F &&f, std::integer_sequence<int, e...>) {
+    (f(std::integral_constant<int, first + e>{}), ...);
+}
+
 struct PagedSegment {   // what a CTA does of one item (48 bytes)
     int r0, rows, length;
     int lo, tps;        // the item's first position and tiles
@@ -214,7 +232,7 @@ struct PagedSegment {   // what a CTA does of one item (48 bytes)
 template <typename S>
 __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn(PagedAttnArgs a) {
     constexpr int HD = S::HD, NT = S::NT, WR = S::WR, TP = S::TP, MT = S::MT, RB = S::RB, RE = S::RE, E = S::E, OM = S::OM;
-    constexpr int PARTS = S::PARTS, KPC = S::I8 ? 4 : 2;   // (k steps of a 16-byte piece)
+    constexpr int PARTS = S::PARTS, ME = S::ME, EM = S::EM, EPO = S::EPO;
     constexpr bool I8 = S::I8, BF16 = S::BF16, SPLIT = S::SPLIT;
     extern __shared__ __align__(128) uint8_t sm[];
     __shared__ int64_t s_sum[4], s_base;
@@ -262,8 +280,9 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn(PagedAttnAr
     }
     __syncthreads();
 
-    uint2 *q_hi = reinterpret_cast<uint2 *>(sm + S::o_q);       // fragments (b0, b1) [k step][n tile][lane]; SPLIT: uint4
-    uint4 *q_both = reinterpret_cast<uint4 *>(sm + S::o_q);
+    // the queries' fragments (b0, b1) [k step][n tile][lane]; two numbers a value (SPLIT, and int8's a, b): uint4
+    uint2 *q_one = reinterpret_cast<uint2 *>(sm + S::o_q + (I8 ? S::KS / 2 * S::NTT * 32 * 16 : 0));   // (int8: c)
+    uint4 *q_two = reinterpret_cast<uint4 *>(sm + S::o_q);
     float *col_s = reinterpret_cast<float *>(sm + S::o_col);
     uint8_t *ring = sm + S::o_ring + wp * E * S::kEntry;
     uint8_t *scales = sm + S::o_scale + wp * S::TS * S::kScale;
@@ -316,58 +335,60 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn(PagedAttnAr
     };
     struct Tile {
         int page;    // of this lane's position (-2: it has none)
+        int in_page; // its place there
         int p0;      // the tile's first position (-1: no tile)
         int kh;
     };
     auto look = [&]() {
         open();
-        if (at_n == 0) return Tile{-2, -1, 0};
-        Tile t{-2, at_p0, at_kh};
-        const int p = at_p0 + lane;
-        if (lane < TP && p < at_length) t.page = at_pages[p / a.kv.page_size];
+        if (at_n == 0) return Tile{-2, 0, -1, 0};
+        const int p = at_p0 + lane, n = static_cast<int>((static_cast<uint64_t>(p) * a.page_mul) >> a.page_shift);
+        Tile t{-2, p - n * a.kv.page_size, at_p0, at_kh};
+        if (p < at_length) t.page = at_pages[n];
         at_p0 += S::CT;
         --at_n;
         return t;
     };
     Tile ahead0 = look(), ahead1 = look();
 
-    // ---- the copies: entry by entry through the tiles looked up (K's parts, then V's)
-    int in_slot = 0, in_entry = 0, in_tile = 0;   // the ring slot, the entry within its tile, the tile's place among scales
-    bool in_any = true, there = false, one_page = false;
+    // ---- the copies: entry by entry through the tiles looked up. The kind of an entry (0 .. EPO-1: K's, then V's) is known
+    // where it is issued: it follows from the kind that is waited for there.
+    int in_slot = 0, in_tile = 0;   // the ring slot; the tile's place among the scales
+    bool in_any = true, one_page = false;
     int64_t place = 0;    // value offset of this lane's position
     uint32_t ok = 0;      // the tile's positions that are on a page
-    auto issue = [&]() {
-        if (in_entry == 0 && in_any) {
+    auto issue = [&](auto kind_) {
+        constexpr int kind = decltype(kind_)::value % (2 * EPO);
+        if (kind == 0 && in_any) {
             const Tile t = ahead0;
             ahead0 = ahead1;
             ahead1 = look();
             in_any = t.p0 >= 0;
             if (in_any) {
-                there = t.page >= 0 && t.page < a.kv.n_pages;
+                in_tile = in_tile + 1 == S::TS ? 0 : in_tile + 1;
+                const bool there = t.page >= 0 && t.page < a.kv.n_pages;
                 if (t.page != -2 && !there) atomicOr(a.status, kErrBadShape);
-                const int ip = (t.p0 + lane) % a.kv.page_size;
-                place = there ? t.page * a.kv.page_stride + ip * a.kv.pos_stride + t.kh * a.kv.head_stride : 0;
+                place = there ? t.page * a.kv.page_stride + t.in_page * a.kv.pos_stride + t.kh * a.kv.head_stride : 0;
                 ok = __ballot_sync(0xffffffffu, there);
                 // positions one after the other on one page: their rows are pos_stride apart
-                const int ip0 = __shfl_sync(0xffffffffu, ip, 0);
-                one_page = ok == static_cast<uint32_t>((1ull << TP) - 1) && ip0 + TP <= a.kv.page_size;
+                one_page = ok == 0xffffffffu && __shfl_sync(0xffffffffu, t.in_page, 0) + TP <= a.kv.page_size;
                 if (wr == 0) {
                     const uint32_t d = scales_a + in_tile * S::kScale;
                     if (lane == 0) *reinterpret_cast<uint32_t *>(scales + in_tile * S::kScale) = ok;
                     if constexpr (I8) {
-                        if (lane < TP) {
-                            const int64_t sp = there ? t.page * a.kv.scale_page_stride + ip * a.kv.scale_pos_stride + t.kh * a.kv.scale_head_stride : 0;
-                            copy4(d + 16 + lane * 4, a.kv.k_scale + sp, there ? 4 : 0);
-                            copy4(d + 16 + (TP + lane) * 4, a.kv.v_scale + sp, there ? 4 : 0);
-                        }
+                        const int64_t sp = there ? t.page * a.kv.scale_page_stride + t.in_page * a.kv.scale_pos_stride + t.kh * a.kv.scale_head_stride : 0;
+                        copy4(d + 16 + lane * 4, a.kv.k_scale + sp, there ? 4 : 0);
+                        copy4(d + 16 + (TP + lane) * 4, a.kv.v_scale + sp, there ? 4 : 0);
                     }
                 }
             }
         }
         if (in_any) {
-            const bool is_v = in_entry >= PARTS;
-            const uint8_t *src = static_cast<const uint8_t *>(is_v ? a.kv.v : a.kv.k) + (in_entry - (is_v ? PARTS : 0)) * RE;
+            constexpr bool is_v = kind >= EPO;
+            constexpr int first_p = kind % EPO / PARTS * 16 * ME, part = kind % PARTS;
+            const uint8_t *src = static_cast<const uint8_t *>(is_v ? a.kv.v : a.kv.k) + part * RE;
             constexpr int CH = RE / 16, PR = 32 / CH;   // 16-byte pieces of a row, rows of a warp's copy
+            constexpr int N = 16 * ME * CH / (32 * WR);
             const int c = lane % CH;
             const uint32_t dst = ring_a + in_slot * S::kEntry;
             // pieces swapped within a row so that the fragment loads of K (8 rows x 4 neighbouring pieces) and of V (every
@@ -379,38 +400,33 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn(PagedAttnAr
                 else sw = RE == 64 ? c : c ^ ((p & 1) << 2);
                 copy16(dst + p * RE + sw * 16, from, bytes);
             };
-            constexpr int N = TP * CH / (32 * WR);
             if (one_page) {
-                const int64_t first = __shfl_sync(0xffffffffu, place, 0), step = a.kv.pos_stride * S::ES;
-                const uint8_t *from = src + first * S::ES + (wr * PR + lane / CH) * step + c * 16;
+                const int64_t step = a.kv.pos_stride * S::ES;
+                const uint8_t *from = src + __shfl_sync(0xffffffffu, place, first_p) * S::ES + (wr * PR + lane / CH) * step + c * 16;
 #pragma unroll
                 for (int k = 0; k < N; ++k) put(k, from, 16), from += step * (PR * WR);
             } else {
 #pragma unroll
                 for (int k = 0; k < N; ++k) {
-                    const int p = (k * WR + wr) * PR + lane / CH;
+                    const int p = first_p + (k * WR + wr) * PR + lane / CH;
                     const int64_t x = __shfl_sync(0xffffffffu, place, p);
                     put(k, src + x * S::ES + c * 16, (ok >> p & 1) ? 16 : 0);
                 }
-            }
-            if (++in_entry == 2 * PARTS) {
-                in_entry = 0;
-                in_tile = in_tile + 1 == S::TS ? 0 : in_tile + 1;
             }
         }
         in_slot = in_slot + 1 == E ? 0 : in_slot + 1;
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
-#pragma unroll 1
-    for (int e = 0; e < E - 1; ++e) issue();
+    in_tile = S::TS - 1;
+    for_kinds(issue, std::make_integer_sequence<int, E - 1>{});
     __syncwarp();   // (the first segments are written)
 
     int slot = 0, tile_at = 0;   // the products' place in the ring and among the scales
-    auto next_entry = [&]() {    // the entry at `slot` has landed, and the one before it is free for a new copy
+    auto next_entry = [&](auto kind_) {   // the entry at `slot`, of this kind, has landed; the one before it is free for a copy
         asm volatile("cp.async.wait_group %0;" ::"n"(E - 2) : "memory");
         if constexpr (WR == 1) __syncwarp();
         else __syncthreads();
-        issue();
+        issue(std::integral_constant<int, decltype(kind_)::value + E - 1>{});
         const uint8_t *ent = ring + slot * S::kEntry;
         slot = slot + 1 == E ? 0 : slot + 1;
         return ent;
@@ -427,31 +443,62 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn(PagedAttnAr
             const int64_t at = r < R ? static_cast<int64_t>(g.r0 + r / G) * a.x.q_stride + static_cast<int64_t>(g.kh * G + r % G) * a.x.q_head_stride + lane * N : 0;
 #pragma unroll
             for (int k = 0; k < N; ++k) v[k] = r < R ? load_act(a.x.q, a.x.type, at + k) : 0.0f;
-            int ex = 0;
-            if constexpr (!BF16) {
-#pragma unroll
-                for (int k = 0; k < N; ++k) top = fmaxf(top, fabsf(v[k]));
-                top = warp_max(top);
-                // 2^-ex brings the largest to [1, 2); zeros, infinities: as they are
-                ex = top > 0.0f && top < INFINITY ? ilogbf(top) : 0;
-#pragma unroll
-                for (int k = 0; k < N; ++k) v[k] = scalbnf(v[k], -ex);
-            }
-            if (lane == 0) col_s[i] = scalbnf(a.x.scale * 1.44269504088896341f, ex);
             const int nt = i >> 3, n = i & 7;
+            if constexpr (I8) {
 #pragma unroll
-            for (int k = 0; k < N; k += 2) {
-                const int d = lane * N + k;
-                constexpr int W = 16 / S::ES;   // dims of a 16-byte piece; 4 lanes' pieces side by side
-                const int ks = d / (4 * W) * (W / 4) + d % W / 4, t = d % (4 * W) / W, b = d % 4 / 2;
-                const int f = (ks * S::NTT + nt) * 32 + n * 4 + t;
-                const uint32_t hi = pack2<BF16>(v[k], v[k + 1]);
-                if constexpr (SPLIT) {
-                    const float2 h = unpack2<BF16>(hi);
-                    reinterpret_cast<uint32_t *>(q_both + f)[b] = hi;
-                    reinterpret_cast<uint32_t *>(q_both + f)[2 + b] = pack2<BF16>(v[k] - h.x, v[k + 1] - h.y);
-                } else {
-                    reinterpret_cast<uint32_t *>(q_hi + f)[b] = hi;
+                for (int k = 0; k < N; ++k) top = max_nan(top, fabsf(v[k]));
+#pragma unroll
+                for (int x = 16; x > 0; x >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, x));
+                const float inv = top > 0.0f ? 127.0f / top : 0.0f;
+                if (lane == 0) col_s[i] = a.x.scale * 1.44269504088896341f * (top * (1.0f / 127.0f));
+                constexpr int W = N < 4 ? N : 4;   // neighbouring dims stored together
+#pragma unroll
+                for (int k = 0; k < N; k += W) {
+                    uint32_t w[3] = {0, 0, 0};
+#pragma unroll
+                    for (int x = 0; x < W; ++x) {
+                        float r = v[k + x] * inv;
+#pragma unroll
+                        for (int y = 0; y < 3; ++y) {
+                            const int digit = __float2int_rn(r);
+                            w[y] |= static_cast<uint32_t>(digit & 0xff) << (8 * x);
+                            r = (r - static_cast<float>(digit)) * 254.0f;
+                        }
+                    }
+                    const int d = lane * N + k, ks = d / 64 * 2 + d % 16 / 8, t = d % 64 / 16, b = d % 8 / 4;
+                    const int f = (ks * S::NTT + nt) * 32 + n * 4 + t;
+                    uint32_t *const at3[3] = {reinterpret_cast<uint32_t *>(q_two + f) + b, reinterpret_cast<uint32_t *>(q_two + f) + 2 + b,
+                                              reinterpret_cast<uint32_t *>(q_one + f) + b};
+#pragma unroll
+                    for (int y = 0; y < 3; ++y)
+                        if constexpr (W == 4) *at3[y] = w[y];
+                        else reinterpret_cast<uint16_t *>(at3[y])[d % 4 / 2] = static_cast<uint16_t>(w[y]);
+                }
+            } else {
+                int ex = 0;
+                if constexpr (!BF16) {
+#pragma unroll
+                    for (int k = 0; k < N; ++k) top = fmaxf(top, fabsf(v[k]));
+                    top = warp_max(top);
+                    // 2^-ex brings the largest to [1, 2); zeros, infinities: as they are
+                    ex = top > 0.0f && top < INFINITY ? ilogbf(top) : 0;
+#pragma unroll
+                    for (int k = 0; k < N; ++k) v[k] = scalbnf(v[k], -ex);
+                }
+                if (lane == 0) col_s[i] = scalbnf(a.x.scale * 1.44269504088896341f, ex);
+#pragma unroll
+                for (int k = 0; k < N; k += 2) {
+                    // (a 16-byte piece has 8 dims, 2 k steps; 4 lanes' pieces lie side by side)
+                    const int d = lane * N + k, ks = d / 32 * 2 + d % 8 / 4, t = d % 32 / 8, b = d % 4 / 2;
+                    const int f = (ks * S::NTT + nt) * 32 + n * 4 + t;
+                    const uint32_t hi = pack2<BF16>(v[k], v[k + 1]);
+                    if constexpr (SPLIT) {
+                        const float2 h = unpack2<BF16>(hi);
+                        reinterpret_cast<uint32_t *>(q_two + f)[b] = hi;
+                        reinterpret_cast<uint32_t *>(q_two + f)[2 + b] = pack2<BF16>(v[k] - h.x, v[k + 1] - h.y);
+                    } else {
+                        reinterpret_cast<uint32_t *>(q_one + f)[b] = hi;
+                    }
                 }
             }
         }
@@ -489,66 +536,101 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn(PagedAttnAr
             bool edge;
             {
                 // ---- S^T = K Q^T
-                float s[MT][NT][4], s2[MT][NT][4];
+                float s[MT][NT][4];
+                auto k_entry = [&](auto kind_) {
+                    constexpr int kind = decltype(kind_)::value, m0 = kind / PARTS * ME, part = kind % PARTS;
+                    const uint8_t *ent = next_entry(kind_);
+                    if (!busy) return;
+                    auto piece = [&](int mt, int h, int j) {   // the 4 neighbouring lanes' 16 bytes of row gid + 8 h
+                        const int p = 16 * mt + 8 * h + gid, c = 4 * j + tig, sw = RE == 64 ? c : c ^ ((p & 1) << 2);
+                        return *reinterpret_cast<const uint4 *>(ent + p * RE + sw * 16);
+                    };
+                    if constexpr (I8) {
+                        // sums on top of 1.5 * 2^23, whose float neighbours are the integers: |sum| <= 127^2 HD < 2^22
+                        int32_t acc[ME][NT][3][4];
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt)
+                        for (int mt = 0; mt < ME; ++mt)
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
+                            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                        for (int c = 0; c < 4; ++c) s[mt][nt][c] = s2[mt][nt][c] = 0.0f;
+                                for (int y = 0; y < 3; ++y)
 #pragma unroll
-                for (int part = 0; part < PARTS; ++part) {
-                    const uint8_t *ent = next_entry();
-                    if (!busy) continue;
+                                    for (int c = 0; c < 4; ++c) acc[mt][nt][y][c] = static_cast<int32_t>(kBiasBits);
 #pragma unroll
-                    for (int j = 0; j < RE / 64; ++j) {
-                        uint4 kg[MT][2];
+                        for (int j = 0; j < RE / 64; ++j) {
+                            uint4 kg[ME][2];
 #pragma unroll
-                        for (int mt = 0; mt < MT; ++mt)
+                            for (int mt = 0; mt < ME; ++mt) kg[mt][0] = piece(mt, 0, j), kg[mt][1] = piece(mt, 1, j);
 #pragma unroll
-                            for (int h = 0; h < 2; ++h) {
-                                const int p = 16 * mt + 8 * h + gid, c = 4 * j + tig, sw = RE == 64 ? c : c ^ ((p & 1) << 2);
-                                kg[mt][h] = *reinterpret_cast<const uint4 *>(ent + p * RE + sw * 16);
-                            }
+                            for (int w = 0; w < 2; ++w)
 #pragma unroll
-                        for (int w = 0; w < KPC; ++w) {
-                            const int ks = (part * (RE / 64) + j) * KPC + w;
-                            uint32_t ka[MT][4];
+                                for (int nt = 0; nt < NT; ++nt) {
+                                    const int f = ((2 * j + w) * S::NTT + wr * NT + nt) * 32 + lane;
+                                    const uint4 ab = q_two[f];
+                                    const uint2 cc = q_one[f];
 #pragma unroll
-                            for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                                for (int h = 0; h < 2; ++h) {
-                                    const uint32_t *x = reinterpret_cast<const uint32_t *>(&kg[mt][h]);
-                                    if constexpr (I8) widen4(x[w], ka[mt][h], ka[mt][2 + h]);
-                                    else ka[mt][h] = x[2 * w], ka[mt][2 + h] = x[2 * w + 1];
-                                }
-#pragma unroll
-                            for (int nt = 0; nt < NT; ++nt) {
-                                const int f = (ks * S::NTT + wr * NT + nt) * 32 + lane;
-                                if constexpr (SPLIT) {
-                                    const uint4 b = q_both[f];
-#pragma unroll
-                                    for (int mt = 0; mt < MT; ++mt) {
-                                        mma_16816<BF16>(s[mt][nt], ka[mt][0], ka[mt][1], ka[mt][2], ka[mt][3], b.x, b.y);
-                                        mma_16816<BF16>(s2[mt][nt], ka[mt][0], ka[mt][1], ka[mt][2], ka[mt][3], b.z, b.w);
+                                    for (int mt = 0; mt < ME; ++mt) {
+                                        const uint32_t a0 = w ? kg[mt][0].z : kg[mt][0].x, a1 = w ? kg[mt][1].z : kg[mt][1].x;
+                                        const uint32_t a2 = w ? kg[mt][0].w : kg[mt][0].y, a3 = w ? kg[mt][1].w : kg[mt][1].y;
+                                        mma_s8_16832(acc[mt][nt][0], a0, a1, a2, a3, ab.x, ab.y);
+                                        mma_s8_16832(acc[mt][nt][1], a0, a1, a2, a3, ab.z, ab.w);
+                                        mma_s8_16832(acc[mt][nt][2], a0, a1, a2, a3, cc.x, cc.y);
                                     }
-                                } else {
-                                    const uint2 b = q_hi[f];
-#pragma unroll
-                                    for (int mt = 0; mt < MT; ++mt)
-                                        mma_16816<BF16>(s[mt][nt], ka[mt][0], ka[mt][1], ka[mt][2], ka[mt][3], b.x, b.y);
                                 }
-                            }
                         }
+#pragma unroll
+                        for (int mt = 0; mt < ME; ++mt)
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                                for (int c = 0; c < 4; ++c)
+                                    s[m0 + mt][nt][c] = fmaf(fmaf(unbias(acc[mt][nt][2][c]), 1.0f / 254.0f, unbias(acc[mt][nt][1][c])),
+                                                             1.0f / 254.0f, unbias(acc[mt][nt][0][c]));
+                    } else {
+                        float hi[ME][NT][4], lo[ME][NT][4];
+#pragma unroll
+                        for (int mt = 0; mt < ME; ++mt)
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                                for (int c = 0; c < 4; ++c) hi[mt][nt][c] = part ? s[m0 + mt][nt][c] : 0.0f, lo[mt][nt][c] = 0.0f;
+#pragma unroll
+                        for (int j = 0; j < RE / 64; ++j) {
+                            uint4 kg[ME][2];
+#pragma unroll
+                            for (int mt = 0; mt < ME; ++mt) kg[mt][0] = piece(mt, 0, j), kg[mt][1] = piece(mt, 1, j);
+#pragma unroll
+                            for (int w = 0; w < 2; ++w)
+#pragma unroll
+                                for (int nt = 0; nt < NT; ++nt) {
+                                    const int f = ((2 * (part * (RE / 64) + j) + w) * S::NTT + wr * NT + nt) * 32 + lane;
+                                    const uint4 b2 = SPLIT ? q_two[f] : make_uint4(0, 0, 0, 0);
+                                    const uint2 b = SPLIT ? make_uint2(b2.x, b2.y) : q_one[f];
+#pragma unroll
+                                    for (int mt = 0; mt < ME; ++mt) {
+                                        const uint32_t a0 = w ? kg[mt][0].z : kg[mt][0].x, a1 = w ? kg[mt][1].z : kg[mt][1].x;
+                                        const uint32_t a2 = w ? kg[mt][0].w : kg[mt][0].y, a3 = w ? kg[mt][1].w : kg[mt][1].y;
+                                        mma_16816<BF16>(hi[mt][nt], a0, a1, a2, a3, b.x, b.y);
+                                        if constexpr (SPLIT) mma_16816<BF16>(lo[mt][nt], a0, a1, a2, a3, b2.z, b2.w);
+                                    }
+                                }
+                        }
+#pragma unroll
+                        for (int mt = 0; mt < ME; ++mt)
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                                for (int c = 0; c < 4; ++c) s[m0 + mt][nt][c] = SPLIT ? hi[mt][nt][c] + lo[mt][nt][c] : hi[mt][nt][c];
                     }
-                }
+                };
+                for_kinds(k_entry, std::make_integer_sequence<int, EPO>{});
                 // ---- scores in bits, masks, running maxima
                 const uint8_t *sc = scales + tile_at * S::kScale;
                 tile_at = tile_at + 1 == S::TS ? 0 : tile_at + 1;
                 const uint32_t bits = *reinterpret_cast<const uint32_t *>(sc);
                 const float *sv = reinterpret_cast<const float *>(sc + 16);
                 edge = p0 < all_lo || p0 + TP - 1 > all_hi;
-                const bool masked = edge || bits != static_cast<uint32_t>((1ull << TP) - 1);
+                const bool masked = edge || bits != 0xffffffffu;
                 float y[MT][NT][4];   // int8: s + log2 vs (masked on its own: an unseen scale may be anything)
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt)
@@ -565,7 +647,6 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn(PagedAttnAr
 #pragma unroll
                             for (int c = 0; c < 2; ++c) {
                                 float &v = s[mt][nt][2 * h + c];
-                                if constexpr (SPLIT) v += s2[mt][nt][2 * h + c];
                                 v *= col[nt][c] * ks;
                                 if constexpr (I8) y[mt][nt][2 * h + c] = v + lv;
                                 if (masked) {
@@ -643,10 +724,10 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn(PagedAttnAr
                 }
             }
             // ---- O^T += V^T P^T
-#pragma unroll
-            for (int part = 0; part < PARTS; ++part) {
-                const uint8_t *ent = next_entry();
-                if (!busy) continue;
+            auto v_entry = [&](auto kind_) {
+                constexpr int m0 = (decltype(kind_)::value - EPO) / PARTS * ME, part = decltype(kind_)::value % PARTS;
+                const uint8_t *ent = next_entry(kind_);
+                if (!busy) return;
                 constexpr int PB = RE / 8 < 16 ? RE / 8 : 16, NP = RE / 8 / PB, NW = PB / 4;
                 constexpr int MW = I8 ? 2 : 1;   // m tiles of a word
                 auto v_words = [&](int mt, int np, uint32_t (&x)[4][NW]) {   // positions 2 tig, + 1, + 8, + 9
@@ -672,7 +753,7 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn(PagedAttnAr
                     if (edge && g.rows > 1) {
                         bool odd = false;
 #pragma unroll
-                        for (int mt = 0; mt < MT; ++mt)
+                        for (int mt = 0; mt < ME; ++mt)
 #pragma unroll
                             for (int np = 0; np < NP; ++np) {
                                 uint32_t x[4][NW];
@@ -689,7 +770,7 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn(PagedAttnAr
                 }
                 if (!apart) {
 #pragma unroll
-                    for (int mt = 0; mt < MT; ++mt)
+                    for (int mt = 0; mt < ME; ++mt)
 #pragma unroll
                         for (int np = 0; np < NP; ++np) {
                             uint32_t x[4][NW];
@@ -713,9 +794,9 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn(PagedAttnAr
                                     const int om = ((part * NP + np) * NW + w) * MW + k;
 #pragma unroll
                                     for (int nt = 0; nt < NT; ++nt) {
-                                        mma_16816<BF16>(o[om][nt], va[k][0], va[k][1], va[k][2], va[k][3], ph[mt][nt][0], ph[mt][nt][1]);
+                                        mma_16816<BF16>(o[om][nt], va[k][0], va[k][1], va[k][2], va[k][3], ph[m0 + mt][nt][0], ph[m0 + mt][nt][1]);
                                         if constexpr (SPLIT)
-                                            mma_16816<BF16>(o[om][nt], va[k][0], va[k][1], va[k][2], va[k][3], pl[mt][nt][0], pl[mt][nt][1]);
+                                            mma_16816<BF16>(o[om][nt], va[k][0], va[k][1], va[k][2], va[k][3], pl[m0 + mt][nt][0], pl[m0 + mt][nt][1]);
                                     }
                                 }
                             }
@@ -724,11 +805,11 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn(PagedAttnAr
                     for (int t = 0; t < g.rows; ++t) {
                         const int hi_p = g.length - g.rows + t - p0, lo_p = a.x.window > 0 ? hi_p - a.x.window + 1 : -(1 << 30);
 #pragma unroll
-                        for (int mt = 0; mt < MT; ++mt) {
+                        for (int mt = 0; mt < ME; ++mt) {
                             uint32_t keep[2];   // the halves of positions 2 tig, 2 tig + 1 (and + 8) that token t sees
 #pragma unroll
                             for (int h = 0; h < 2; ++h) {
-                                const int p = 16 * mt + 2 * tig + 8 * h;
+                                const int p = 16 * (m0 + mt) + 2 * tig + 8 * h;
                                 keep[h] = (p >= lo_p && p <= hi_p ? 0xffffu : 0u) | (p + 1 >= lo_p && p + 1 <= hi_p ? 0xffff0000u : 0u);
                             }
 #pragma unroll
@@ -746,8 +827,8 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn(PagedAttnAr
 #pragma unroll
                                     for (int nt = 0; nt < NT; ++nt) {
                                         float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                                        mma_16816<BF16>(d, va[0], va[1], va[2], va[3], ph[mt][nt][0], ph[mt][nt][1]);
-                                        if constexpr (SPLIT) mma_16816<BF16>(d, va[0], va[1], va[2], va[3], pl[mt][nt][0], pl[mt][nt][1]);
+                                        mma_16816<BF16>(d, va[0], va[1], va[2], va[3], ph[m0 + mt][nt][0], ph[m0 + mt][nt][1]);
+                                        if constexpr (SPLIT) mma_16816<BF16>(d, va[0], va[1], va[2], va[3], pl[m0 + mt][nt][0], pl[m0 + mt][nt][1]);
 #pragma unroll
                                         for (int x4 = 0; x4 < 4; ++x4)
                                             if (lim[nt][x4 & 1] - p0 == hi_p && lim[nt][x4 & 1] >= 0) o[(part * NP + np) * NW + w][nt][x4] += d[x4];
@@ -757,7 +838,8 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn(PagedAttnAr
                         }
                     }
                 }
-            }
+            };
+            for_kinds<EPO>(v_entry, std::make_integer_sequence<int, EPO>{});
         }
         // a lane summed its positions' weights: the others' of the column are on the lanes with the same tig
 #pragma unroll

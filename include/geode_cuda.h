@@ -380,7 +380,8 @@ typedef struct {
 
 /* The step's rows: sequence s owns rows row_start[s] .. row_start[s+1]-1 (at most max_rows) of the step's buffers of
  * n_rows rows; its cache holds length[s] positions, its rows the last of them; position p lies on page
- * pages[s * pages_stride + p / page_size], p / page_size < max_pages. The three arrays are device memory (int32), so a
+ * pages[s * pages_stride + p / page_size], p / page_size < max_pages (max_pages * page_size at most 2^30). The three
+ * arrays are device memory (int32), so a
  * captured step follows its plan from replay to replay. Rows of no sequence (behind row_start[n_seq]) are neither read
  * nor written. What is out of range on the device raises the status word's flag 2 (gcuda_op_status): a sequence whose
  * rows or length are out of range is left out whole; a position on a page id outside [0, n_pages) is not stored and
