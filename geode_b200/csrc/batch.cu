@@ -3,7 +3,6 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
-#include <atomic>
 #include <type_traits>
 
 #include "../../include/geode_cuda.h"
@@ -63,14 +62,7 @@ int launch_adjust_slices(AdjustArgs a, cudaStream_t st) {
     using P = AdjustShape<T, U>;
     a.slices = (a.V + P::slice - 1) / P::slice;
     if (static_cast<int64_t>(a.S) * a.slices > 0x7fffffff) return GCUDA_E_ARG;
-    static std::atomic<uint64_t> opted{0};   // devices whose shared-memory opt-in is done
-    const int dev = current_device();
-    if (dev < 0) return GCUDA_E_CUDA;
-    if (!(opted.load(std::memory_order_relaxed) >> dev & 1)) {
-        if (cudaFuncSetAttribute(k_logits_adjust<T, U>, cudaFuncAttributeMaxDynamicSharedMemorySize, P::smem) != cudaSuccess)
-            return GCUDA_E_CUDA;
-        opted.fetch_or(1ull << dev, std::memory_order_relaxed);
-    }
+    if (!shared_opt_in<k_logits_adjust<T, U>>(P::smem)) return GCUDA_E_CUDA;
     return launched(launch_ex(k_logits_adjust<T, U>, dim3(a.S * a.slices), dim3(kAdjustThreads), P::smem, st, true, a));
 }
 // Slices of four loads a thread where that makes two CTAs an SM or more, of one load otherwise
@@ -90,12 +82,28 @@ int gcuda_op_paged_append(const gcuda_paged_kv *kv, const gcuda_paged_batch *b, 
         x->rope_dim % 2 || x->rope_dim > kv->head_dim || (x->rope_dim > 0 && !x->inv_freq) || !(x->eps >= 0.0f) ||
         (x->q && x->q == x->q_out && (x->q_stride != x->q_out_stride || x->q_head_stride != kv->head_dim)))
         return GCUDA_E_ARG;
-    AppendArgs a{*kv, *b, *x, device_status()};
+    // A row's warps: one where the rows alone make three CTAs an SM, else more, up to a turn for every warp
+    const int per_turn = 256 / kv->head_dim;   // vectors
+    const int turns = (x->n_heads + per_turn - 1) / per_turn + 2 * ((kv->n_kv_heads + per_turn - 1) / per_turn);
+    const int warps = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(turns, (3ll * kAppendWarps * sm_count() + b->n_rows - 1) / b->n_rows)));
+    const int64_t grid = (static_cast<int64_t>(b->n_rows) * warps + kAppendWarps - 1) / kAppendWarps;
+    if (grid > 0x7fffffff) return GCUDA_E_ARG;
+    const int half = x->rope_dim / 2;
+    const size_t word = kv->type == GCUDA_I8 ? 8 : 4;   // the angles' and the odd halves' staging values
+    const size_t smem = kAppendThreads * kAppendAhead * 8 * value_bytes(x->type) + kAppendWarps * half * 2 * word +
+                        (half % 8 ? kAppendThreads * 8 * word : 0);
+    const size_t es = value_bytes(x->type);
+    auto vec = [&](const void *p, int64_t stride, int64_t head_stride) {
+        return p && !misaligned(p, 16) && stride * static_cast<int64_t>(es) % 16 == 0 && head_stride * static_cast<int64_t>(es) % 16 == 0;
+    };
+    AppendArgs a{*kv, *b, *x, warps, vec(x->q, x->q_stride, x->q_head_stride), vec(x->k, x->k_stride, 0),
+                 vec(x->v, x->v_stride, 0), vec(x->q_out, x->q_out_stride, 0), device_status()};
     if (!a.status) return GCUDA_E_CUDA;
     return by_types(x->type, kv->type, [&](auto act, auto cache) {
         return by_dim(kv->head_dim, [&](auto hd) {
-            return launched(launch_ex(k_paged_append<hd(), decltype(act), cache()>, dim3(b->n_rows), dim3(kAppendThreads), 0,
-                                      static_cast<cudaStream_t>(stream), false, a));
+            if (!shared_opt_in<k_paged_append<hd(), decltype(act), cache()>>(kAppendMaxShared)) return static_cast<int>(GCUDA_E_CUDA);
+            return launched(launch_ex(k_paged_append<hd(), decltype(act), cache()>, dim3(static_cast<unsigned>(grid)), dim3(kAppendThreads), smem,
+                                      static_cast<cudaStream_t>(stream), true, a));
         });
     });
 }

@@ -84,6 +84,18 @@ inline uint32_t *device_status() {
     return d.status[dev];
 }
 
+// A kernel's shared-memory opt-in on the current device, once per device (bytes: the largest any of its launches takes).
+template <auto kern>
+inline bool shared_opt_in(int bytes) {
+    static std::atomic<uint64_t> done{0};
+    const int dev = current_device();
+    if (dev < 0) return false;
+    if (done.load(std::memory_order_acquire) >> dev & 1) return true;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return false;
+    done.fetch_or(1ull << dev, std::memory_order_release);
+    return true;
+}
+
 // Launch with the programmatic-stream-serialization attribute when pdl: the kernel may begin (its prologue, the
 // weight stream) before the previous kernel on the stream ends; it waits for it at griddepcontrol.wait.
 template <typename Kern, typename... Args>

@@ -45,19 +45,28 @@ __device__ __forceinline__ SeqRows seq_rows(const gcuda_paged_batch &b, int page
 }
 
 // ---------------------------------------------------------------------------------------------- append ----
-// One CTA per row: the row's sequence is found by all threads at once (row_start is read in one round of loads, no
-// search down a tree), the rotary cosines and sines of its position are taken once for all heads, then a warp per head
-// vector. Angles are position * inv_freq in 64 bits (at position 10^6 a 32-bit angle is off by 0.03). Queries and keys
-// for a 16-bit cache go through float; keys for the int8 cache through double up to the rounding to float, so that
-// their codes are those of the definition (a float rounding moves one code in about 10^5).
+// One or more warps to a row, each on its own (no barrier): a head vector is 8 neighbouring values to a lane, so a warp's
+// turn is 1, 2 or 4 vectors of one kind (queries, keys, values), and a lane has the same dims of every head of its row, so
+// that the norm's weights and the rotary cosines and sines stay in registers. The turns' rows come through a ring in
+// shared memory, the first of them asked for before anything else; then the row's sequence is found (one round of loads
+// over up to 256 row_start entries), its length and page read and the angles taken. Angles are position * inv_freq in 64
+// bits (at position 10^6 a 32-bit angle is off by 0.03), reduced to a turn there. Queries and keys for a 16-bit cache go
+// through float; keys for the int8 cache through double up to the rounding to float, so that their codes are those of the
+// definition (a float rounding moves one code in about 10^5).
 struct AppendArgs {
     gcuda_paged_kv kv;
     gcuda_paged_batch b;
     gcuda_append_rows x;
+    int warps;                       // of a row
+    bool vec_q, vec_k, vec_v, vec_o; // 16-byte loads and stores of these rows
     uint32_t *status;
 };
 
 constexpr int kAppendThreads = 256;
+constexpr int kAppendWarps = kAppendThreads / 32;
+constexpr int kAppendAhead = 4;   // turns whose copies to shared memory are in flight
+// (float rows of 256, every dimension rotated by an odd half: ring, angles and staging)
+constexpr int kAppendMaxShared = kAppendThreads * kAppendAhead * 32 + kAppendWarps * 128 * 16 + kAppendThreads * 8 * 8;
 
 __device__ __forceinline__ float max_nan(float a, float b) {   // (a NaN among the values stays one)
     float r;
@@ -65,120 +74,298 @@ __device__ __forceinline__ float max_nan(float a, float b) {   // (a NaN among t
     return r;
 }
 
-// Norm (w: NULL off) and rotation of the HD values a warp holds (lane + 32 i), through its staging row st.
-template <int HD, typename T>
-__device__ __forceinline__ void norm_rotate(T (&v)[HD / 32], const float *w, float eps, int half, const double2 *trig, T *st) {
-    const int lane = threadIdx.x & 31;
-    if (w) {
-        T ss = 0;
+// The nearest integers to 127 y / top, the even one of two, as bytes: by a float product where that is sure (it is within
+// 10^-4 of the quotient; added to 1.5 * 2^23 its low bits are the integer), next to a half by comparing 2 * 127 |y| with
+// (2 k + 1) top, both exact in double
+__device__ __forceinline__ uint2 codes_of(const float (&y)[8], float top) {
+    const float inv = top > 0.0f ? 127.0f / top : 0.0f;
+    uint32_t w[2] = {0, 0}, near = 0;
 #pragma unroll
-        for (int i = 0; i < HD / 32; ++i) ss += v[i] * v[i];
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        const T inv = T(1) / sqrt(ss / T(HD) + T(eps));
-#pragma unroll
-        for (int i = 0; i < HD / 32; ++i) v[i] = v[i] * inv * (T(1) + T(w[lane + 32 * i]));
+    for (int i = 0; i < 8; ++i) {
+        const float c = __fmul_rn(y[i], inv), m = __fadd_rn(c, kBiasF);
+        if (fabsf(c - __fsub_rn(m, kBiasF)) > 0.499f) near |= 1u << i;
+        w[i / 4] |= (__float_as_uint(m) & 0xffu) << (8 * (i % 4));
     }
-    if (half == 0) return;
+    if (near) {
 #pragma unroll
-    for (int i = 0; i < HD / 32; ++i) st[lane + 32 * i] = v[i];
+        for (int i = 0; i < 8; ++i)
+            if (near >> i & 1) {
+                const double k = floor(static_cast<double>(__fmul_rn(fabsf(y[i]), inv)));
+                const double a = 254.0 * static_cast<double>(fabsf(y[i])), h = (2.0 * k + 1.0) * static_cast<double>(top);
+                const int n = static_cast<int>(k), r = a > h ? n + 1 : a < h ? n : n + (n & 1);
+                w[i / 4] = (w[i / 4] & ~(0xffu << (8 * (i % 4)))) | static_cast<uint32_t>((y[i] < 0.0f ? -r : r) & 0xff) << (8 * (i % 4));
+            }
+    }
+    return make_uint2(w[0], w[1]);
+}
+
+// 1 / sqrt(mean x^2 + eps) of a vector of HD, 8 values to a lane
+template <int HD>
+__device__ __forceinline__ float head_factor(const float (&v)[8], float eps) {
+    float ss = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) ss = fmaf(v[i], v[i], ss);
+#pragma unroll
+    for (int o = HD / 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    return rsqrtf(ss * (1.0f / HD) + eps);
+}
+template <int HD>
+__device__ __forceinline__ double head_factor(const double (&v)[8], double eps) {
+    double ss = 0.0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) ss = fma(v[i], v[i], ss);
+#pragma unroll
+    for (int o = HD / 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    return rsqrt(ss * (1.0 / HD) + eps);
+}
+
+// Rotation of a lane's 8 values at `at`, trig the row's (cos, sin) [half]. A half of whole lanes: partners by shuffles;
+// else through st, a vector's HD values of shared memory.
+template <typename T, typename T2>
+__device__ __forceinline__ void head_rotate(T (&v)[8], int at, int half, const T2 *trig, T *st) {
+    const int lane = threadIdx.x & 31;
+    if (half % 8 == 0) {
+        const bool mine = at < 2 * half, low = at < half;
+        const int other = mine ? (low ? lane + half / 8 : lane - half / 8) : lane;
+        const T2 *t = trig + (mine ? (low ? at : at - half) : 0);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const T p = __shfl_sync(0xffffffffu, v[i], other);
+            if (mine) v[i] = low ? v[i] * T(t[i].x) - p * T(t[i].y) : v[i] * T(t[i].x) + p * T(t[i].y);
+        }
+        return;
+    }
     __syncwarp();
 #pragma unroll
-    for (int i = 0; i < HD / 32; ++i) {
-        const int d = lane + 32 * i;
+    for (int i = 0; i < 8; ++i) st[at + i] = v[i];
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int d = at + i;
         if (d < half) v[i] = v[i] * T(trig[d].x) - st[d + half] * T(trig[d].y);
         else if (d < 2 * half) v[i] = v[i] * T(trig[d - half].x) + st[d - half] * T(trig[d - half].y);
     }
-    __syncwarp();
+}
+
+// The last sequence s with row_start[s] <= row (a warp's lanes alike), -1: none. Rounds of 32 probes while more than 256
+// are left, then all of these.
+__device__ __forceinline__ int find_sequence(const gcuda_paged_batch &b, int row) {
+    const int lane = threadIdx.x & 31;
+    int lo = 0, n = b.n_seq;   // the answer is among [lo, lo + n), or there is none
+    while (n > 256) {
+        const int gap = (n + 31) / 32, s = lo + lane * gap;
+        const uint32_t le = __ballot_sync(0xffffffffu, lane * gap < n && b.row_start[min(s, b.n_seq)] <= row);
+        const int k = le ? 31 - __clz(le) : 0;
+        n = min(gap, n - k * gap);
+        lo += k * gap;
+    }
+    int found = -1;
+    int v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = lane + 32 * i < n ? b.row_start[lo + lane + 32 * i] : 0x7fffffff;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const uint32_t le = __ballot_sync(0xffffffffu, v[i] <= row);
+        if (le) found = lo + 32 * i + 31 - __clz(le);
+    }
+    return found;
 }
 
 template <int HD, typename TA, int CACHE>
-__global__ void __launch_bounds__(kAppendThreads) k_paged_append(AppendArgs a) {
-    __shared__ double2 trig[HD / 2];
-    __shared__ double stage[kAppendThreads / 32][HD];
-    __shared__ int s_seq;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, row = blockIdx.x;
-    if (tid == 0) s_seq = -1;
-    __syncthreads();
-    for (int s = tid; s < a.b.n_seq; s += kAppendThreads)
-        if (a.b.row_start[s] <= row && row < a.b.row_start[s + 1]) atomicMax(&s_seq, s);
-    __syncthreads();
-    const int seq = s_seq;
-    if (seq < 0) return;
-    const SeqRows q = seq_rows(a.b, a.kv.page_size, seq, a.status);
-    if (row - q.r0 >= q.rows) return;
-    const int pos = q.length - q.rows + (row - q.r0);
+__global__ void __launch_bounds__(kAppendThreads, 3) k_paged_append(AppendArgs a) {
+    constexpr int LV = HD / 8, VW = 32 / LV;   // lanes of a vector, vectors of a turn
+    constexpr bool I8 = CACHE == GCUDA_I8;
+    using Trig = std::conditional_t<I8, double2, float2>;
+    using Wide = std::conditional_t<I8, double, float>;
+    extern __shared__ __align__(16) uint8_t append_sm[];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane / LV, at = lane % LV * 8;
+    const int64_t work = static_cast<int64_t>(blockIdx.x) * kAppendWarps + warp;
+    const int row = static_cast<int>(work / a.warps), first = static_cast<int>(work % a.warps);
+    const int nh = a.x.n_heads, nkv = a.kv.n_kv_heads, half = a.x.rope_dim / 2;
+    const int tq = (nh + VW - 1) / VW, tk = (nkv + VW - 1) / VW, turns = tq + 2 * tk;
+    if (row >= a.b.n_rows) return;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;");
+
+    constexpr int U = sizeof(TA) * 8 / 16;   // 16-byte pieces of 8 values
+    struct __align__(16) Raw {
+        uint4 w[U];
+    };
+    Raw *ring = reinterpret_cast<Raw *>(append_sm) + (warp * kAppendAhead) * 32 + lane;   // [turn][lane]: a lane's own
+    const TA *src_q = static_cast<const TA *>(a.x.q) + row * a.x.q_stride + at, *src_k = static_cast<const TA *>(a.x.k) + row * a.x.k_stride + at,
+             *src_v = static_cast<const TA *>(a.x.v) + row * a.x.v_stride + at;
+    auto fetch = [&](int turn, int slot) {
+        if (turn < turns) {
+            const TA *src;
+            bool vec, in;
+            if (turn < tq) {
+                const int h = turn * VW + sub;
+                in = h < nh, vec = a.vec_q;
+                src = src_q + h * a.x.q_head_stride;
+            } else {
+                const bool k = turn < tq + tk;
+                const int h = (turn - (k ? tq : tq + tk)) * VW + sub;
+                in = h < nkv, vec = k ? a.vec_k : a.vec_v;
+                src = (k ? src_k : src_v) + h * HD;
+            }
+            Raw *dst = ring + slot * 32;
+            if (!in) {
+                *dst = Raw{};
+            } else if (vec) {
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_addr(&dst->w[u])), "l"(reinterpret_cast<const uint4 *>(src) + u) : "memory");
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) reinterpret_cast<TA *>(dst)[i] = src[i];
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    for (int i = 0; i < kAppendAhead - 1; ++i) fetch(first + i * a.warps, i);
+
+    // the row's place
+    const int seq = find_sequence(a.b, row);
+    int pos = -1, page = -1;
+    if (seq >= 0) {
+        const SeqRows q = seq_rows(a.b, a.kv.page_size, seq, a.status);
+        if (row - q.r0 < q.rows) {
+            pos = q.length - q.rows + (row - q.r0);
+            if (pos >= 0) page = a.b.pages[seq * a.b.pages_stride + pos / a.kv.page_size];
+            if ((page < 0 || page >= a.kv.n_pages) && lane == 0) atomicOr(a.status, kErrBadShape);
+        }
+    }
+    const bool stored = page >= 0 && page < a.kv.n_pages;
+    const int in_page = pos >= 0 ? pos % a.kv.page_size : 0;
+    Trig *trig = reinterpret_cast<Trig *>(append_sm + kAppendWarps * kAppendAhead * 32 * sizeof(Raw)) + warp * half;
+    Wide *st = reinterpret_cast<Wide *>(append_sm + kAppendWarps * (kAppendAhead * 32 * sizeof(Raw) + half * sizeof(Trig))) + (warp * VW + sub) * HD;   // (odd halves only)
+    for (int i = lane; i < half && pos >= 0; i += 32) {
+        const double angle = static_cast<double>(pos) * static_cast<double>(a.x.inv_freq[i]);
+        if constexpr (I8) {
+            double sn, cs;
+            sincos(angle, &sn, &cs);
+            trig[i] = make_double2(cs, sn);
+        } else {
+            const double t = angle * 0.15915494309189534;   // in turns
+            float sn, cs;
+            sincospif(2.0f * static_cast<float>(t - rint(t)), &sn, &cs);
+            trig[i] = make_float2(cs, sn);
+        }
+    }
+    __syncwarp();
     if (pos < 0) {
-        if (tid == 0) atomicOr(a.status, kErrBadShape);
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
         return;
     }
-    const int half = a.x.rope_dim / 2;
-    for (int i = tid; i < half; i += kAppendThreads) {
-        double sn, cs;
-        sincos(static_cast<double>(pos) * static_cast<double>(a.x.inv_freq[i]), &sn, &cs);
-        trig[i] = make_double2(cs, sn);
+    // whole halves: a lane's cosines and (signed) sines, (1, 0) where it does not rotate, and its partner
+    const bool whole = half % 8 == 0, mine = at < 2 * half, low = at < half;
+    const int other = mine ? (low ? lane + half / 8 : lane - half / 8) : lane;
+    float cs[8], sn[8], wq[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const bool turn = whole && mine;
+        const Trig t = turn ? trig[(low ? at : at - half) + i] : Trig{1, 0};
+        cs[i] = static_cast<float>(t.x);
+        sn[i] = static_cast<float>(turn && low ? -t.y : t.y);
+        wq[i] = a.x.q_norm ? 1.0f + a.x.q_norm[at + i] : 1.0f;
     }
-    const int page = a.b.pages[seq * a.b.pages_stride + pos / a.kv.page_size];
-    const bool stored = page >= 0 && page < a.kv.n_pages;
-    if (!stored && tid == 0) atomicOr(a.status, kErrBadShape);
-    __syncthreads();
-    const int nh = a.x.n_heads, nkv = a.kv.n_kv_heads, in_page = pos % a.kv.page_size;
-    for (int item = warp; item < nh + 2 * nkv; item += kAppendThreads / 32) {
-        if (item < nh) {
-            const TA *src = static_cast<const TA *>(a.x.q) + row * a.x.q_stride + item * a.x.q_head_stride;
-            TA *dst = static_cast<TA *>(a.x.q_out) + row * a.x.q_out_stride + item * HD;
-            float v[HD / 32];
+    auto rotate = [&](float (&v)[8]) {
+        if (half == 0) return;
+        if (whole) {
 #pragma unroll
-            for (int i = 0; i < HD / 32; ++i) v[i] = to_float(src[lane + 32 * i]);
-            norm_rotate<HD, float>(v, a.x.q_norm, a.x.eps, half, trig, reinterpret_cast<float *>(stage[warp]));
+            for (int i = 0; i < 8; ++i) v[i] = fmaf(v[i], cs[i], __shfl_sync(0xffffffffu, v[i], other) * sn[i]);
+        } else {
+            head_rotate<float>(v, at, half, trig, reinterpret_cast<float *>(st));
+        }
+    };
+    const int64_t place = stored ? page * a.kv.page_stride + in_page * a.kv.pos_stride + at : 0;
+    const int64_t place_s = stored ? page * a.kv.scale_page_stride + in_page * a.kv.scale_pos_stride : 0;
+    TA *out = static_cast<TA *>(a.x.q_out) + row * a.x.q_out_stride + at;
+    int slot = 0;
+#pragma unroll 1
+    for (int turn = first; turn < turns; turn += a.warps) {
+        fetch(turn + (kAppendAhead - 1) * a.warps, slot == 0 ? kAppendAhead - 1 : slot - 1);
+        asm volatile("cp.async.wait_group %0;" ::"n"(kAppendAhead - 1) : "memory");   // (a lane reads what it copied)
+        float v[8];
+        {
+            const Raw r = ring[slot * 32];
+            const TA *x = reinterpret_cast<const TA *>(&r);
 #pragma unroll
-            for (int i = 0; i < HD / 32; ++i) dst[lane + 32 * i] = from_float<TA>(v[i]);
+            for (int i = 0; i < 8; ++i) v[i] = to_float(x[i]);
+        }
+        slot = slot + 1 == kAppendAhead ? 0 : slot + 1;
+        if (turn < tq) {
+            const int h = turn * VW + sub;
+            if (a.x.q_norm) {
+                const float f = head_factor<HD>(v, a.x.eps);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] *= f * wq[i];
+            }
+            rotate(v);
+            if (h >= nh) continue;
+            Raw o;
+            TA *y = reinterpret_cast<TA *>(&o);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) y[i] = from_float<TA>(v[i]);
+            TA *dst = out + h * HD;
+            if (a.vec_o) {
+#pragma unroll
+                for (int u = 0; u < U; ++u) reinterpret_cast<uint4 *>(dst)[u] = o.w[u];
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) dst[i] = y[i];
+            }
             continue;
         }
         if (!stored) continue;
-        const bool is_k = item < nh + nkv;
-        const int h = is_k ? item - nh : item - nh - nkv;
-        const TA *src = is_k ? static_cast<const TA *>(a.x.k) + row * a.x.k_stride + h * HD
-                             : static_cast<const TA *>(a.x.v) + row * a.x.v_stride + h * HD;
-        float v[HD / 32];
-#pragma unroll
-        for (int i = 0; i < HD / 32; ++i) v[i] = to_float(src[lane + 32 * i]);
+        const bool is_k = turn < tq + tk;
+        const int h = (turn - (is_k ? tq : tq + tk)) * VW + sub;
         if (is_k) {
-            if constexpr (CACHE == GCUDA_I8) {
-                double d[HD / 32];
+            if constexpr (I8) {
+                double y[8];
 #pragma unroll
-                for (int i = 0; i < HD / 32; ++i) d[i] = v[i];
-                norm_rotate<HD, double>(d, a.x.k_norm, a.x.eps, half, trig, stage[warp]);
+                for (int i = 0; i < 8; ++i) y[i] = v[i];
+                if (a.x.k_norm) {
+                    const double f = head_factor<HD>(y, static_cast<double>(a.x.eps));
 #pragma unroll
-                for (int i = 0; i < HD / 32; ++i) v[i] = static_cast<float>(d[i]);
+                    for (int i = 0; i < 8; ++i) y[i] = y[i] * f * (1.0 + static_cast<double>(a.x.k_norm[at + i]));
+                }
+                if (half) head_rotate<double>(y, at, half, trig, st);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = static_cast<float>(y[i]);
             } else {
-                norm_rotate<HD, float>(v, a.x.k_norm, a.x.eps, half, trig, reinterpret_cast<float *>(stage[warp]));
+                if (a.x.k_norm) {
+                    const float f = head_factor<HD>(v, a.x.eps);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) v[i] *= f * (1.0f + a.x.k_norm[at + i]);
+                }
+                rotate(v);
             }
         }
-        const int64_t at = page * a.kv.page_stride + in_page * a.kv.pos_stride + h * a.kv.head_stride;
+        const int64_t to = place + h * a.kv.head_stride;
         void *base = is_k ? a.kv.k : a.kv.v;
-        if constexpr (CACHE == GCUDA_I8) {
+        if constexpr (I8) {
             float top = 0.0f;
 #pragma unroll
-            for (int i = 0; i < HD / 32; ++i) top = max_nan(top, fabsf(v[i]));
+            for (int i = 0; i < 8; ++i) top = max_nan(top, fabsf(v[i]));
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
-            int8_t *dst = static_cast<int8_t *>(base) + at;
-#pragma unroll
-            for (int i = 0; i < HD / 32; ++i)
-                dst[lane + 32 * i] = top > 0.0f ? static_cast<int8_t>(__double2int_rn(static_cast<double>(v[i]) * 127.0 / static_cast<double>(top)))
-                                                : static_cast<int8_t>(0);
-            if (lane == 0)
-                (is_k ? a.kv.k_scale : a.kv.v_scale)[page * a.kv.scale_page_stride + in_page * a.kv.scale_pos_stride +
-                                                     h * a.kv.scale_head_stride] =
+            for (int o = LV / 2; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+            if (h >= nkv) continue;
+            *reinterpret_cast<uint2 *>(static_cast<int8_t *>(base) + to) = codes_of(v, top);
+            if (lane % LV == 0)
+                (is_k ? a.kv.k_scale : a.kv.v_scale)[place_s + h * a.kv.scale_head_stride] =
                     static_cast<float>(static_cast<double>(top) / 127.0);
         } else {
             using TC = std::conditional_t<CACHE == GCUDA_BF16, __nv_bfloat16, __half>;
-            TC *dst = static_cast<TC *>(base) + at;
+            if (h >= nkv) continue;
+            uint4 o;
+            TC *y = reinterpret_cast<TC *>(&o);
 #pragma unroll
-            for (int i = 0; i < HD / 32; ++i) dst[lane + 32 * i] = from_float<TC>(v[i]);
+            for (int i = 0; i < 8; ++i) y[i] = from_float<TC>(v[i]);
+            *reinterpret_cast<uint4 *>(static_cast<TC *>(base) + to) = o;
         }
     }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
 }  // namespace gcu

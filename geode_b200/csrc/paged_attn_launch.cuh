@@ -2,8 +2,6 @@
 // paged_attn_*.cu files, one per type, which compile side by side).
 #pragma once
 
-#include <atomic>
-
 #include "device.hpp"
 #include "paged_attn.cuh"
 #include "paged_attn_plan.hpp"
@@ -13,14 +11,7 @@ namespace gcu {
 template <typename S>
 int launch_paged_shape(const PagedAttnArgs &a, const PagedAttnPlan &p, cudaStream_t st) {
     const int grid = p.grid;
-    static std::atomic<uint64_t> opted{0};   // devices whose shared-memory opt-in is done
-    const int dev = current_device();
-    if (dev < 0) return GCUDA_E_CUDA;
-    if (!(opted.load(std::memory_order_relaxed) >> dev & 1)) {
-        if (cudaFuncSetAttribute(k_paged_attn<S>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem) != cudaSuccess)
-            return GCUDA_E_CUDA;
-        opted.fetch_or(1ull << dev, std::memory_order_relaxed);
-    }
+    if (!shared_opt_in<k_paged_attn<S>>(S::kSmem)) return GCUDA_E_CUDA;
     if (launch_ex(k_paged_attn<S>, dim3(grid), dim3(kPagedAttnThreads), S::kSmem, st, true, a) != cudaSuccess) return GCUDA_E_CUDA;
     if (grid == 1) return GCUDA_OK;   // (nothing is cut)
     const int units = S::NTT * S::OM / 2, per = kJoinThreads / 32 / p.split;
