@@ -1,7 +1,7 @@
 // paged_attn.cuh - attention of each sequence's newest rows over its pages (flash decoding over a paged cache).
 //
 // An item is one (sequence, key head, block of query rows): the sequence's T rows times the G query heads that share the
-// key head, R = T * G rows in blocks of kRows. Items are cut into tiles of positions and the tiles of all items, laid end
+// key head, R = T * G rows in blocks of kRows = 8 (k_paged_attn), 16 or 40 (k_paged_attn_rows, paged_attn_rows.cuh). Items are cut into tiles of positions and the tiles of all items, laid end
 // to end with a few tiles' time for each item's beginning, are dealt out evenly to the resident CTAs (each CTA finds its
 // share by a scan over the lengths on the device: whatever the lengths, every CTA has the same work). What a CTA holds
 // of an item that it does not finish goes to the scratch and k_paged_attn_join adds the parts up. The copies run ahead
@@ -44,37 +44,15 @@ struct PagedAttnArgs {
 constexpr int kPagedAttnThreads = 128;
 constexpr float kWeightBias = 14.0f;   // f16 weights reach up to 2^14: the smallest kept is 2^-39 of the largest
 
-// Shapes of one instantiation. NT: n tiles (8 query rows) a warp; WR: warps that share the positions (each with its own
-// rows; the CTA's other factor, 4 / WR, takes positions). An entry of the ring is K's or V's rows of ME m tiles (16
-// positions each), at most 256 bytes of a row; a tile is EPO entries of K, then as many of V.
-template <int HD_, int CACHE_, bool SPLIT_, int NT_, int WR_>
-struct PagedShape {
-    static constexpr int HD = HD_, CACHE = CACHE_, NT = NT_, WR = WR_;
+// What the kernels' shapes share. NT: n tiles (8 query rows each) of an item; ES, RB: bytes of a value, of a row
+template <int HD_, int CACHE_, bool SPLIT_, int NT_>
+struct PagedBase {
+    static constexpr int HD = HD_, CACHE = CACHE_, NT = NT_, kRows = 8 * NT;
     static constexpr bool SPLIT = SPLIT_, I8 = CACHE == GCUDA_I8, BF16 = CACHE == GCUDA_BF16;
-    static constexpr int WP = 4 / WR;
-    static constexpr int ES = I8 ? 1 : 2, RB = HD * ES;          // bytes of a value, of a row
-    static constexpr int RE = RB < 256 ? RB : 256, PARTS = RB / RE;
-    static constexpr int MT = 2, TP = 16 * MT;                    // m tiles, positions of a warp's tile
-    static constexpr int ME = RB < 256 ? 2 : 1, EM = MT / ME, EPO = EM * PARTS;
-    static constexpr int CT = TP * WP;                            // positions of a CTA's tile
-    // an item's beginning and end cost about what 64 KB of rows do
-    static constexpr int kItemCost = 65536 / (2 * CT * RB) > 0 ? 65536 / (2 * CT * RB) : 1;
-    static constexpr int NTT = NT * WR, kRows = 8 * NTT;
-    static constexpr int KS = HD / 16, OM = HD / 16;
-    static constexpr int kEntry = 16 * ME * RE;
-    static constexpr int kRing = (WR > 1 ? 40 : NT == 1 ? 16 : 12) * 1024;      // bytes of a position group's ring
-    static constexpr int E = kRing / kEntry < 12 ? kRing / kEntry : 12;
-    static constexpr int TS = E / (2 * EPO) + 2;                // tiles whose scales and valid bits are kept
-    static constexpr int kScale = (I8 ? 2 * TP * 4 : 0) + 16;
-    static constexpr int kQ = I8 ? KS / 2 * NTT * 32 * 24 : KS * NTT * 32 * 8 * (SPLIT ? 2 : 1);
-    static constexpr int o_q = 0, o_ring = o_q + kQ, o_scale = o_ring + WP * E * kEntry;
-    static constexpr int o_col = o_scale + WP * TS * kScale;      // [kRows] column factor
-    static constexpr int o_seg = o_col + kRows * 4;               // [warp][kSegs] segments looked up, not yet done
-    static constexpr int kSegs = E / (2 * EPO) + 5;
-    static constexpr int o_stat = o_seg + 4 * kSegs * 48;         // [4][kRows] m, l, m' of each position group
-    static constexpr int o_join = o_stat + (WR == 1 ? 4 * kRows * 16 : 0);   // [group][m tile][lane] O of an n tile
-    static constexpr int kSmem = o_join + (WR == 1 ? 4 * OM * 32 * 16 : 0);
-    static_assert(E >= 3, "two entries in flight");
+    static constexpr int ES = I8 ? 1 : 2, RB = HD * ES, OM = HD / 16;
+    // the queries' fragments: int8 three digits a value in k steps of 32 dims, else one or two numbers in k steps of 16
+    static constexpr int kQ = I8 ? HD / 32 * NT * 32 * 24 : HD / 16 * NT * 32 * 8 * (SPLIT ? 2 : 1);
+    static constexpr int kQTwo = I8 ? HD / 32 * NT * 32 * 16 : 0;   // (int8: where the third digits start)
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -138,10 +116,23 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void *src, uint32_t b
 __device__ __forceinline__ void copy4(uint32_t dst, const void *src, uint32_t bytes) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
-__device__ __forceinline__ float load_act(const void *p, int type, int64_t i) {
-    if (type == GCUDA_F32) return static_cast<const float *>(p)[i];
-    if (type == GCUDA_BF16) return __bfloat162float(static_cast<const __nv_bfloat16 *>(p)[i]);
-    return __half2float(static_cast<const __half *>(p)[i]);
+template <int N>
+__device__ __forceinline__ void load_act(float (&v)[N], const void *p, int type, int64_t i) {
+    if (type == GCUDA_F32) {
+#pragma unroll
+        for (int k = 0; k < N; ++k) v[k] = static_cast<const float *>(p)[i + k];
+    } else if (type == GCUDA_BF16) {
+#pragma unroll
+        for (int k = 0; k < N; ++k) v[k] = __bfloat162float(static_cast<const __nv_bfloat16 *>(p)[i + k]);
+    } else {
+#pragma unroll
+        for (int k = 0; k < N; ++k) v[k] = __half2float(static_cast<const __half *>(p)[i + k]);
+    }
+}
+__device__ __forceinline__ void store_act2(void *p, int type, int64_t i, float x, float y) {
+    if (type == GCUDA_F32) static_cast<float *>(p)[i] = x, static_cast<float *>(p)[i + 1] = y;
+    else if (type == GCUDA_BF16) static_cast<__nv_bfloat16 *>(p)[i] = __float2bfloat16_rn(x), static_cast<__nv_bfloat16 *>(p)[i + 1] = __float2bfloat16_rn(y);
+    else static_cast<__half *>(p)[i] = __float2half_rn(x), static_cast<__half *>(p)[i + 1] = __float2half_rn(y);
 }
 __device__ __forceinline__ void store_act4(void *p, int type, int64_t i, float4 v) {   // (rows of out are packed heads: aligned by 4 or by 1)
     const float f[4] = {v.x, v.y, v.z, v.w};
@@ -162,29 +153,42 @@ __device__ __forceinline__ void store_act4(void *p, int type, int64_t i, float4 
     }
 }
 
-// The dims of m tile m's rows gid and gid + 8: the first of the two neighbours (a lane's 8th of a row is taken in pieces
-// of at most 16 bytes, 8 pieces side by side)
-template <int HD, int ES>
-__device__ __forceinline__ int dim_of(int m, int gid) {
-    constexpr int PB = HD * ES / 8 < 16 ? HD * ES / 8 : 16, DPP = PB / ES;
-    return 2 * m / DPP * 8 * DPP + gid * DPP + 2 * m % DPP;
-}
-
-// One row block's finished values of m tiles m, m + 1 (four neighbouring dims) of the rows 2 tig, 2 tig + 1 of an n tile
+// One row block's finished values of m tiles m, m + 1 (mostly four neighbouring dims) of the rows 2 tig, 2 tig + 1 of an n
+// tile
 template <typename S>
 __device__ __forceinline__ void write_out(const PagedAttnArgs &a, int r0, int rows, int item, int nt, int m, const float4 &x,
                                           const float4 &y, float inv0, float inv1) {
     const int lane = threadIdx.x & 31, gid = lane >> 2, tig = lane & 3;
     const int G = a.x.n_heads / a.kv.n_kv_heads, R = rows * G, nrb = (R + S::kRows - 1) / S::kRows;
-    const int kh = item / nrb, rb = item % nrb, d = dim_of<S::HD, S::ES>(m, gid);
+    const int kh = item / nrb, rb = item % nrb, d = S::dim(m, gid), d2 = S::dim(m + 1, gid);
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
         const int r = rb * S::kRows + 8 * nt + 2 * tig + c;
         if (r >= R) continue;
         const float inv = c ? inv1 : inv0;
-        const int64_t at = static_cast<int64_t>(r0 + r / G) * a.x.out_stride + static_cast<int64_t>(kh * G + r % G) * S::HD + d;
-        store_act4(a.x.out, a.x.type, at,
-                   c ? make_float4(x.y * inv, x.w * inv, y.y * inv, y.w * inv) : make_float4(x.x * inv, x.z * inv, y.x * inv, y.z * inv));
+        const int64_t at = static_cast<int64_t>(r0 + r / G) * a.x.out_stride + static_cast<int64_t>(kh * G + r % G) * S::HD;
+        const float4 v = c ? make_float4(x.y * inv, x.w * inv, y.y * inv, y.w * inv) : make_float4(x.x * inv, x.z * inv, y.x * inv, y.z * inv);
+        if (d2 == d + 2) {
+            store_act4(a.x.out, a.x.type, at + d, v);
+        } else {
+            store_act2(a.x.out, a.x.type, at + d, v.x, v.y);
+            store_act2(a.x.out, a.x.type, at + d2, v.z, v.w);
+        }
+    }
+}
+// the same of one m tile (two dims)
+template <typename S>
+__device__ __forceinline__ void write_one(const PagedAttnArgs &a, int r0, int rows, int item, int nt, int m, const float4 &x,
+                                          float inv0, float inv1) {
+    const int lane = threadIdx.x & 31, gid = lane >> 2, tig = lane & 3;
+    const int G = a.x.n_heads / a.kv.n_kv_heads, R = rows * G, nrb = (R + S::kRows - 1) / S::kRows;
+    const int kh = item / nrb, rb = item % nrb;
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+        const int r = rb * S::kRows + 8 * nt + 2 * tig + c;
+        if (r >= R) continue;
+        const int64_t at = static_cast<int64_t>(r0 + r / G) * a.x.out_stride + static_cast<int64_t>(kh * G + r % G) * S::HD + S::dim(m, gid);
+        store_act2(a.x.out, a.x.type, at, c ? x.y * inv1 : x.x * inv0, c ? x.w * inv1 : x.z * inv0);
     }
 }
 // a row's factor 1 / l (with O's own exponent) from its joined (m, l, m'): zeros where it saw nothing
@@ -229,77 +233,82 @@ struct PagedSegment {   // what a CTA does of one item (48 bytes)
     int kh, rb;         // its key head, its block of rows
 };
 
+// A CTA's share of the work and the way through it. A warp walks for itself (all alike): look() gives the next tile and
+// the page of this lane's position in it; the segments it opens wait in shared memory until the products reach them. The
+// following sequence's plan is loaded a sequence ahead.
+struct PagedTile {
+    int page;    // of this lane's position (-2: it has none)
+    int in_page; // its place there
+    int p0;      // the warp's first position in the tile (-1: no tile)
+    int kh;
+};
+struct PagedWalkShared {
+    int64_t sum[4], base;
+    int seq;
+};
+
 template <typename S>
-__global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn(PagedAttnArgs a) {
-    constexpr int HD = S::HD, NT = S::NT, WR = S::WR, TP = S::TP, MT = S::MT, RB = S::RB, RE = S::RE, E = S::E, OM = S::OM;
-    constexpr int PARTS = S::PARTS, ME = S::ME, EM = S::EM, EPO = S::EPO;
-    constexpr bool I8 = S::I8, BF16 = S::BF16, SPLIT = S::SPLIT;
-    extern __shared__ __align__(128) uint8_t sm[];
-    __shared__ int64_t s_sum[4], s_base;
-    __shared__ int s_seq;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gid = lane >> 2, tig = lane & 3;
-    const int wp = warp / WR, wr = warp % WR;
-    const int G = a.x.n_heads / a.kv.n_kv_heads, cta = blockIdx.x;
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    asm volatile("griddepcontrol.launch_dependents;");
+struct PagedWalk {
+    const PagedAttnArgs &a;
+    PagedSegment *segs;      // this warp's [kSegs]
+    int64_t total, ctas, u, end, base;
+    SeqRows sq, sq_next;
+    const int *pages;        // the segment being looked up: its pages,
+    int p0, n, length, kh;   // next tile's position for this warp, tiles left
+    int seq, opened;
 
-    // this CTA's share [begin, end) of all work: each thread sums a run of sequences, then a scan over the threads
-    if (tid == 0) a.cut[cta] = make_int4(0, 0, 0, 0);
-    const int run = (a.b.n_seq + kPagedAttnThreads - 1) / kPagedAttnThreads;
-    const int s_lo = min(tid * run, a.b.n_seq), s_hi = min(s_lo + run, a.b.n_seq);
-    int64_t mine = 0;
-    for (int s = s_lo; s < s_hi; ++s) mine += seq_cost<S>(a, seq_rows(a.b, a.kv.page_size, s, a.status));
-    int64_t before = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int64_t v = __shfl_up_sync(0xffffffffu, before, o);
-        if (lane >= o) before += v;
+    __device__ __forceinline__ SeqRows load(int s) const {
+        return s < a.b.n_seq ? seq_rows(a.b, a.kv.page_size, s, a.status) : SeqRows{0, 0, 0};
     }
-    if (lane == 31) s_sum[warp] = before;
-    __syncthreads();
-    before -= mine;
-    int64_t total = 0;
+    // This CTA's share [u, end) of all work: each thread sums a run of sequences, then a scan over the threads. False:
+    // nothing for this CTA.
+    __device__ __forceinline__ bool start(PagedWalkShared &sh) {
+        const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, cta = blockIdx.x;
+        const int run = (a.b.n_seq + kPagedAttnThreads - 1) / kPagedAttnThreads;
+        const int s_lo = min(tid * run, a.b.n_seq), s_hi = min(s_lo + run, a.b.n_seq);
+        int64_t mine = 0;
+        for (int s = s_lo; s < s_hi; ++s) mine += seq_cost<S>(a, load(s));
+        int64_t before = mine;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-        if (w < warp) before += s_sum[w];
-        total += s_sum[w];
-    }
-    const int64_t ctas = min(static_cast<int64_t>(gridDim.x), total);
-    if (cta >= ctas) return;
-    const int64_t begin = total * cta / ctas, end = total * (cta + 1) / ctas;
-    if (before <= begin && begin < before + mine) {
-        int64_t base = before;
-        int s = s_lo;
-        for (; s < s_hi; ++s) {
-            const int64_t n = seq_cost<S>(a, seq_rows(a.b, a.kv.page_size, s, a.status));
-            if (begin < base + n) break;
-            base += n;
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t v = __shfl_up_sync(0xffffffffu, before, o);
+            if (lane >= o) before += v;
         }
-        s_seq = s;
-        s_base = base;
+        if (lane == 31) sh.sum[warp] = before;
+        __syncthreads();
+        before -= mine;
+        total = 0;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            if (w < warp) before += sh.sum[w];
+            total += sh.sum[w];
+        }
+        ctas = min(static_cast<int64_t>(gridDim.x), total);
+        if (cta >= ctas) return false;
+        u = total * cta / ctas;
+        end = total * (cta + 1) / ctas;
+        if (before <= u && u < before + mine) {
+            int64_t b = before;
+            int s = s_lo;
+            for (; s < s_hi; ++s) {
+                const int64_t c = seq_cost<S>(a, load(s));
+                if (u < b + c) break;
+                b += c;
+            }
+            sh.seq = s;
+            sh.base = b;
+        }
+        __syncthreads();
+        seq = sh.seq;
+        base = sh.base;
+        sq = load(seq);
+        sq_next = load(seq + 1);
+        n = opened = 0;
+        return true;
     }
-    __syncthreads();
-
-    // the queries' fragments (b0, b1) [k step][n tile][lane]; two numbers a value (SPLIT, and int8's a, b): uint4
-    uint2 *q_one = reinterpret_cast<uint2 *>(sm + S::o_q + (I8 ? S::KS / 2 * S::NTT * 32 * 16 : 0));   // (int8: c)
-    uint4 *q_two = reinterpret_cast<uint4 *>(sm + S::o_q);
-    float *col_s = reinterpret_cast<float *>(sm + S::o_col);
-    uint8_t *ring = sm + S::o_ring + wp * E * S::kEntry;
-    uint8_t *scales = sm + S::o_scale + wp * S::TS * S::kScale;
-    PagedSegment *segs = reinterpret_cast<PagedSegment *>(sm + S::o_seg) + warp * S::kSegs;
-    const uint32_t ring_a = smem_addr(ring), scales_a = smem_addr(scales);
-
-    // ---- looking ahead: the next tile of this CTA's share, and the page of this lane's position in it. A warp does this
-    // for itself (all alike); the segments it opens wait in shared memory until the products reach them. The following
-    // sequence's plan is loaded a sequence ahead.
-    int seq = s_seq, opened = 0;
-    int64_t base = s_base, u = begin;
-    auto load_seq = [&](int s) { return s < a.b.n_seq ? seq_rows(a.b, a.kv.page_size, s, a.status) : SeqRows{0, 0, 0}; };
-    SeqRows sq = load_seq(seq), sq_next = load_seq(seq + 1);
-    int at_p0 = 0, at_n = 0, at_length = 0, at_kh = 0;   // the segment being looked up: next tile's position, tiles left
-    const int *at_pages = nullptr;
-    auto open = [&]() {   // the next segment with tiles (none left: at_n 0)
-        while (at_n == 0 && u < end) {
+    __device__ __forceinline__ void open() {   // the next segment with tiles (none left: n 0)
+        const int G = a.x.n_heads / a.kv.n_kv_heads, warp = threadIdx.x >> 5;
+        while (n == 0 && u < end) {
             if (sq.rows > 0) {
                 PagedSegment g;
                 g.r0 = sq.r0, g.rows = sq.rows, g.length = sq.length;
@@ -307,142 +316,66 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn(PagedAttnAr
                 const int nrb = (sq.rows * G + S::kRows - 1) / S::kRows, per = S::kItemCost + g.tps;
                 const int64_t off = u - base;
                 g.item = static_cast<int>(off / per);
-                const int o = static_cast<int>(off % per), n = static_cast<int>(min(static_cast<int64_t>(per - o), end - u));
+                const int o = static_cast<int>(off % per), m = static_cast<int>(min(static_cast<int64_t>(per - o), end - u));
                 g.t0 = max(0, o - S::kItemCost);
-                g.n = max(0, o + n - S::kItemCost) - g.t0;
+                g.n = max(0, o + m - S::kItemCost) - g.t0;
                 // (the CTA that holds the item's last tile, by the shares' own division)
-                g.parts = g.t0 == 0 && g.n < g.tps ? static_cast<int>(((u - o + per) * ctas - 1) / total) - cta + 1 : 0;
+                g.parts = g.t0 == 0 && g.n < g.tps ? static_cast<int>(((u - o + per) * ctas - 1) / total) - static_cast<int>(blockIdx.x) + 1 : 0;
                 g.no = opened;
                 g.kh = g.item / nrb;
                 g.rb = g.item % nrb;
                 if (g.n > 0) {
-                    at_n = g.n;
-                    at_p0 = g.lo + g.t0 * S::CT + wp * TP;
-                    at_length = g.length;
-                    at_kh = g.kh;
-                    at_pages = a.b.pages + seq * a.b.pages_stride;
-                    if (lane == 0) segs[opened % S::kSegs] = g;
+                    n = g.n;
+                    p0 = g.lo + g.t0 * S::CT + warp * S::TP;
+                    length = g.length;
+                    kh = g.kh;
+                    pages = a.b.pages + seq * a.b.pages_stride;
+                    if ((threadIdx.x & 31) == 0) segs[opened % S::kSegs] = g;
                     ++opened;
                 }
-                u += n;
+                u += m;
                 if (u - base < static_cast<int64_t>(per) * a.kv.n_kv_heads * nrb) continue;
                 base = u;
             }
             ++seq;
             sq = sq_next;
-            sq_next = load_seq(seq + 1);
+            sq_next = load(seq + 1);
         }
-    };
-    struct Tile {
-        int page;    // of this lane's position (-2: it has none)
-        int in_page; // its place there
-        int p0;      // the tile's first position (-1: no tile)
-        int kh;
-    };
-    auto look = [&]() {
+    }
+    __device__ __forceinline__ PagedTile look() {
         open();
-        if (at_n == 0) return Tile{-2, 0, -1, 0};
-        const int p = at_p0 + lane, n = static_cast<int>((static_cast<uint64_t>(p) * a.page_mul) >> a.page_shift);
-        Tile t{-2, p - n * a.kv.page_size, at_p0, at_kh};
-        if (p < at_length) t.page = at_pages[n];
-        at_p0 += S::CT;
-        --at_n;
+        if (n == 0) return PagedTile{-2, 0, -1, 0};
+        const int lane = threadIdx.x & 31, p = p0 + lane, k = static_cast<int>((static_cast<uint64_t>(p) * a.page_mul) >> a.page_shift);
+        PagedTile t{-2, p - k * a.kv.page_size, p0, kh};
+        if (lane < S::TP && p < length) t.page = pages[k];
+        p0 += S::CT;
+        --n;
         return t;
-    };
-    Tile ahead0 = look(), ahead1 = look();
+    }
+};
 
-    // ---- the copies: entry by entry through the tiles looked up. The kind of an entry (0 .. EPO-1: K's, then V's) is known
-    // where it is issued: it follows from the kind that is waited for there.
-    int in_slot = 0, in_tile = 0;   // the ring slot; the tile's place among the scales
-    bool in_any = true, one_page = false;
-    int64_t place = 0;    // value offset of this lane's position
-    uint32_t ok = 0;      // the tile's positions that are on a page
-    auto issue = [&](auto kind_) {
-        constexpr int kind = decltype(kind_)::value % (2 * EPO);
-        if (kind == 0 && in_any) {
-            const Tile t = ahead0;
-            ahead0 = ahead1;
-            ahead1 = look();
-            in_any = t.p0 >= 0;
-            if (in_any) {
-                in_tile = in_tile + 1 == S::TS ? 0 : in_tile + 1;
-                const bool there = t.page >= 0 && t.page < a.kv.n_pages;
-                if (t.page != -2 && !there) atomicOr(a.status, kErrBadShape);
-                place = there ? t.page * a.kv.page_stride + t.in_page * a.kv.pos_stride + t.kh * a.kv.head_stride : 0;
-                ok = __ballot_sync(0xffffffffu, there);
-                // positions one after the other on one page: their rows are pos_stride apart
-                one_page = ok == 0xffffffffu && __shfl_sync(0xffffffffu, t.in_page, 0) + TP <= a.kv.page_size;
-                if (wr == 0) {
-                    const uint32_t d = scales_a + in_tile * S::kScale;
-                    if (lane == 0) *reinterpret_cast<uint32_t *>(scales + in_tile * S::kScale) = ok;
-                    if constexpr (I8) {
-                        const int64_t sp = there ? t.page * a.kv.scale_page_stride + t.in_page * a.kv.scale_pos_stride + t.kh * a.kv.scale_head_stride : 0;
-                        copy4(d + 16 + lane * 4, a.kv.k_scale + sp, there ? 4 : 0);
-                        copy4(d + 16 + (TP + lane) * 4, a.kv.v_scale + sp, there ? 4 : 0);
-                    }
-                }
-            }
+// The segment's queries as fragments (b0, b1) [k step][n tile][lane] and the rows' column factors: warp w takes rows w,
+// w + 4, ..; a lane HD / 32 neighbouring dims; up to five rows' loads in flight.
+template <typename S>
+__device__ __forceinline__ void build_queries(const PagedAttnArgs &a, const PagedSegment &g, uint8_t *sm_q, float *col) {
+    constexpr bool I8 = S::I8, BF16 = S::BF16, SPLIT = S::SPLIT;
+    constexpr int HD = S::HD, N = HD / 32, B = S::kRows / 4 < 5 ? S::kRows / 4 : 5;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, G = a.x.n_heads / a.kv.n_kv_heads, R = g.rows * G;
+    uint2 *q_one = reinterpret_cast<uint2 *>(sm_q + S::kQTwo);   // (int8: the third digits)
+    uint4 *q_two = reinterpret_cast<uint4 *>(sm_q);              // two numbers a value (SPLIT, and int8's first digits)
+    for (int i0 = warp; i0 < S::kRows; i0 += 4 * B) {
+        float vs[B][N];
+#pragma unroll
+        for (int b = 0; b < B; ++b) {
+            const int r = g.rb * S::kRows + i0 + 4 * b;
+#pragma unroll
+            for (int k = 0; k < N; ++k) vs[b][k] = 0.0f;
+            if (r < R) load_act(vs[b], a.x.q, a.x.type, static_cast<int64_t>(g.r0 + r / G) * a.x.q_stride + static_cast<int64_t>(g.kh * G + r % G) * a.x.q_head_stride + lane * N);
         }
-        if (in_any) {
-            constexpr bool is_v = kind >= EPO;
-            constexpr int first_p = kind % EPO / PARTS * 16 * ME, part = kind % PARTS;
-            const uint8_t *src = static_cast<const uint8_t *>(is_v ? a.kv.v : a.kv.k) + part * RE;
-            constexpr int CH = RE / 16, PR = 32 / CH;   // 16-byte pieces of a row, rows of a warp's copy
-            constexpr int N = 16 * ME * CH / (32 * WR);
-            const int c = lane % CH;
-            const uint32_t dst = ring_a + in_slot * S::kEntry;
-            // pieces swapped within a row so that the fragment loads of K (8 rows x 4 neighbouring pieces) and of V (every
-            // second row x 2 pieces) meet no bank twice
-            auto put = [&](int k, const uint8_t *from, uint32_t bytes) {
-                const int p = (k * WR + wr) * PR + lane / CH;
-                int sw;
-                if (is_v) sw = RE == 64 ? c ^ ((p >> 1 & 1) << 1) : c ^ ((p >> 1 & 3) << 1);
-                else sw = RE == 64 ? c : c ^ ((p & 1) << 2);
-                copy16(dst + p * RE + sw * 16, from, bytes);
-            };
-            if (one_page) {
-                const int64_t step = a.kv.pos_stride * S::ES;
-                const uint8_t *from = src + __shfl_sync(0xffffffffu, place, first_p) * S::ES + (wr * PR + lane / CH) * step + c * 16;
 #pragma unroll
-                for (int k = 0; k < N; ++k) put(k, from, 16), from += step * (PR * WR);
-            } else {
-#pragma unroll
-                for (int k = 0; k < N; ++k) {
-                    const int p = first_p + (k * WR + wr) * PR + lane / CH;
-                    const int64_t x = __shfl_sync(0xffffffffu, place, p);
-                    put(k, src + x * S::ES + c * 16, (ok >> p & 1) ? 16 : 0);
-                }
-            }
-        }
-        in_slot = in_slot + 1 == E ? 0 : in_slot + 1;
-        asm volatile("cp.async.commit_group;" ::: "memory");
-    };
-    in_tile = S::TS - 1;
-    for_kinds(issue, std::make_integer_sequence<int, E - 1>{});
-    __syncwarp();   // (the first segments are written)
-
-    int slot = 0, tile_at = 0;   // the products' place in the ring and among the scales
-    auto next_entry = [&](auto kind_) {   // the entry at `slot`, of this kind, has landed; the one before it is free for a copy
-        asm volatile("cp.async.wait_group %0;" ::"n"(E - 2) : "memory");
-        if constexpr (WR == 1) __syncwarp();
-        else __syncthreads();
-        issue(std::integral_constant<int, decltype(kind_)::value + E - 1>{});
-        const uint8_t *ent = ring + slot * S::kEntry;
-        slot = slot + 1 == E ? 0 : slot + 1;
-        return ent;
-    };
-
-    for (int done = 0; done < opened; ++done) {
-        const PagedSegment g = segs[done % S::kSegs];
-        const int R = g.rows * G;
-        // ---- the queries as fragments: warp w takes rows w, w + 4, ..; lane HD / 32 neighbouring dims
-        for (int i = warp; i < S::kRows; i += 4) {
-            constexpr int N = HD / 32;
-            const int r = g.rb * S::kRows + i;
-            float v[N], top = 0.0f;
-            const int64_t at = r < R ? static_cast<int64_t>(g.r0 + r / G) * a.x.q_stride + static_cast<int64_t>(g.kh * G + r % G) * a.x.q_head_stride + lane * N : 0;
-#pragma unroll
-            for (int k = 0; k < N; ++k) v[k] = r < R ? load_act(a.x.q, a.x.type, at + k) : 0.0f;
+        for (int b = 0; b < B; ++b) {
+            const int i = i0 + 4 * b;
+            float (&v)[N] = vs[b], top = 0.0f;
             const int nt = i >> 3, n = i & 7;
             if constexpr (I8) {
 #pragma unroll
@@ -450,7 +383,7 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn(PagedAttnAr
 #pragma unroll
                 for (int x = 16; x > 0; x >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, x));
                 const float inv = top > 0.0f ? 127.0f / top : 0.0f;
-                if (lane == 0) col_s[i] = a.x.scale * 1.44269504088896341f * (top * (1.0f / 127.0f));
+                if (lane == 0) col[i] = a.x.scale * 1.44269504088896341f * (top * (1.0f / 127.0f));
                 constexpr int W = N < 4 ? N : 4;   // neighbouring dims stored together
 #pragma unroll
                 for (int k = 0; k < N; k += W) {
@@ -465,10 +398,10 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn(PagedAttnAr
                             r = (r - static_cast<float>(digit)) * 254.0f;
                         }
                     }
-                    const int d = lane * N + k, ks = d / 64 * 2 + d % 16 / 8, t = d % 64 / 16, b = d % 8 / 4;
-                    const int f = (ks * S::NTT + nt) * 32 + n * 4 + t;
-                    uint32_t *const at3[3] = {reinterpret_cast<uint32_t *>(q_two + f) + b, reinterpret_cast<uint32_t *>(q_two + f) + 2 + b,
-                                              reinterpret_cast<uint32_t *>(q_one + f) + b};
+                    const int d = lane * N + k, ks = d / 64 * 2 + d % 16 / 8, t = d % 64 / 16, half = d % 8 / 4;
+                    const int f = (ks * S::NT + nt) * 32 + n * 4 + t;
+                    uint32_t *const at3[3] = {reinterpret_cast<uint32_t *>(q_two + f) + half, reinterpret_cast<uint32_t *>(q_two + f) + 2 + half,
+                                              reinterpret_cast<uint32_t *>(q_one + f) + half};
 #pragma unroll
                     for (int y = 0; y < 3; ++y)
                         if constexpr (W == 4) *at3[y] = w[y];
@@ -485,23 +418,167 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn(PagedAttnAr
 #pragma unroll
                     for (int k = 0; k < N; ++k) v[k] = scalbnf(v[k], -ex);
                 }
-                if (lane == 0) col_s[i] = scalbnf(a.x.scale * 1.44269504088896341f, ex);
+                if (lane == 0) col[i] = scalbnf(a.x.scale * 1.44269504088896341f, ex);
 #pragma unroll
                 for (int k = 0; k < N; k += 2) {
                     // (a 16-byte piece has 8 dims, 2 k steps; 4 lanes' pieces lie side by side)
-                    const int d = lane * N + k, ks = d / 32 * 2 + d % 8 / 4, t = d % 32 / 8, b = d % 4 / 2;
-                    const int f = (ks * S::NTT + nt) * 32 + n * 4 + t;
+                    const int d = lane * N + k, ks = d / 32 * 2 + d % 8 / 4, t = d % 32 / 8, half = d % 4 / 2;
+                    const int f = (ks * S::NT + nt) * 32 + n * 4 + t;
                     const uint32_t hi = pack2<BF16>(v[k], v[k + 1]);
                     if constexpr (SPLIT) {
                         const float2 h = unpack2<BF16>(hi);
-                        reinterpret_cast<uint32_t *>(q_two + f)[b] = hi;
-                        reinterpret_cast<uint32_t *>(q_two + f)[2 + b] = pack2<BF16>(v[k] - h.x, v[k + 1] - h.y);
+                        reinterpret_cast<uint32_t *>(q_two + f)[half] = hi;
+                        reinterpret_cast<uint32_t *>(q_two + f)[2 + half] = pack2<BF16>(v[k] - h.x, v[k + 1] - h.y);
                     } else {
-                        reinterpret_cast<uint32_t *>(q_one + f)[b] = hi;
+                        reinterpret_cast<uint32_t *>(q_one + f)[half] = hi;
                     }
                 }
             }
         }
+    }
+}
+
+// Shapes of k_paged_attn: 8 query rows, each warp with positions of its own. An entry of the ring is K's or V's rows of ME m
+// tiles (16 positions each), at most 256 bytes of a row; a tile is EPO entries of K, then as many of V.
+template <int HD_, int CACHE_, bool SPLIT_>
+struct PagedShape : PagedBase<HD_, CACHE_, SPLIT_, 1> {
+    using B = PagedBase<HD_, CACHE_, SPLIT_, 1>;
+    using B::RB, B::I8, B::OM, B::ES, B::kRows;
+    static constexpr int RE = RB < 256 ? RB : 256, PARTS = RB / RE;
+    static constexpr int MT = 2, TP = 16 * MT;                    // m tiles, positions of a warp's tile
+    static constexpr int ME = RB < 256 ? 2 : 1, EM = MT / ME, EPO = EM * PARTS;
+    static constexpr int CT = 4 * TP;                             // positions of a CTA's tile
+    // an item's beginning and end cost about what 64 KB of rows do
+    static constexpr int kItemCost = 65536 / (2 * CT * RB) > 0 ? 65536 / (2 * CT * RB) : 1;
+    static constexpr int kEntry = 16 * ME * RE;
+    static constexpr int kRing = 16 * 1024;                       // bytes of a warp's ring
+    static constexpr int E = kRing / kEntry < 12 ? kRing / kEntry : 12;
+    static constexpr int TS = E / (2 * EPO) + 2;                  // tiles whose scales and valid bits are kept
+    static constexpr int kScale = (I8 ? 2 * TP * 4 : 0) + 16;
+    static constexpr int kSegs = E / (2 * EPO) + 5;               // segments looked up, not yet done
+    static constexpr int o_q = 0, o_ring = o_q + B::kQ, o_scale = o_ring + 4 * E * kEntry;
+    static constexpr int o_col = o_scale + 4 * TS * kScale;       // [kRows] column factor
+    static constexpr int o_seg = o_col + kRows * 4;               // [warp][kSegs]
+    static constexpr int o_stat = o_seg + 4 * kSegs * 48;         // [warp][kRows] m, l, m'
+    static constexpr int o_join = o_stat + 4 * kRows * 16;        // [warp][m tile][lane] O
+    static constexpr int kSmem = o_join + 4 * OM * 32 * 16;
+    static_assert(E >= 3, "two entries in flight");
+    // the dims of m tile m's rows gid and gid + 8 (the first of the two neighbours): a lane's 8th of a row is taken in
+    // pieces of at most 16 bytes, 8 pieces side by side
+    static __device__ __forceinline__ int dim(int m, int gid) {
+        constexpr int PB = RB / 8 < 16 ? RB / 8 : 16, DPP = PB / ES;
+        return 2 * m / DPP * 8 * DPP + gid * DPP + 2 * m % DPP;
+    }
+};
+
+// Eight query rows or fewer: each of the four warps takes positions of its own, keeps a running maximum, sum and output
+// over them and meets the others only at an item's end.
+template <typename S>
+__global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn(PagedAttnArgs a) {
+    constexpr int NT = 1, TP = S::TP, MT = S::MT, RE = S::RE, E = S::E, OM = S::OM, PARTS = S::PARTS, ME = S::ME, EPO = S::EPO;
+    constexpr bool I8 = S::I8, BF16 = S::BF16, SPLIT = S::SPLIT;
+    extern __shared__ __align__(128) uint8_t sm[];
+    __shared__ PagedWalkShared sh;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gid = lane >> 2, tig = lane & 3;
+    const int G = a.x.n_heads / a.kv.n_kv_heads, cta = blockIdx.x;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;");
+    if (tid == 0) a.cut[cta] = make_int4(0, 0, 0, 0);
+    PagedWalk<S> walk{a, reinterpret_cast<PagedSegment *>(sm + S::o_seg) + warp * S::kSegs};
+    if (!walk.start(sh)) return;
+
+    // the queries' fragments (b0, b1) [k step][n tile][lane]; two numbers a value (SPLIT, and int8's a, b): uint4
+    uint2 *q_one = reinterpret_cast<uint2 *>(sm + S::o_q + S::kQTwo);   // (int8: c)
+    uint4 *q_two = reinterpret_cast<uint4 *>(sm + S::o_q);
+    float *col_s = reinterpret_cast<float *>(sm + S::o_col);
+    uint8_t *ring = sm + S::o_ring + warp * E * S::kEntry;
+    uint8_t *scales = sm + S::o_scale + warp * S::TS * S::kScale;
+    const uint32_t ring_a = smem_addr(ring), scales_a = smem_addr(scales);
+
+    PagedTile ahead0 = walk.look(), ahead1 = walk.look();
+
+    // ---- the copies: entry by entry through the tiles looked up. The kind of an entry (0 .. EPO-1: K's, then V's) is known
+    // where it is issued: it follows from the kind that is waited for there.
+    int in_slot = 0, in_tile = 0;   // the ring slot; the tile's place among the scales
+    bool in_any = true, one_page = false;
+    int64_t place = 0;    // value offset of this lane's position
+    uint32_t ok = 0;      // the tile's positions that are on a page
+    auto issue = [&](auto kind_) {
+        constexpr int kind = decltype(kind_)::value % (2 * EPO);
+        if (kind == 0 && in_any) {
+            const PagedTile t = ahead0;
+            ahead0 = ahead1;
+            ahead1 = walk.look();
+            in_any = t.p0 >= 0;
+            if (in_any) {
+                in_tile = in_tile + 1 == S::TS ? 0 : in_tile + 1;
+                const bool there = t.page >= 0 && t.page < a.kv.n_pages;
+                if (t.page != -2 && !there) atomicOr(a.status, kErrBadShape);
+                place = there ? t.page * a.kv.page_stride + t.in_page * a.kv.pos_stride + t.kh * a.kv.head_stride : 0;
+                ok = __ballot_sync(0xffffffffu, there);
+                // positions one after the other on one page: their rows are pos_stride apart
+                one_page = ok == 0xffffffffu && __shfl_sync(0xffffffffu, t.in_page, 0) + TP <= a.kv.page_size;
+                const uint32_t d = scales_a + in_tile * S::kScale;
+                if (lane == 0) *reinterpret_cast<uint32_t *>(scales + in_tile * S::kScale) = ok;
+                if constexpr (I8) {
+                    const int64_t sp = there ? t.page * a.kv.scale_page_stride + t.in_page * a.kv.scale_pos_stride + t.kh * a.kv.scale_head_stride : 0;
+                    copy4(d + 16 + lane * 4, a.kv.k_scale + sp, there ? 4 : 0);
+                    copy4(d + 16 + (TP + lane) * 4, a.kv.v_scale + sp, there ? 4 : 0);
+                }
+            }
+        }
+        if (in_any) {
+            constexpr bool is_v = kind >= EPO;
+            constexpr int first_p = kind % EPO / PARTS * 16 * ME, part = kind % PARTS;
+            const uint8_t *src = static_cast<const uint8_t *>(is_v ? a.kv.v : a.kv.k) + part * RE;
+            constexpr int CH = RE / 16, PR = 32 / CH;   // 16-byte pieces of a row, rows of a warp's copy
+            constexpr int N = 16 * ME * CH / 32;
+            const int c = lane % CH;
+            const uint32_t dst = ring_a + in_slot * S::kEntry;
+            // pieces swapped within a row so that the fragment loads of K (8 rows x 4 neighbouring pieces) and of V (every
+            // second row x 2 pieces) meet no bank twice
+            auto put = [&](int k, const uint8_t *from, uint32_t bytes) {
+                const int p = k * PR + lane / CH;
+                int sw;
+                if (is_v) sw = RE == 64 ? c ^ ((p >> 1 & 1) << 1) : c ^ ((p >> 1 & 3) << 1);
+                else sw = RE == 64 ? c : c ^ ((p & 1) << 2);
+                copy16(dst + p * RE + sw * 16, from, bytes);
+            };
+            if (one_page) {
+                const int64_t step = a.kv.pos_stride * S::ES;
+                const uint8_t *from = src + __shfl_sync(0xffffffffu, place, first_p) * S::ES + lane / CH * step + c * 16;
+#pragma unroll
+                for (int k = 0; k < N; ++k) put(k, from, 16), from += step * PR;
+            } else {
+#pragma unroll
+                for (int k = 0; k < N; ++k) {
+                    const int p = first_p + k * PR + lane / CH;
+                    const int64_t x = __shfl_sync(0xffffffffu, place, p);
+                    put(k, src + x * S::ES + c * 16, (ok >> p & 1) ? 16 : 0);
+                }
+            }
+        }
+        in_slot = in_slot + 1 == E ? 0 : in_slot + 1;
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    in_tile = S::TS - 1;
+    for_kinds(issue, std::make_integer_sequence<int, E - 1>{});
+    __syncwarp();   // (the first segments are written)
+
+    int slot = 0, tile_at = 0;   // the products' place in the ring and among the scales
+    auto next_entry = [&](auto kind_) {   // the entry at `slot`, of this kind, has landed; the one before it is free for a copy
+        asm volatile("cp.async.wait_group %0;" ::"n"(E - 2) : "memory");
+        __syncwarp();
+        issue(std::integral_constant<int, decltype(kind_)::value + E - 1>{});
+        const uint8_t *ent = ring + slot * S::kEntry;
+        slot = slot + 1 == E ? 0 : slot + 1;
+        return ent;
+    };
+
+    for (int done = 0; done < walk.opened; ++done) {
+        const PagedSegment g = walk.segs[done % S::kSegs];
+        const int R = g.rows * G;
+        build_queries<S>(a, g, sm + S::o_q, col_s);
         __syncthreads();
 
         // ---- this lane's columns: rows 2 tig, 2 tig + 1 of each of the warp's n tiles
@@ -511,7 +588,7 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn(PagedAttnAr
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                const int i = 8 * (wr * NT + nt) + 2 * tig + c, r = g.rb * S::kRows + i;
+                const int i = 8 * nt + 2 * tig + c, r = g.rb * S::kRows + i;
                 col[nt][c] = col_s[i];
                 lim[nt][c] = r < R ? g.length - g.rows + r / G : -1;
                 m[nt][c] = mo[nt][c] = -INFINITY;
@@ -528,10 +605,9 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn(PagedAttnAr
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int c = 0; c < 4; ++c) o[k][nt][c] = 0.0f;
-        const bool busy = g.rb * S::kRows + 8 * wr * NT < R;   // this warp has rows
 
         for (int i = 0; i < g.n; ++i) {
-            const int p0 = g.lo + (g.t0 + i) * S::CT + wp * TP;
+            const int p0 = g.lo + (g.t0 + i) * S::CT + warp * TP;
             uint32_t ph[MT][NT][2], pl[MT][NT][2];   // the weights as fragments: (b0, b1), and what is left of them
             bool edge;
             {
@@ -540,7 +616,6 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn(PagedAttnAr
                 auto k_entry = [&](auto kind_) {
                     constexpr int kind = decltype(kind_)::value, m0 = kind / PARTS * ME, part = kind % PARTS;
                     const uint8_t *ent = next_entry(kind_);
-                    if (!busy) return;
                     auto piece = [&](int mt, int h, int j) {   // the 4 neighbouring lanes' 16 bytes of row gid + 8 h
                         const int p = 16 * mt + 8 * h + gid, c = 4 * j + tig, sw = RE == 64 ? c : c ^ ((p & 1) << 2);
                         return *reinterpret_cast<const uint4 *>(ent + p * RE + sw * 16);
@@ -565,7 +640,7 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn(PagedAttnAr
                             for (int w = 0; w < 2; ++w)
 #pragma unroll
                                 for (int nt = 0; nt < NT; ++nt) {
-                                    const int f = ((2 * j + w) * S::NTT + wr * NT + nt) * 32 + lane;
+                                    const int f = ((2 * j + w) * NT + nt) * 32 + lane;
                                     const uint4 ab = q_two[f];
                                     const uint2 cc = q_one[f];
 #pragma unroll
@@ -603,7 +678,7 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn(PagedAttnAr
                             for (int w = 0; w < 2; ++w)
 #pragma unroll
                                 for (int nt = 0; nt < NT; ++nt) {
-                                    const int f = ((2 * (part * (RE / 64) + j) + w) * S::NTT + wr * NT + nt) * 32 + lane;
+                                    const int f = ((2 * (part * (RE / 64) + j) + w) * NT + nt) * 32 + lane;
                                     const uint4 b2 = SPLIT ? q_two[f] : make_uint4(0, 0, 0, 0);
                                     const uint2 b = SPLIT ? make_uint2(b2.x, b2.y) : q_one[f];
 #pragma unroll
@@ -727,7 +802,6 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn(PagedAttnAr
             auto v_entry = [&](auto kind_) {
                 constexpr int m0 = (decltype(kind_)::value - EPO) / PARTS * ME, part = decltype(kind_)::value % PARTS;
                 const uint8_t *ent = next_entry(kind_);
-                if (!busy) return;
                 constexpr int PB = RE / 8 < 16 ? RE / 8 : 16, NP = RE / 8 / PB, NW = PB / 4;
                 constexpr int MW = I8 ? 2 : 1;   // m tiles of a word
                 auto v_words = [&](int mt, int np, uint32_t (&x)[4][NW]) {   // positions 2 tig, + 1, + 8, + 9
@@ -747,7 +821,8 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn(PagedAttnAr
                     }
                 };
                 // a row must not be touched by values that it does not see, and zero times an infinity is not zero: at
-                // the edges of what the rows see a 16-bit tile that holds such values goes a token at a time
+                // the edges of what the rows see a 16-bit tile that holds such values goes a token at a time (the same
+                // sums in the same order: bit for bit what finite values there give)
                 bool apart = false;
                 if constexpr (!I8) {
                     if (edge && g.rows > 1) {
@@ -826,12 +901,14 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn(PagedAttnAr
                                     }
 #pragma unroll
                                     for (int nt = 0; nt < NT; ++nt) {
-                                        float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                                        float d[4];
+#pragma unroll
+                                        for (int x4 = 0; x4 < 4; ++x4) d[x4] = o[(part * NP + np) * NW + w][nt][x4];
                                         mma_16816<BF16>(d, va[0], va[1], va[2], va[3], ph[m0 + mt][nt][0], ph[m0 + mt][nt][1]);
                                         if constexpr (SPLIT) mma_16816<BF16>(d, va[0], va[1], va[2], va[3], pl[m0 + mt][nt][0], pl[m0 + mt][nt][1]);
 #pragma unroll
                                         for (int x4 = 0; x4 < 4; ++x4)
-                                            if (lim[nt][x4 & 1] - p0 == hi_p && lim[nt][x4 & 1] >= 0) o[(part * NP + np) * NW + w][nt][x4] += d[x4];
+                                            if (lim[nt][x4 & 1] - p0 == hi_p && lim[nt][x4 & 1] >= 0) o[(part * NP + np) * NW + w][nt][x4] = d[x4];
                                     }
                                 }
                             }
@@ -853,94 +930,64 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn(PagedAttnAr
         const bool whole = g.t0 == 0 && g.n == g.tps;
         const int keep_slot = 2 * cta + (g.no == 0 ? 0 : 1);
         if (g.parts > 0 && tid == 0) a.cut[cta] = make_int4(2 * g.parts + (keep_slot & 1), g.item, g.r0, g.rows);
-        if constexpr (WR == 1) {
-            float4 *stat = reinterpret_cast<float4 *>(sm + S::o_stat);
-            float4 *buf = reinterpret_cast<float4 *>(sm + S::o_join);   // [group][m tile][lane], an n tile at a time
-            if (gid == 0)
+        float4 *stat = reinterpret_cast<float4 *>(sm + S::o_stat);
+        float4 *buf = reinterpret_cast<float4 *>(sm + S::o_join);   // [group][m tile][lane], an n tile at a time
+        if (gid == 0)
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                    for (int c = 0; c < 2; ++c) stat[warp * S::kRows + 8 * nt + 2 * tig + c] = make_float4(m[nt][c], l[nt][c], mo[nt][c], 0.0f);
+                for (int c = 0; c < 2; ++c) stat[warp * S::kRows + 8 * nt + 2 * tig + c] = make_float4(m[nt][c], l[nt][c], mo[nt][c], 0.0f);
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                if (nt > 0) __syncthreads();
+        for (int nt = 0; nt < NT; ++nt) {
+            if (nt > 0) __syncthreads();
 #pragma unroll
-                for (int k = 0; k < OM; ++k)
-                    buf[(warp * OM + k) * 32 + lane] = make_float4(o[k][nt][0], o[k][nt][1], o[k][nt][2], o[k][nt][3]);
-                __syncthreads();   // (the queries' fragments are free from here, the buffer after the next barrier)
-                float M[2] = {-INFINITY, -INFINITY}, Mo[2] = {-INFINITY, -INFINITY}, Ls[2] = {0.0f, 0.0f}, f[4][2];
-                float4 st[4][2];
+            for (int k = 0; k < OM; ++k)
+                buf[(warp * OM + k) * 32 + lane] = make_float4(o[k][nt][0], o[k][nt][1], o[k][nt][2], o[k][nt][3]);
+            __syncthreads();   // (the queries' fragments are free from here, the buffer after the next barrier)
+            float M[2] = {-INFINITY, -INFINITY}, Mo[2] = {-INFINITY, -INFINITY}, Ls[2] = {0.0f, 0.0f}, f[4][2];
+            float4 st[4][2];
 #pragma unroll
-                for (int w = 0; w < 4; ++w)
+            for (int w = 0; w < 4; ++w)
 #pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        st[w][c] = stat[w * S::kRows + 8 * nt + 2 * tig + c];
-                        M[c] = fmaxf(M[c], st[w][c].x);
-                        Mo[c] = fmaxf(Mo[c], st[w][c].z);
-                    }
+                for (int c = 0; c < 2; ++c) {
+                    st[w][c] = stat[w * S::kRows + 8 * nt + 2 * tig + c];
+                    M[c] = fmaxf(M[c], st[w][c].x);
+                    Mo[c] = fmaxf(Mo[c], st[w][c].z);
+                }
 #pragma unroll
-                for (int w = 0; w < 4; ++w)
+            for (int w = 0; w < 4; ++w)
 #pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        Ls[c] += st[w][c].x == -INFINITY ? 0.0f : st[w][c].y * ex2(st[w][c].x - M[c]);
-                        f[w][c] = st[w][c].z == -INFINITY ? 0.0f : ex2(st[w][c].z - Mo[c]);
-                    }
-                const float inv0 = row_factor(M[0], Ls[0], Mo[0]), inv1 = row_factor(M[1], Ls[1], Mo[1]);
-                for (int k = 2 * warp; k < OM; k += 8) {
-                    float4 v[2];
+                for (int c = 0; c < 2; ++c) {
+                    Ls[c] += st[w][c].x == -INFINITY ? 0.0f : st[w][c].y * ex2(st[w][c].x - M[c]);
+                    f[w][c] = st[w][c].z == -INFINITY ? 0.0f : ex2(st[w][c].z - Mo[c]);
+                }
+            const float inv0 = row_factor(M[0], Ls[0], Mo[0]), inv1 = row_factor(M[1], Ls[1], Mo[1]);
+            for (int k = 2 * warp; k < OM; k += 8) {
+                float4 v[2];
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        v[h] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                for (int h = 0; h < 2; ++h) {
+                    v[h] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-                        for (int w = 0; w < 4; ++w) {
-                            const float4 x = buf[(w * OM + k + h) * 32 + lane];
-                            v[h].x += x.x * f[w][0], v[h].y += x.y * f[w][1], v[h].z += x.z * f[w][0], v[h].w += x.w * f[w][1];
-                        }
-                    }
-                    if (whole) {
-                        write_out<S>(a, g.r0, g.rows, g.item, nt, k, v[0], v[1], inv0, inv1);
-                    } else {
-                        float4 *d = a.part + ((static_cast<int64_t>(keep_slot) * NT + nt) * OM + k) * 32 + lane;
-                        d[0] = v[0];
-                        d[32] = v[1];
+                    for (int w = 0; w < 4; ++w) {
+                        const float4 x = buf[(w * OM + k + h) * 32 + lane];
+                        v[h].x += x.x * f[w][0], v[h].y += x.y * f[w][1], v[h].z += x.z * f[w][0], v[h].w += x.w * f[w][1];
                     }
                 }
-                if (warp == 0 && gid == 0)
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        const int i = 8 * nt + 2 * tig + c;
-                        if (whole) write_lse<S>(a, g.r0, g.rows, g.item, i, M[c], Ls[c]);
-                        else a.stats[static_cast<int64_t>(keep_slot) * S::kRows + i] = make_float4(M[c], Ls[c], Mo[c], 0.0f);
-                    }
-            }
-        } else {
-            if (busy) {
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    const int n = wr * NT + nt;
-                    const float inv0 = row_factor(m[nt][0], l[nt][0], mo[nt][0]), inv1 = row_factor(m[nt][1], l[nt][1], mo[nt][1]);
-#pragma unroll
-                    for (int k = 0; k < OM; k += 2) {
-                        const float4 v0 = make_float4(o[k][nt][0], o[k][nt][1], o[k][nt][2], o[k][nt][3]);
-                        const float4 v1 = make_float4(o[k + 1][nt][0], o[k + 1][nt][1], o[k + 1][nt][2], o[k + 1][nt][3]);
-                        if (whole) {
-                            write_out<S>(a, g.r0, g.rows, g.item, n, k, v0, v1, inv0, inv1);
-                        } else {
-                            float4 *d = a.part + ((static_cast<int64_t>(keep_slot) * S::NTT + n) * OM + k) * 32 + lane;
-                            d[0] = v0;
-                            d[32] = v1;
-                        }
-                    }
-                    if (gid == 0)
-#pragma unroll
-                        for (int c = 0; c < 2; ++c) {
-                            const int i = 8 * n + 2 * tig + c;
-                            if (whole) write_lse<S>(a, g.r0, g.rows, g.item, i, m[nt][c], l[nt][c]);
-                            else a.stats[static_cast<int64_t>(keep_slot) * S::kRows + i] = make_float4(m[nt][c], l[nt][c], mo[nt][c], 0.0f);
-                        }
+                if (whole) {
+                    write_out<S>(a, g.r0, g.rows, g.item, nt, k, v[0], v[1], inv0, inv1);
+                } else {
+                    float4 *d = a.part + ((static_cast<int64_t>(keep_slot) * NT + nt) * OM + k) * 32 + lane;
+                    d[0] = v[0];
+                    d[32] = v[1];
                 }
             }
-            __syncthreads();   // every warp is through with the queries' fragments
+            if (warp == 0 && gid == 0)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const int i = 8 * nt + 2 * tig + c;
+                    if (whole) write_lse<S>(a, g.r0, g.rows, g.item, i, M[c], Ls[c]);
+                    else a.stats[static_cast<int64_t>(keep_slot) * S::kRows + i] = make_float4(M[c], Ls[c], Mo[c], 0.0f);
+                }
         }
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -987,7 +1034,7 @@ __global__ void __launch_bounds__(kJoinThreads, 2) k_paged_attn_join(PagedAttnAr
     auto slot = [&](int k) { return static_cast<int64_t>(2 * (c + k) + (k == 0 ? item.x & 1 : 0)); };
     const int nt = unit / (OM / 2), k2 = unit % (OM / 2) * 2;
     const int G = a.x.n_heads / a.kv.n_kv_heads, R = item.w * G, nrb = (R + S::kRows - 1) / S::kRows;
-    const bool live = nt < S::NTT && item.y % nrb * S::kRows + 8 * nt < R;
+    const bool live = nt < S::NT && item.y % nrb * S::kRows + 8 * nt < R;
     constexpr int B = 4;   // parts whose loads are in flight together
     float M[2] = {-INFINITY, -INFINITY}, Mo[2] = {-INFINITY, -INFINITY}, L[2] = {0.0f, 0.0f};
     float4 v[2] = {make_float4(0.0f, 0.0f, 0.0f, 0.0f), make_float4(0.0f, 0.0f, 0.0f, 0.0f)};
@@ -1027,7 +1074,7 @@ __global__ void __launch_bounds__(kJoinThreads, 2) k_paged_attn_join(PagedAttnAr
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 st[b][h] = in ? a.stats[at * S::kRows + 8 * nt + 2 * tig + h] : make_float4(-INFINITY, 0.0f, -INFINITY, 0.0f);
-                x[b][h] = in ? a.part[((at * S::NTT + nt) * OM + k2 + h) * 32 + lane] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                x[b][h] = in ? a.part[((at * S::NT + nt) * OM + k2 + h) * 32 + lane] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             }
         }
         take(st, x);

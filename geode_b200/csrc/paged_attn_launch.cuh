@@ -5,17 +5,17 @@
 #include "device.hpp"
 #include "paged_attn.cuh"
 #include "paged_attn_plan.hpp"
+#include "paged_attn_rows.cuh"
 
 namespace gcu {
 
-template <typename S>
+template <typename S, auto kern>
 int launch_paged_shape(const PagedAttnArgs &a, const PagedAttnPlan &p, cudaStream_t st) {
-    const int grid = p.grid;
-    if (!shared_opt_in<k_paged_attn<S>>(S::kSmem)) return GCUDA_E_CUDA;
-    if (launch_ex(k_paged_attn<S>, dim3(grid), dim3(kPagedAttnThreads), S::kSmem, st, true, a) != cudaSuccess) return GCUDA_E_CUDA;
-    if (grid == 1) return GCUDA_OK;   // (nothing is cut)
-    const int units = S::NTT * S::OM / 2, per = kJoinThreads / 32 / p.split;
-    return launch_ex(k_paged_attn_join<S>, dim3(p.cuts, (units + per - 1) / per), dim3(kJoinThreads), 0, st, true, a, p.split, grid) ==
+    if (!shared_opt_in<kern>(S::kSmem)) return GCUDA_E_CUDA;
+    if (launch_ex(kern, dim3(p.grid), dim3(kPagedAttnThreads), S::kSmem, st, true, a) != cudaSuccess) return GCUDA_E_CUDA;
+    if (p.grid == 1) return GCUDA_OK;   // (nothing is cut)
+    const int units = S::NT * S::OM / 2, per = kJoinThreads / 32 / p.split;
+    return launch_ex(k_paged_attn_join<S>, dim3(p.cuts, (units + per - 1) / per), dim3(kJoinThreads), 0, st, true, a, p.split, p.grid) ==
                    cudaSuccess
                ? GCUDA_OK
                : GCUDA_E_CUDA;
@@ -23,9 +23,12 @@ int launch_paged_shape(const PagedAttnArgs &a, const PagedAttnPlan &p, cudaStrea
 
 template <int CACHE, int HD, bool SPLIT>
 int launch_paged_rows(const PagedAttnArgs &a, const PagedAttnPlan &p, cudaStream_t st) {
-    if (p.rows == 8) return launch_paged_shape<PagedShape<HD, CACHE, SPLIT, 1, 1>>(a, p, st);
-    if (p.rows == 16) return launch_paged_shape<PagedShape<HD, CACHE, SPLIT, 2, 1>>(a, p, st);
-    return launch_paged_shape<PagedShape<HD, CACHE, SPLIT, 2, 4>>(a, p, st);
+    using S8 = PagedShape<HD, CACHE, SPLIT>;
+    using S16 = PagedRowsShape<HD, CACHE, SPLIT, 2>;
+    using S40 = PagedRowsShape<HD, CACHE, SPLIT, 5>;
+    if (p.rows == S8::kRows) return launch_paged_shape<S8, k_paged_attn<S8>>(a, p, st);
+    if (p.rows == S16::kRows) return launch_paged_shape<S16, k_paged_attn_rows<S16>>(a, p, st);
+    return launch_paged_shape<S40, k_paged_attn_rows<S40>>(a, p, st);
 }
 template <int CACHE, int HD>
 int launch_paged_split(const PagedAttnArgs &a, const PagedAttnPlan &p, cudaStream_t st) {

@@ -9,19 +9,19 @@ namespace gcu {
 
 struct PagedAttnArgs;
 struct PagedAttnPlan {
-    int rows;      // query rows of a block (8, 16: position groups of one warp; 64: four warps share the positions)
+    int rows;      // query rows of a block: 8 (k_paged_attn), 16 or 40 (k_paged_attn_rows)
     int grid;      // main CTAs
     int split;     // warps that share an item's parts in the join
     int cuts;      // the join's CTAs: one for each item that may be cut, or (many items, split 1) for each main CTA
     size_t cut, stats, part, total;   // scratch offsets
 };
 
-// Query rows sharing a key head, R = max_rows * n_heads / n_kv_heads, choose the shape: blocks of 8 or 16 rows leave all
-// four warps to the positions; more rows share each position's copy among four warps of 16 rows.
+// Query rows sharing a key head, R = max_rows * n_heads / n_kv_heads, choose the shape: up to 8 leave each warp alone with
+// its positions; more are worked on by all four warps together, in blocks of 16 or 40.
 inline PagedAttnPlan plan_paged_attn(const gcuda_paged_kv &kv, const gcuda_paged_batch &b, int n_heads) {
     PagedAttnPlan p{};
     const int64_t R = static_cast<int64_t>(b.max_rows) * (n_heads / kv.n_kv_heads);
-    p.rows = R <= 8 ? 8 : R <= 16 ? 16 : 64;
+    p.rows = R <= 8 ? 8 : R <= 16 ? 16 : 40;
     // two resident CTAs an SM; no more than there can be work: a tile of 16 positions and an item's cost of up to 32 each
     const int64_t per_seq = std::max<int64_t>(1, (static_cast<int64_t>(b.max_pages) * kv.page_size + 15) / 16);
     const int64_t blocks = (R + p.rows - 1) / p.rows;
