@@ -9,8 +9,8 @@
 //
 // Both products run on the tensor cores (mma.sync m16n8k16, float sums) with the cache as the 16-row operand and the
 // query rows as the 8-column one, so that one token's few rows fill the instruction: S^T = K Q^T, then O^T = V^T P^T.
-// The order of dims inside a product is free as long as both operands agree, so a lane takes 16 consecutive bytes of a
-// cache row as its fragments of several products: no transposition, no staging of widened rows. int8 keys are multiplied
+// K's fragments come by ldmatrix as they lie; V's by rows, positions interleaved by byte permutation (the order of dims in
+// O^T is free): no staging of transposed or widened rows. int8 keys are multiplied
 // as they are (m16n8k32, integer sums); int8 values are widened to f16 in registers (exact).
 //
 // Arithmetic: over an int8 cache a query row is its largest value times (a + (b + c / 254) / 254) / 127 with int8 a, b, c:
@@ -42,7 +42,11 @@ struct PagedAttnArgs {
 };
 
 constexpr int kPagedAttnThreads = 128;
-constexpr float kWeightBias = 14.0f;   // f16 weights reach up to 2^14: the smallest kept is 2^-39 of the largest
+// The maximum that a row's weights are relative to follows the true one only when that is kSlack (in bits) above it: with
+// many rows some maximum grows in nearly every tile, and following each costs a reduction and a rescaling of the outputs
+// (32 verify batches of 5 rows: 125 us with every growth followed). f16 weights start at up to 2^kWeightBias, so they
+// reach 2^14 at most, and the smallest kept is 2^-30 of the largest.
+constexpr float kSlack = 8.0f, kWeightBias = 6.0f;
 
 // What the kernels' shapes share. NT: n tiles (8 query rows each) of an item; ES, RB: bytes of a value, of a row
 template <int HD_, int CACHE_, bool SPLIT_, int NT_>
@@ -116,17 +120,45 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void *src, uint32_t b
 __device__ __forceinline__ void copy4(uint32_t dst, const void *src, uint32_t bytes) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
+// N neighbouring values (2, 4 or 8); wide loads where they are aligned
 template <int N>
 __device__ __forceinline__ void load_act(float (&v)[N], const void *p, int type, int64_t i) {
     if (type == GCUDA_F32) {
+        const float *f = static_cast<const float *>(p) + i;
+        if constexpr (N >= 4) {
+            if ((reinterpret_cast<uintptr_t>(f) & 15) == 0) {
 #pragma unroll
-        for (int k = 0; k < N; ++k) v[k] = static_cast<const float *>(p)[i + k];
-    } else if (type == GCUDA_BF16) {
+                for (int k = 0; k < N; k += 4) {
+                    const float4 x = *reinterpret_cast<const float4 *>(f + k);
+                    v[k] = x.x, v[k + 1] = x.y, v[k + 2] = x.z, v[k + 3] = x.w;
+                }
+                return;
+            }
+        }
 #pragma unroll
-        for (int k = 0; k < N; ++k) v[k] = __bfloat162float(static_cast<const __nv_bfloat16 *>(p)[i + k]);
+        for (int k = 0; k < N; ++k) v[k] = f[k];
+        return;
+    }
+    const uint16_t *h = static_cast<const uint16_t *>(p) + i;
+    uint32_t w[N / 2];
+    if ((reinterpret_cast<uintptr_t>(h) & (2 * N - 1)) == 0) {
+        if constexpr (N == 8) {
+            const uint4 x = *reinterpret_cast<const uint4 *>(h);
+            w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
+        } else if constexpr (N == 4) {
+            const uint2 x = *reinterpret_cast<const uint2 *>(h);
+            w[0] = x.x, w[1] = x.y;
+        } else {
+            w[0] = *reinterpret_cast<const uint32_t *>(h);
+        }
     } else {
 #pragma unroll
-        for (int k = 0; k < N; ++k) v[k] = __half2float(static_cast<const __half *>(p)[i + k]);
+        for (int k = 0; k < N; k += 2) w[k / 2] = h[k] | static_cast<uint32_t>(h[k + 1]) << 16;
+    }
+#pragma unroll
+    for (int k = 0; k < N; k += 2) {
+        const float2 x = type == GCUDA_BF16 ? unpack2<true>(w[k / 2]) : unpack2<false>(w[k / 2]);
+        v[k] = x.x, v[k + 1] = x.y;
     }
 }
 __device__ __forceinline__ void store_act2(void *p, int type, int64_t i, float x, float y) {
@@ -234,8 +266,9 @@ struct PagedSegment {   // what a CTA does of one item (48 bytes)
 };
 
 // A CTA's share of the work and the way through it. A warp walks for itself (all alike): look() gives the next tile and
-// the page of this lane's position in it; the segments it opens wait in shared memory until the products reach them. The
-// following sequence's plan is loaded a sequence ahead.
+// the page of this lane's position in it; the segments it opens wait in shared memory until the products reach them, and
+// so does what only the opening of the next one needs (it would cost the products some thirty registers). The following
+// sequence's plan is loaded a sequence ahead.
 struct PagedTile {
     int page;    // of this lane's position (-2: it has none)
     int in_page; // its place there
@@ -245,24 +278,29 @@ struct PagedTile {
 struct PagedWalkShared {
     int64_t sum[4], base;
     int seq;
+    struct Warp {
+        int64_t total, ctas, u, end, base;
+        SeqRows sq, sq_next;
+        int seq;
+    } warp[4];
 };
 
 template <typename S>
 struct PagedWalk {
     const PagedAttnArgs &a;
+    PagedWalkShared &sh;
     PagedSegment *segs;      // this warp's [kSegs]
-    int64_t total, ctas, u, end, base;
-    SeqRows sq, sq_next;
     const int *pages;        // the segment being looked up: its pages,
     int p0, n, length, kh;   // next tile's position for this warp, tiles left
-    int seq, opened;
+    int opened;
+    bool more;               // work is left behind that segment
 
     __device__ __forceinline__ SeqRows load(int s) const {
         return s < a.b.n_seq ? seq_rows(a.b, a.kv.page_size, s, a.status) : SeqRows{0, 0, 0};
     }
     // This CTA's share [u, end) of all work: each thread sums a run of sequences, then a scan over the threads. False:
     // nothing for this CTA.
-    __device__ __forceinline__ bool start(PagedWalkShared &sh) {
+    __device__ __forceinline__ bool start() {
         const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, cta = blockIdx.x;
         const int run = (a.b.n_seq + kPagedAttnThreads - 1) / kPagedAttnThreads;
         const int s_lo = min(tid * run, a.b.n_seq), s_hi = min(s_lo + run, a.b.n_seq);
@@ -277,16 +315,15 @@ struct PagedWalk {
         if (lane == 31) sh.sum[warp] = before;
         __syncthreads();
         before -= mine;
-        total = 0;
+        int64_t total = 0;
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
             if (w < warp) before += sh.sum[w];
             total += sh.sum[w];
         }
-        ctas = min(static_cast<int64_t>(gridDim.x), total);
+        const int64_t ctas = min(static_cast<int64_t>(gridDim.x), total);
         if (cta >= ctas) return false;
-        u = total * cta / ctas;
-        end = total * (cta + 1) / ctas;
+        const int64_t u = total * cta / ctas;
         if (before <= u && u < before + mine) {
             int64_t b = before;
             int s = s_lo;
@@ -299,28 +336,28 @@ struct PagedWalk {
             sh.base = b;
         }
         __syncthreads();
-        seq = sh.seq;
-        base = sh.base;
-        sq = load(seq);
-        sq_next = load(seq + 1);
+        if (lane == 0) sh.warp[warp] = {total, ctas, u, total * (cta + 1) / ctas, sh.base, load(sh.seq), load(sh.seq + 1), sh.seq};
+        __syncwarp();
         n = opened = 0;
+        more = true;
         return true;
     }
     __device__ __forceinline__ void open() {   // the next segment with tiles (none left: n 0)
         const int G = a.x.n_heads / a.kv.n_kv_heads, warp = threadIdx.x >> 5;
-        while (n == 0 && u < end) {
-            if (sq.rows > 0) {
+        PagedWalkShared::Warp w = sh.warp[warp];
+        while (n == 0 && w.u < w.end) {
+            if (w.sq.rows > 0) {
                 PagedSegment g;
-                g.r0 = sq.r0, g.rows = sq.rows, g.length = sq.length;
-                g.tps = seq_tiles<S>(a, sq, g.lo);
-                const int nrb = (sq.rows * G + S::kRows - 1) / S::kRows, per = S::kItemCost + g.tps;
-                const int64_t off = u - base;
+                g.r0 = w.sq.r0, g.rows = w.sq.rows, g.length = w.sq.length;
+                g.tps = seq_tiles<S>(a, w.sq, g.lo);
+                const int nrb = (g.rows * G + S::kRows - 1) / S::kRows, per = S::kItemCost + g.tps;
+                const int64_t off = w.u - w.base;
                 g.item = static_cast<int>(off / per);
-                const int o = static_cast<int>(off % per), m = static_cast<int>(min(static_cast<int64_t>(per - o), end - u));
+                const int o = static_cast<int>(off % per), m = static_cast<int>(min(static_cast<int64_t>(per - o), w.end - w.u));
                 g.t0 = max(0, o - S::kItemCost);
                 g.n = max(0, o + m - S::kItemCost) - g.t0;
                 // (the CTA that holds the item's last tile, by the shares' own division)
-                g.parts = g.t0 == 0 && g.n < g.tps ? static_cast<int>(((u - o + per) * ctas - 1) / total) - static_cast<int>(blockIdx.x) + 1 : 0;
+                g.parts = g.t0 == 0 && g.n < g.tps ? static_cast<int>(((w.u - o + per) * w.ctas - 1) / w.total) - static_cast<int>(blockIdx.x) + 1 : 0;
                 g.no = opened;
                 g.kh = g.item / nrb;
                 g.rb = g.item % nrb;
@@ -329,22 +366,29 @@ struct PagedWalk {
                     p0 = g.lo + g.t0 * S::CT + warp * S::TP;
                     length = g.length;
                     kh = g.kh;
-                    pages = a.b.pages + seq * a.b.pages_stride;
+                    pages = a.b.pages + w.seq * a.b.pages_stride;
                     if ((threadIdx.x & 31) == 0) segs[opened % S::kSegs] = g;
                     ++opened;
                 }
-                u += m;
-                if (u - base < static_cast<int64_t>(per) * a.kv.n_kv_heads * nrb) continue;
-                base = u;
+                w.u += m;
+                if (w.u - w.base < static_cast<int64_t>(per) * a.kv.n_kv_heads * nrb) continue;
+                w.base = w.u;
             }
-            ++seq;
-            sq = sq_next;
-            sq_next = load(seq + 1);
+            ++w.seq;
+            w.sq = w.sq_next;
+            w.sq_next = load(w.seq + 1);
         }
+        more = w.u < w.end;
+        __syncwarp();
+        if ((threadIdx.x & 31) == 0) sh.warp[warp] = w;
+        __syncwarp();
     }
     __device__ __forceinline__ PagedTile look() {
-        open();
-        if (n == 0) return PagedTile{-2, 0, -1, 0};
+        if (n == 0) {
+            if (!more) return PagedTile{-2, 0, -1, 0};
+            open();
+            if (n == 0) return PagedTile{-2, 0, -1, 0};
+        }
         const int lane = threadIdx.x & 31, p = p0 + lane, k = static_cast<int>((static_cast<uint64_t>(p) * a.page_mul) >> a.page_shift);
         PagedTile t{-2, p - k * a.kv.page_size, p0, kh};
         if (lane < S::TP && p < length) t.page = pages[k];
@@ -353,6 +397,58 @@ struct PagedWalk {
         return t;
     }
 };
+
+// Where the 16-byte pieces of a tile's rows lie in shared memory: rows of RE bytes, a row's pieces swapped so that the
+// fragment loads of K (8 rows x one piece) and of V (every second row x 2 pieces) meet no bank twice. A warp's k-th copy
+// takes PR rows; its place is the first one's, some bits of it flipped (flip), and k times PR rows on.
+template <int RE, bool V>
+struct PagedPieces {
+    static constexpr int CH = RE / 16, PR = 32 / CH;   // pieces of a row; rows of a copy
+    static __host__ __device__ constexpr int turn(int p) {
+        return V ? (RE == 64 ? (p >> 1 & 1) << 1 : (p >> 1 & 3) << 1) : (RE == 64 ? p >> 1 & 3 : p & 7);
+    }
+    static __device__ __forceinline__ uint32_t first(int lane) { return lane / CH * RE + (lane % CH ^ turn(lane / CH)) * 16; }
+    static __host__ __device__ constexpr uint32_t flip(int k) { return turn(k * PR) << 4; }   // (the lane's own row bits are in first())
+};
+// K's fragments of 16 positions (rows of RE bytes at `rows`) and one k step (32 bytes of each): a0 .. a3
+template <int RE>
+struct KeyFragments {
+    uint32_t at;   // this lane's row and piece of k step 0
+    __device__ __forceinline__ explicit KeyFragments(const uint8_t *rows) {
+        const int lane = threadIdx.x & 31, p = (lane & 7) + (lane & 8);
+        at = smem_addr(rows) + p * RE + ((lane >> 4) ^ PagedPieces<RE, false>::turn(p)) * 16;
+    }
+    __device__ __forceinline__ uint4 operator()(int ks) const {   // (a row starts on a multiple of its size: the step's bits flip)
+        uint4 r;
+        asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                     : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(at ^ (ks << 5)) : "memory");
+        return r;
+    }
+};
+// The copies of N * PR rows (16-byte aligned to 256 bytes of shared memory at dst) of one page, or of any pages: `place`
+// the value offset of lane p's row (rows first_p ..), ok a bit for each that is there.
+template <int RE, bool V, int N, int ES>
+__device__ __forceinline__ void copy_rows(uint32_t dst, const uint8_t *src, int64_t pos_stride, int64_t place, uint32_t ok, bool one_page, int first_p) {
+    using P = PagedPieces<RE, V>;
+    const int lane = threadIdx.x & 31, rl = lane / P::CH, c = lane % P::CH;
+    const uint32_t to = dst + P::first(lane);
+    if (one_page) {
+        const int64_t step = pos_stride * ES;
+        const uint8_t *from = src + __shfl_sync(0xffffffffu, place, first_p) * ES + rl * step + c * 16;
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            copy16((to ^ P::flip(k)) + k * P::PR * RE, from, 16);
+            from += step * P::PR;
+        }
+        return;
+    }
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+        const int p = first_p + k * P::PR + rl;
+        const int64_t x = __shfl_sync(0xffffffffu, place, p);
+        copy16((to ^ P::flip(k)) + k * P::PR * RE, src + x * ES + c * 16, (ok >> p & 1) ? 16 : 0);
+    }
+}
 
 // The segment's queries as fragments (b0, b1) [k step][n tile][lane] and the rows' column factors: warp w takes rows w,
 // w + 4, ..; a lane HD / 32 neighbouring dims; up to five rows' loads in flight.
@@ -392,13 +488,13 @@ __device__ __forceinline__ void build_queries(const PagedAttnArgs &a, const Page
                     for (int x = 0; x < W; ++x) {
                         float r = v[k + x] * inv;
 #pragma unroll
-                        for (int y = 0; y < 3; ++y) {
-                            const int digit = __float2int_rn(r);
-                            w[y] |= static_cast<uint32_t>(digit & 0xff) << (8 * x);
-                            r = (r - static_cast<float>(digit)) * 254.0f;
+                        for (int y = 0; y < 3; ++y) {   // (on top of 1.5 * 2^23 the low bits are the integer)
+                            const float t = __fadd_rn(r, kBiasF);
+                            w[y] |= (__float_as_uint(t) & 0xffu) << (8 * x);
+                            r = __fmul_rn(__fsub_rn(r, __fsub_rn(t, kBiasF)), 254.0f);
                         }
                     }
-                    const int d = lane * N + k, ks = d / 64 * 2 + d % 16 / 8, t = d % 64 / 16, half = d % 8 / 4;
+                    const int d = lane * N + k, ks = d / 32, t = d % 16 / 4, half = d % 32 / 16;
                     const int f = (ks * S::NT + nt) * 32 + n * 4 + t;
                     uint32_t *const at3[3] = {reinterpret_cast<uint32_t *>(q_two + f) + half, reinterpret_cast<uint32_t *>(q_two + f) + 2 + half,
                                               reinterpret_cast<uint32_t *>(q_one + f) + half};
@@ -421,8 +517,7 @@ __device__ __forceinline__ void build_queries(const PagedAttnArgs &a, const Page
                 if (lane == 0) col[i] = scalbnf(a.x.scale * 1.44269504088896341f, ex);
 #pragma unroll
                 for (int k = 0; k < N; k += 2) {
-                    // (a 16-byte piece has 8 dims, 2 k steps; 4 lanes' pieces lie side by side)
-                    const int d = lane * N + k, ks = d / 32 * 2 + d % 8 / 4, t = d % 32 / 8, half = d % 4 / 2;
+                    const int d = lane * N + k, ks = d / 16, t = d % 8 / 2, half = d % 16 / 8;
                     const int f = (ks * S::NT + nt) * 32 + n * 4 + t;
                     const uint32_t hi = pack2<BF16>(v[k], v[k + 1]);
                     if constexpr (SPLIT) {
@@ -456,7 +551,7 @@ struct PagedShape : PagedBase<HD_, CACHE_, SPLIT_, 1> {
     static constexpr int TS = E / (2 * EPO) + 2;                  // tiles whose scales and valid bits are kept
     static constexpr int kScale = (I8 ? 2 * TP * 4 : 0) + 16;
     static constexpr int kSegs = E / (2 * EPO) + 5;               // segments looked up, not yet done
-    static constexpr int o_q = 0, o_ring = o_q + B::kQ, o_scale = o_ring + 4 * E * kEntry;
+    static constexpr int o_ring = 0, o_q = o_ring + 4 * E * kEntry, o_scale = o_q + B::kQ;
     static constexpr int o_col = o_scale + 4 * TS * kScale;       // [kRows] column factor
     static constexpr int o_seg = o_col + kRows * 4;               // [warp][kSegs]
     static constexpr int o_stat = o_seg + 4 * kSegs * 48;         // [warp][kRows] m, l, m'
@@ -477,15 +572,15 @@ template <typename S>
 __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn(PagedAttnArgs a) {
     constexpr int NT = 1, TP = S::TP, MT = S::MT, RE = S::RE, E = S::E, OM = S::OM, PARTS = S::PARTS, ME = S::ME, EPO = S::EPO;
     constexpr bool I8 = S::I8, BF16 = S::BF16, SPLIT = S::SPLIT;
-    extern __shared__ __align__(128) uint8_t sm[];
+    extern __shared__ __align__(1024) uint8_t sm[];   // (a row of the ring starts on a multiple of its size)
     __shared__ PagedWalkShared sh;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gid = lane >> 2, tig = lane & 3;
     const int G = a.x.n_heads / a.kv.n_kv_heads, cta = blockIdx.x;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;");
     if (tid == 0) a.cut[cta] = make_int4(0, 0, 0, 0);
-    PagedWalk<S> walk{a, reinterpret_cast<PagedSegment *>(sm + S::o_seg) + warp * S::kSegs};
-    if (!walk.start(sh)) return;
+    PagedWalk<S> walk{a, sh, reinterpret_cast<PagedSegment *>(sm + S::o_seg) + warp * S::kSegs};
+    if (!walk.start()) return;
 
     // the queries' fragments (b0, b1) [k step][n tile][lane]; two numbers a value (SPLIT, and int8's a, b): uint4
     uint2 *q_one = reinterpret_cast<uint2 *>(sm + S::o_q + S::kQTwo);   // (int8: c)
@@ -531,32 +626,7 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn(PagedAttnAr
             constexpr bool is_v = kind >= EPO;
             constexpr int first_p = kind % EPO / PARTS * 16 * ME, part = kind % PARTS;
             const uint8_t *src = static_cast<const uint8_t *>(is_v ? a.kv.v : a.kv.k) + part * RE;
-            constexpr int CH = RE / 16, PR = 32 / CH;   // 16-byte pieces of a row, rows of a warp's copy
-            constexpr int N = 16 * ME * CH / 32;
-            const int c = lane % CH;
-            const uint32_t dst = ring_a + in_slot * S::kEntry;
-            // pieces swapped within a row so that the fragment loads of K (8 rows x 4 neighbouring pieces) and of V (every
-            // second row x 2 pieces) meet no bank twice
-            auto put = [&](int k, const uint8_t *from, uint32_t bytes) {
-                const int p = k * PR + lane / CH;
-                int sw;
-                if (is_v) sw = RE == 64 ? c ^ ((p >> 1 & 1) << 1) : c ^ ((p >> 1 & 3) << 1);
-                else sw = RE == 64 ? c : c ^ ((p & 1) << 2);
-                copy16(dst + p * RE + sw * 16, from, bytes);
-            };
-            if (one_page) {
-                const int64_t step = a.kv.pos_stride * S::ES;
-                const uint8_t *from = src + __shfl_sync(0xffffffffu, place, first_p) * S::ES + lane / CH * step + c * 16;
-#pragma unroll
-                for (int k = 0; k < N; ++k) put(k, from, 16), from += step * PR;
-            } else {
-#pragma unroll
-                for (int k = 0; k < N; ++k) {
-                    const int p = first_p + k * PR + lane / CH;
-                    const int64_t x = __shfl_sync(0xffffffffu, place, p);
-                    put(k, src + x * S::ES + c * 16, (ok >> p & 1) ? 16 : 0);
-                }
-            }
+            copy_rows<RE, is_v, 16 * ME * (RE / 16) / 32, S::ES>(ring_a + in_slot * S::kEntry, src, a.kv.pos_stride, place, ok, one_page, first_p);
         }
         in_slot = in_slot + 1 == E ? 0 : in_slot + 1;
         asm volatile("cp.async.commit_group;" ::: "memory");
@@ -614,12 +684,10 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn(PagedAttnAr
                 // ---- S^T = K Q^T
                 float s[MT][NT][4];
                 auto k_entry = [&](auto kind_) {
-                    constexpr int kind = decltype(kind_)::value, m0 = kind / PARTS * ME, part = kind % PARTS;
+                    constexpr int kind = decltype(kind_)::value, m0 = kind / PARTS * ME;
+                    [[maybe_unused]] constexpr int part = kind % PARTS;
                     const uint8_t *ent = next_entry(kind_);
-                    auto piece = [&](int mt, int h, int j) {   // the 4 neighbouring lanes' 16 bytes of row gid + 8 h
-                        const int p = 16 * mt + 8 * h + gid, c = 4 * j + tig, sw = RE == 64 ? c : c ^ ((p & 1) << 2);
-                        return *reinterpret_cast<const uint4 *>(ent + p * RE + sw * 16);
-                    };
+                    auto keys = [&](int mt, int ks) { return KeyFragments<RE>(ent + 16 * mt * RE)(ks); };
                     if constexpr (I8) {
                         // sums on top of 1.5 * 2^23, whose float neighbours are the integers: |sum| <= 127^2 HD < 2^22
                         int32_t acc[ME][NT][3][4];
@@ -632,27 +700,20 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn(PagedAttnAr
 #pragma unroll
                                     for (int c = 0; c < 4; ++c) acc[mt][nt][y][c] = static_cast<int32_t>(kBiasBits);
 #pragma unroll
-                        for (int j = 0; j < RE / 64; ++j) {
-                            uint4 kg[ME][2];
+                        for (int ks = 0; ks < RE / 32; ++ks)
 #pragma unroll
-                            for (int mt = 0; mt < ME; ++mt) kg[mt][0] = piece(mt, 0, j), kg[mt][1] = piece(mt, 1, j);
+                            for (int nt = 0; nt < NT; ++nt) {
+                                const int f = (ks * NT + nt) * 32 + lane;
+                                const uint4 ab = q_two[f];
+                                const uint2 cc = q_one[f];
 #pragma unroll
-                            for (int w = 0; w < 2; ++w)
-#pragma unroll
-                                for (int nt = 0; nt < NT; ++nt) {
-                                    const int f = ((2 * j + w) * NT + nt) * 32 + lane;
-                                    const uint4 ab = q_two[f];
-                                    const uint2 cc = q_one[f];
-#pragma unroll
-                                    for (int mt = 0; mt < ME; ++mt) {
-                                        const uint32_t a0 = w ? kg[mt][0].z : kg[mt][0].x, a1 = w ? kg[mt][1].z : kg[mt][1].x;
-                                        const uint32_t a2 = w ? kg[mt][0].w : kg[mt][0].y, a3 = w ? kg[mt][1].w : kg[mt][1].y;
-                                        mma_s8_16832(acc[mt][nt][0], a0, a1, a2, a3, ab.x, ab.y);
-                                        mma_s8_16832(acc[mt][nt][1], a0, a1, a2, a3, ab.z, ab.w);
-                                        mma_s8_16832(acc[mt][nt][2], a0, a1, a2, a3, cc.x, cc.y);
-                                    }
+                                for (int mt = 0; mt < ME; ++mt) {
+                                    const uint4 k = keys(mt, ks);
+                                    mma_s8_16832(acc[mt][nt][0], k.x, k.y, k.z, k.w, ab.x, ab.y);
+                                    mma_s8_16832(acc[mt][nt][1], k.x, k.y, k.z, k.w, ab.z, ab.w);
+                                    mma_s8_16832(acc[mt][nt][2], k.x, k.y, k.z, k.w, cc.x, cc.y);
                                 }
-                        }
+                            }
 #pragma unroll
                         for (int mt = 0; mt < ME; ++mt)
 #pragma unroll
@@ -670,26 +731,19 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn(PagedAttnAr
 #pragma unroll
                                 for (int c = 0; c < 4; ++c) hi[mt][nt][c] = part ? s[m0 + mt][nt][c] : 0.0f, lo[mt][nt][c] = 0.0f;
 #pragma unroll
-                        for (int j = 0; j < RE / 64; ++j) {
-                            uint4 kg[ME][2];
+                        for (int ks = 0; ks < RE / 32; ++ks)
 #pragma unroll
-                            for (int mt = 0; mt < ME; ++mt) kg[mt][0] = piece(mt, 0, j), kg[mt][1] = piece(mt, 1, j);
+                            for (int nt = 0; nt < NT; ++nt) {
+                                const int f = ((part * (RE / 32) + ks) * NT + nt) * 32 + lane;
+                                const uint4 b2 = SPLIT ? q_two[f] : make_uint4(0, 0, 0, 0);
+                                const uint2 b = SPLIT ? make_uint2(b2.x, b2.y) : q_one[f];
 #pragma unroll
-                            for (int w = 0; w < 2; ++w)
-#pragma unroll
-                                for (int nt = 0; nt < NT; ++nt) {
-                                    const int f = ((2 * (part * (RE / 64) + j) + w) * NT + nt) * 32 + lane;
-                                    const uint4 b2 = SPLIT ? q_two[f] : make_uint4(0, 0, 0, 0);
-                                    const uint2 b = SPLIT ? make_uint2(b2.x, b2.y) : q_one[f];
-#pragma unroll
-                                    for (int mt = 0; mt < ME; ++mt) {
-                                        const uint32_t a0 = w ? kg[mt][0].z : kg[mt][0].x, a1 = w ? kg[mt][1].z : kg[mt][1].x;
-                                        const uint32_t a2 = w ? kg[mt][0].w : kg[mt][0].y, a3 = w ? kg[mt][1].w : kg[mt][1].y;
-                                        mma_16816<BF16>(hi[mt][nt], a0, a1, a2, a3, b.x, b.y);
-                                        if constexpr (SPLIT) mma_16816<BF16>(lo[mt][nt], a0, a1, a2, a3, b2.z, b2.w);
-                                    }
+                                for (int mt = 0; mt < ME; ++mt) {
+                                    const uint4 k = keys(mt, ks);
+                                    mma_16816<BF16>(hi[mt][nt], k.x, k.y, k.z, k.w, b.x, b.y);
+                                    if constexpr (SPLIT) mma_16816<BF16>(lo[mt][nt], k.x, k.y, k.z, k.w, b2.z, b2.w);
                                 }
-                        }
+                            }
 #pragma unroll
                         for (int mt = 0; mt < ME; ++mt)
 #pragma unroll
@@ -706,16 +760,22 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn(PagedAttnAr
                 const float *sv = reinterpret_cast<const float *>(sc + 16);
                 edge = p0 < all_lo || p0 + TP - 1 > all_hi;
                 const bool masked = edge || bits != 0xffffffffu;
-                float y[MT][NT][4];   // int8: s + log2 vs (masked on its own: an unseen scale may be anything)
+                // int8: lv = log2 vs. An unseen scale may be anything: -inf + lv is then no number, which the maxima pass over;
+                // the weight of such a score (a bit of hidden) is set to 0
+                float lv[MT][2];
+                uint32_t hidden = 0;
+                bool strange = false;
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         const int p = 16 * mt + 8 * h + gid;
-                        float ks = 1.0f, lv = 0.0f;
+                        float ks = 1.0f;
+                        lv[mt][h] = 0.0f;
                         if constexpr (I8) {
                             ks = sv[p];
-                            lv = lg2(sv[TP + p]);
+                            lv[mt][h] = lg2(sv[TP + p]);
+                            strange = strange || !(lv[mt][h] < INFINITY);
                         }
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt)
@@ -723,16 +783,16 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn(PagedAttnAr
                             for (int c = 0; c < 2; ++c) {
                                 float &v = s[mt][nt][2 * h + c];
                                 v *= col[nt][c] * ks;
-                                if constexpr (I8) y[mt][nt][2 * h + c] = v + lv;
                                 if (masked) {
                                     const int gp = p0 + p;
                                     if (gp > lim[nt][c] || !(bits >> p & 1) || (a.x.window > 0 && gp <= lim[nt][c] - a.x.window)) {
                                         v = -INFINITY;
-                                        if constexpr (I8) y[mt][nt][2 * h + c] = -INFINITY;
+                                        hidden |= 1u << ((mt * NT + nt) * 4 + 2 * h + c);
                                     }
                                 }
                             }
                     }
+                strange = I8 && masked && __any_sync(0xffffffffu, strange);
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
                     float top[2] = {-INFINITY, -INFINITY}, topo[2] = {-INFINITY, -INFINITY};
@@ -743,11 +803,11 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn(PagedAttnAr
 #pragma unroll
                             for (int c = 0; c < 2; ++c) {
                                 top[c] = fmaxf(top[c], s[mt][nt][2 * h + c]);
-                                if constexpr (I8) topo[c] = fmaxf(topo[c], y[mt][nt][2 * h + c]);
+                                if constexpr (I8) topo[c] = fmaxf(topo[c], s[mt][nt][2 * h + c] + lv[mt][h]);
                             }
-                    // (the maxima grow seldom: the reduction over the positions' lanes and the rescaling only then)
-                    const bool grows = top[0] > m[nt][0] || top[1] > m[nt][1] ||
-                                       (I8 && (topo[0] - kWeightBias > mo[nt][0] || topo[1] - kWeightBias > mo[nt][1]));
+                    // (far seldom: the reduction over the positions' lanes and the rescaling only then)
+                    const bool grows = top[0] > m[nt][0] + kSlack || top[1] > m[nt][1] + kSlack ||
+                                       (I8 && (topo[0] > mo[nt][0] + (kWeightBias + kSlack) || topo[1] > mo[nt][1] + (kWeightBias + kSlack)));
                     if (__any_sync(0xffffffffu, grows)) {
 #pragma unroll
                         for (int c = 0; c < 2; ++c) {
@@ -780,10 +840,11 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn(PagedAttnAr
                             const float oz = mo[nt][c] == -INFINITY ? 0.0f : mo[nt][c];
                             if constexpr (I8) {
                                 l[nt][c] += ex2(s[mt][nt][x] - mz);
-                                w[x] = ex2(y[mt][nt][x] - oz);
+                                w[x] = ex2(s[mt][nt][x] + lv[mt][x >> 1] - oz);
+                                if (strange && (hidden >> ((mt * NT + nt) * 4 + x) & 1)) w[x] = 0.0f;
                             } else {
                                 w[x] = ex2(s[mt][nt][x] - oz);
-                                l[nt][c] += BF16 ? w[x] : w[x] * 6.103515625e-5f;   // 2^-14
+                                l[nt][c] += BF16 ? w[x] : w[x] * 0.015625f;   // 2^-kWeightBias
                             }
                         }
 #pragma unroll

@@ -4,7 +4,7 @@
 // Here the products weigh as much as the copies, so no cache row is widened twice: of a tile's 64 positions each of the
 // four warps multiplies its 16 with all rows' queries (S^T = K Q^T), the weights go through shared memory as ready
 // fragments, and in the second product each warp has a quarter of the dims for all rows and all 64 positions. The running
-// maxima are the CTA's: a tile on which none grows (nearly all but the first) costs one vote, folded into the barrier.
+// maxima are the CTA's: a tile on which none grows far (nearly all but the first) costs one vote, folded into the barrier.
 #pragma once
 
 #include "paged_attn.cuh"
@@ -23,7 +23,7 @@ struct PagedRowsShape : PagedBase<HD_, CACHE_, SPLIT_, NT_> {
     static constexpr int kScale = (I8 ? 2 * TP * 4 : 0) + 16;
     static constexpr int DL = HD / 32, MW = HD / 64;              // dims of a lane, m tiles of a warp in the second product
     static constexpr int kP = 4 * NT * 32 * (SPLIT ? 16 : 8);     // the weights [16 positions][n tile][lane]
-    static constexpr int o_q = 0, o_ring = o_q + B::kQ, o_p = o_ring + E * kEntry, o_scale = o_p + kP;
+    static constexpr int o_ring = 0, o_q = o_ring + E * kEntry, o_p = o_q + B::kQ, o_scale = o_p + kP;
     static constexpr int o_col = o_scale + 4 * TS * kScale;       // [kRows] column factor, then the last position seen
     static constexpr int o_seg = o_col + kRows * 8;
     static constexpr int o_max = o_seg + 4 * kSegs * 48;          // [warp][kRows] a tile's maxima; at the end the sums
@@ -35,15 +35,15 @@ template <typename S>
 __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn_rows(PagedAttnArgs a) {
     constexpr int NT = S::NT, RB = S::RB, E = S::E, OM = S::OM, MW = S::MW, TP = S::TP;
     constexpr bool I8 = S::I8, BF16 = S::BF16, SPLIT = S::SPLIT;
-    extern __shared__ __align__(128) uint8_t sm[];
+    extern __shared__ __align__(1024) uint8_t sm[];   // (a row of the ring starts on a multiple of its size)
     __shared__ PagedWalkShared sh;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gid = lane >> 2, tig = lane & 3;
     const int G = a.x.n_heads / a.kv.n_kv_heads, cta = blockIdx.x;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;");
     if (tid == 0) a.cut[cta] = make_int4(0, 0, 0, 0);
-    PagedWalk<S> walk{a, reinterpret_cast<PagedSegment *>(sm + S::o_seg) + warp * S::kSegs};
-    if (!walk.start(sh)) return;
+    PagedWalk<S> walk{a, sh, reinterpret_cast<PagedSegment *>(sm + S::o_seg) + warp * S::kSegs};
+    if (!walk.start()) return;
 
     const uint2 *q_one = reinterpret_cast<const uint2 *>(sm + S::o_q + S::kQTwo);
     const uint4 *q_two = reinterpret_cast<const uint4 *>(sm + S::o_q);
@@ -86,29 +86,7 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn_rows(PagedA
         }
         if (in_any) {
             const uint8_t *src = static_cast<const uint8_t *>(is_v ? a.kv.v : a.kv.k);
-            constexpr int CH = RB / 16, PR = 32 / CH, N = TP * CH / 32;   // 16-byte pieces of a row, rows of a copy, copies
-            const int c = lane % CH;
-            const uint32_t dst = ring_a + in_slot * S::kEntry + warp * TP * RB;
-            auto put = [&](int k, const uint8_t *from, uint32_t bytes) {   // (pieces swapped within a row: no bank met twice)
-                const int p = k * PR + lane / CH;
-                int sw;
-                if (is_v) sw = RB == 64 ? c ^ ((p >> 1 & 1) << 1) : c ^ ((p >> 1 & 3) << 1);
-                else sw = RB == 64 ? c : c ^ ((p & 1) << 2);
-                copy16(dst + p * RB + sw * 16, from, bytes);
-            };
-            if (one_page) {
-                const int64_t step = a.kv.pos_stride * S::ES;
-                const uint8_t *from = src + __shfl_sync(0xffffffffu, place, 0) * S::ES + lane / CH * step + c * 16;
-#pragma unroll
-                for (int k = 0; k < N; ++k) put(k, from, 16), from += step * PR;
-            } else {
-#pragma unroll
-                for (int k = 0; k < N; ++k) {
-                    const int p = k * PR + lane / CH;
-                    const int64_t x = __shfl_sync(0xffffffffu, place, p);
-                    put(k, src + x * S::ES + c * 16, (ok >> p & 1) ? 16 : 0);
-                }
-            }
+            copy_rows<RB, is_v, TP * (RB / 16) / 32, S::ES>(ring_a + in_slot * S::kEntry + warp * TP * RB, src, a.kv.pos_stride, place, ok, one_page, 0);
         }
         in_slot = in_slot + 1 == E ? 0 : in_slot + 1;
         asm volatile("cp.async.commit_group;" ::: "memory");
@@ -152,14 +130,11 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn_rows(PagedA
         for (int i = 0; i < g.n; ++i) {
             const int tile0 = g.lo + (g.t0 + i) * S::CT, p0 = tile0 + warp * TP;
             const bool edge = tile0 < all_lo || tile0 + S::CT - 1 > all_hi;
-            // ---- S^T = K Q^T of this warp's 16 positions, three n tiles at a time
+            // ---- S^T = K Q^T of this warp's 16 positions, two n tiles at a time
             const uint8_t *ent = next_entry(std::integral_constant<int, 0>{}) + warp * TP * RB;
-            auto piece = [&](int h, int j) {
-                const int p = 8 * h + gid, c = 4 * j + tig, sw = RB == 64 ? c : c ^ ((p & 1) << 2);
-                return *reinterpret_cast<const uint4 *>(ent + p * RB + sw * 16);
-            };
+            const KeyFragments<RB> keys(ent);
             float s[NT][4];
-            constexpr int NG = 3;
+            constexpr int NG = 2;
 #pragma unroll
             for (int n0 = 0; n0 < NT; n0 += NG) {
                 if constexpr (I8) {
@@ -171,22 +146,19 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn_rows(PagedA
                         for (int y = 0; y < 3; ++y)
 #pragma unroll
                             for (int c = 0; c < 4; ++c) acc[x][y][c] = static_cast<int32_t>(kBiasBits);
+#pragma unroll 4   // (unrolled whole, the kernel outgrows the instruction cache)
+                    for (int ks = 0; ks < RB / 32; ++ks) {
+                        const uint4 k = keys(ks);
 #pragma unroll
-                    for (int j = 0; j < RB / 64; ++j) {
-                        const uint4 k0 = piece(0, j), k1 = piece(1, j);
-#pragma unroll
-                        for (int w = 0; w < 2; ++w)
-#pragma unroll
-                            for (int x = 0; x < NG; ++x) {
-                                if (n0 + x >= NT) continue;
-                                const int f = ((2 * j + w) * NT + n0 + x) * 32 + lane;
-                                const uint4 ab = q_two[f];
-                                const uint2 cc = q_one[f];
-                                const uint32_t a0 = w ? k0.z : k0.x, a1 = w ? k1.z : k1.x, a2 = w ? k0.w : k0.y, a3 = w ? k1.w : k1.y;
-                                mma_s8_16832(acc[x][0], a0, a1, a2, a3, ab.x, ab.y);
-                                mma_s8_16832(acc[x][1], a0, a1, a2, a3, ab.z, ab.w);
-                                mma_s8_16832(acc[x][2], a0, a1, a2, a3, cc.x, cc.y);
-                            }
+                        for (int x = 0; x < NG; ++x) {
+                            if (n0 + x >= NT) continue;
+                            const int f = (ks * NT + n0 + x) * 32 + lane;
+                            const uint4 ab = q_two[f];
+                            const uint2 cc = q_one[f];
+                            mma_s8_16832(acc[x][0], k.x, k.y, k.z, k.w, ab.x, ab.y);
+                            mma_s8_16832(acc[x][1], k.x, k.y, k.z, k.w, ab.z, ab.w);
+                            mma_s8_16832(acc[x][2], k.x, k.y, k.z, k.w, cc.x, cc.y);
+                        }
                     }
 #pragma unroll
                     for (int x = 0; x < NG; ++x)
@@ -201,21 +173,18 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn_rows(PagedA
                     for (int x = 0; x < NG; ++x)
 #pragma unroll
                         for (int c = 0; c < 4; ++c) hi[x][c] = lo[x][c] = 0.0f;
+#pragma unroll 4   // (unrolled whole, the kernel outgrows the instruction cache)
+                    for (int ks = 0; ks < RB / 32; ++ks) {
+                        const uint4 k = keys(ks);
 #pragma unroll
-                    for (int j = 0; j < RB / 64; ++j) {
-                        const uint4 k0 = piece(0, j), k1 = piece(1, j);
-#pragma unroll
-                        for (int w = 0; w < 2; ++w)
-#pragma unroll
-                            for (int x = 0; x < NG; ++x) {
-                                if (n0 + x >= NT) continue;
-                                const int f = ((2 * j + w) * NT + n0 + x) * 32 + lane;
-                                const uint4 b2 = SPLIT ? q_two[f] : make_uint4(0, 0, 0, 0);
-                                const uint2 b = SPLIT ? make_uint2(b2.x, b2.y) : q_one[f];
-                                const uint32_t a0 = w ? k0.z : k0.x, a1 = w ? k1.z : k1.x, a2 = w ? k0.w : k0.y, a3 = w ? k1.w : k1.y;
-                                mma_16816<BF16>(hi[x], a0, a1, a2, a3, b.x, b.y);
-                                if constexpr (SPLIT) mma_16816<BF16>(lo[x], a0, a1, a2, a3, b2.z, b2.w);
-                            }
+                        for (int x = 0; x < NG; ++x) {
+                            if (n0 + x >= NT) continue;
+                            const int f = (ks * NT + n0 + x) * 32 + lane;
+                            const uint4 b2 = SPLIT ? q_two[f] : make_uint4(0, 0, 0, 0);
+                            const uint2 b = SPLIT ? make_uint2(b2.x, b2.y) : q_one[f];
+                            mma_16816<BF16>(hi[x], k.x, k.y, k.z, k.w, b.x, b.y);
+                            if constexpr (SPLIT) mma_16816<BF16>(lo[x], k.x, k.y, k.z, k.w, b2.z, b2.w);
+                        }
                     }
 #pragma unroll
                     for (int x = 0; x < NG; ++x)
@@ -224,7 +193,7 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn_rows(PagedA
                             for (int c = 0; c < 4; ++c) s[n0 + x][c] = SPLIT ? hi[x][c] + lo[x][c] : hi[x][c];
                 }
             }
-            // ---- scores in bits, masks (a bit for each masked one: an unseen scale may be anything), does a maximum grow
+            // ---- scores in bits, masks, does a maximum grow far
             const uint8_t *sc = scales + tile_at * S::kScale;
             tile_at = tile_at + 1 == S::TS ? 0 : tile_at + 1;
             const uint32_t bits = *reinterpret_cast<const uint32_t *>(sc);
@@ -235,11 +204,12 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn_rows(PagedA
 #pragma unroll
                 for (int h = 0; h < 2; ++h) ks[h] = sv[8 * h + gid], lv[h] = lg2(sv[TP + 8 * h + gid]);
             }
+            // an unseen scale may be anything: -inf + log2 vs is then no number, which the maxima pass over; the weight of
+            // such a score (a bit of hidden) is set to 0
             uint32_t hidden = 0;
+            const bool strange = I8 && masked && __any_sync(0xffffffffu, !(lv[0] < INFINITY) || !(lv[1] < INFINITY));
             bool grows = false;
-            auto value = [&](int nt, int x) {   // s + log2 vs
-                return hidden >> (4 * nt + x) & 1 ? -INFINITY : s[nt][x] + lv[x >> 1];
-            };
+            auto value = [&](int nt, int x) { return s[nt][x] + lv[x >> 1]; };
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
                 const float2 col = *reinterpret_cast<const float2 *>(col_s + 8 * nt + 2 * tig);
@@ -257,8 +227,10 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn_rows(PagedA
                     }
                 }
 #pragma unroll
-                for (int x = 0; x < 4; ++x)
-                    grows = grows || s[nt][x] > m[nt][x & 1] || (I8 && value(nt, x) - kWeightBias > mo[nt][x & 1]);
+                for (int c = 0; c < 2; ++c) {
+                    grows = grows || fmaxf(s[nt][c], s[nt][2 + c]) > m[nt][c] + kSlack;
+                    if constexpr (I8) grows = grows || fmaxf(value(nt, c), value(nt, 2 + c)) > mo[nt][c] + (kWeightBias + kSlack);
+                }
             }
             if (__syncthreads_or(grows)) {
 #pragma unroll
@@ -308,9 +280,13 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn_rows(PagedA
                         w[x] = ex2(value(nt, x) - oz);
                     } else {
                         w[x] = ex2(s[nt][x] - oz);
-                        l[nt][c] += BF16 ? w[x] : w[x] * 6.103515625e-5f;   // 2^-14
+                        l[nt][c] += BF16 ? w[x] : w[x] * 0.015625f;   // 2^-kWeightBias
                     }
                 }
+                if (strange)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x)
+                        if (hidden >> (4 * nt + x) & 1) w[x] = 0.0f;
                 const uint32_t h0 = pack2<BF16>(w[0], w[1]), h1 = pack2<BF16>(w[2], w[3]);
                 const uint32_t b0 = move_trans(h0), b1 = move_trans(h1);
                 const int f = (warp * NT + nt) * 32 + lane;
@@ -385,7 +361,7 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn_rows(PagedA
                 }
             }
             if (!apart) {
-#pragma unroll
+#pragma unroll 1
                 for (int kt = 0; kt < 4; ++kt) {
                     uint32_t x[4][NW], va[MW][4];
                     v_words(kt, x);
