@@ -13,8 +13,8 @@
 // O^T is free): no staging of transposed or widened rows. int8 keys are multiplied
 // as they are (m16n8k32, integer sums); int8 values are widened to f16 in registers (exact).
 //
-// Arithmetic: over an int8 cache a query row is its largest value times (a + (b + c / 254) / 254) / 127 with int8 a, b, c:
-// every value to 2^-24 of the row's largest, each sum of products exact. Over a 16-bit cache queries are in the cache's
+// Arithmetic: over an int8 cache a query row is its largest value times (65536 a + 256 b + c) / (127 * 65536) with int8 a, b,
+// c: every value to 2^-24 of the row's largest, each sum of products exact. Over a 16-bit cache queries are in the cache's
 // type (f16: scaled by a power of two per row); float activations, and f16 ones over bf16, are held as a sum of two such
 // numbers. Weights are rounded once to 16 bits, an error of at most half a step relative to each, below the output's own
 // rounding; for float activations they are a sum of two (22 bits, 16 for bf16).
@@ -84,6 +84,10 @@ __device__ __forceinline__ void mma_s8_16832(int32_t (&d)[4], uint32_t a0, uint3
     asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// 65536 a + 256 b + c of sums that were made on top of kBiasBits
+__device__ __forceinline__ float digits_sum(int32_t a, int32_t b, int32_t c) {
+    return fmaf(fmaf(unbias(a), 256.0f, unbias(b)), 256.0f, unbias(c));
 }
 __device__ __forceinline__ uint32_t move_trans(uint32_t x) {   // an 8x8 matrix of 16-bit values, transposed
     uint32_t y;
@@ -235,6 +239,13 @@ __device__ __forceinline__ void write_lse(const PagedAttnArgs &a, int r0, int ro
         l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.693147180559945309f;
 }
 
+// a / b of numbers >= 0: in 32 bits where they fit (a 64-bit division takes some 400 cycles, and four of them stand between
+// a CTA's start and its first copy)
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+    if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+    return a / b;
+}
+
 // The positions [lo, hi) that a sequence's rows see between them, and its tiles a (key head, row block)
 template <typename S>
 __device__ __forceinline__ int seq_tiles(const PagedAttnArgs &a, const SeqRows &q, int &lo) {
@@ -323,7 +334,7 @@ struct PagedWalk {
         }
         const int64_t ctas = min(static_cast<int64_t>(gridDim.x), total);
         if (cta >= ctas) return false;
-        const int64_t u = total * cta / ctas;
+        const int64_t u = quotient(total * cta, ctas);
         if (before <= u && u < before + mine) {
             int64_t b = before;
             int s = s_lo;
@@ -336,7 +347,7 @@ struct PagedWalk {
             sh.base = b;
         }
         __syncthreads();
-        if (lane == 0) sh.warp[warp] = {total, ctas, u, total * (cta + 1) / ctas, sh.base, load(sh.seq), load(sh.seq + 1), sh.seq};
+        if (lane == 0) sh.warp[warp] = {total, ctas, u, quotient(total * (cta + 1), ctas), sh.base, load(sh.seq), load(sh.seq + 1), sh.seq};
         __syncwarp();
         n = opened = 0;
         more = true;
@@ -352,12 +363,12 @@ struct PagedWalk {
                 g.tps = seq_tiles<S>(a, w.sq, g.lo);
                 const int nrb = (g.rows * G + S::kRows - 1) / S::kRows, per = S::kItemCost + g.tps;
                 const int64_t off = w.u - w.base;
-                g.item = static_cast<int>(off / per);
-                const int o = static_cast<int>(off % per), m = static_cast<int>(min(static_cast<int64_t>(per - o), w.end - w.u));
+                g.item = static_cast<int>(quotient(off, per));
+                const int o = static_cast<int>(off - static_cast<int64_t>(g.item) * per), m = static_cast<int>(min(static_cast<int64_t>(per - o), w.end - w.u));
                 g.t0 = max(0, o - S::kItemCost);
                 g.n = max(0, o + m - S::kItemCost) - g.t0;
                 // (the CTA that holds the item's last tile, by the shares' own division)
-                g.parts = g.t0 == 0 && g.n < g.tps ? static_cast<int>(((w.u - o + per) * w.ctas - 1) / w.total) - static_cast<int>(blockIdx.x) + 1 : 0;
+                g.parts = g.t0 == 0 && g.n < g.tps ? static_cast<int>(quotient((w.u - o + per) * w.ctas - 1, w.total)) - static_cast<int>(blockIdx.x) + 1 : 0;
                 g.no = opened;
                 g.kh = g.item / nrb;
                 g.rb = g.item % nrb;
@@ -472,36 +483,32 @@ __device__ __forceinline__ void build_queries(const PagedAttnArgs &a, const Page
         for (int b = 0; b < B; ++b) {
             const int i = i0 + 4 * b;
             float (&v)[N] = vs[b], top = 0.0f;
-            const int nt = i >> 3, n = i & 7;
+            const int nt = i >> 3, row = i & 7;
             if constexpr (I8) {
 #pragma unroll
                 for (int k = 0; k < N; ++k) top = max_nan(top, fabsf(v[k]));
 #pragma unroll
                 for (int x = 16; x > 0; x >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, x));
-                const float inv = top > 0.0f ? 127.0f / top : 0.0f;
-                if (lane == 0) col[i] = a.x.scale * 1.44269504088896341f * (top * (1.0f / 127.0f));
+                // (the nearest integer n to 127 * 65536 v / top; the bytes of n + 0x808080, their top bits flipped, are its
+                // signed digits)
+                const float inv = top > 0.0f ? 8323072.0f / top : 0.0f;
+                if (lane == 0) col[i] = a.x.scale * 1.44269504088896341f * (top * (1.0f / 8323072.0f));
+                uint32_t n[N];
+#pragma unroll
+                for (int k = 0; k < N; ++k) n[k] = static_cast<uint32_t>(__float2int_rn(v[k] * inv)) + 0x808080u;
                 constexpr int W = N < 4 ? N : 4;   // neighbouring dims stored together
 #pragma unroll
                 for (int k = 0; k < N; k += W) {
-                    uint32_t w[3] = {0, 0, 0};
-#pragma unroll
-                    for (int x = 0; x < W; ++x) {
-                        float r = v[k + x] * inv;
-#pragma unroll
-                        for (int y = 0; y < 3; ++y) {   // (on top of 1.5 * 2^23 the low bits are the integer)
-                            const float t = __fadd_rn(r, kBiasF);
-                            w[y] |= (__float_as_uint(t) & 0xffu) << (8 * x);
-                            r = __fmul_rn(__fsub_rn(r, __fsub_rn(t, kBiasF)), 254.0f);
-                        }
-                    }
-                    const int d = lane * N + k, ks = d / 32, t = d % 16 / 4, half = d % 32 / 16;
-                    const int f = (ks * S::NT + nt) * 32 + n * 4 + t;
+                    const int d = lane * N + k, ks = d / 32, t = d % 16 / 4, half = d % 32 / 16, f = (ks * S::NT + nt) * 32 + row * 4 + t;
                     uint32_t *const at3[3] = {reinterpret_cast<uint32_t *>(q_two + f) + half, reinterpret_cast<uint32_t *>(q_two + f) + 2 + half,
                                               reinterpret_cast<uint32_t *>(q_one + f) + half};
 #pragma unroll
-                    for (int y = 0; y < 3; ++y)
-                        if constexpr (W == 4) *at3[y] = w[y];
-                        else reinterpret_cast<uint16_t *>(at3[y])[d % 4 / 2] = static_cast<uint16_t>(w[y]);
+                    for (int y = 0; y < 3; ++y) {
+                        const uint32_t byte = 2 - y, pick = byte | (byte + 4) << 4;
+                        const uint32_t lo = __byte_perm(n[k], n[k + 1], pick);
+                        if constexpr (W == 4) *at3[y] = __byte_perm(lo, __byte_perm(n[k + 2], n[k + 3], pick), 0x5410) ^ 0x80808080u;
+                        else reinterpret_cast<uint16_t *>(at3[y])[d % 4 / 2] = static_cast<uint16_t>(lo ^ 0x8080u);
+                    }
                 }
             } else {
                 int ex = 0;
@@ -518,7 +525,7 @@ __device__ __forceinline__ void build_queries(const PagedAttnArgs &a, const Page
 #pragma unroll
                 for (int k = 0; k < N; k += 2) {
                     const int d = lane * N + k, ks = d / 16, t = d % 8 / 2, half = d % 16 / 8;
-                    const int f = (ks * S::NT + nt) * 32 + n * 4 + t;
+                    const int f = (ks * S::NT + nt) * 32 + row * 4 + t;
                     const uint32_t hi = pack2<BF16>(v[k], v[k + 1]);
                     if constexpr (SPLIT) {
                         const float2 h = unpack2<BF16>(hi);
@@ -543,8 +550,9 @@ struct PagedShape : PagedBase<HD_, CACHE_, SPLIT_, 1> {
     static constexpr int MT = 2, TP = 16 * MT;                    // m tiles, positions of a warp's tile
     static constexpr int ME = RB < 256 ? 2 : 1, EM = MT / ME, EPO = EM * PARTS;
     static constexpr int CT = 4 * TP;                             // positions of a CTA's tile
-    // an item's beginning and end cost about what 64 KB of rows do
-    static constexpr int kItemCost = 65536 / (2 * CT * RB) > 0 ? 65536 / (2 * CT * RB) : 1;
+    // an item's beginning and end cost about what 128 KB of rows do (5 us; with half of it the CTAs with two items finish
+    // 2.4 us after those with one)
+    static constexpr int kItemCost = 131072 / (2 * CT * RB) > 0 ? 131072 / (2 * CT * RB) : 1;
     static constexpr int kEntry = 16 * ME * RE;
     static constexpr int kRing = 16 * 1024;                       // bytes of a warp's ring
     static constexpr int E = kRing / kEntry < 12 ? kRing / kEntry : 12;
@@ -719,9 +727,7 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn(PagedAttnAr
 #pragma unroll
                             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                                for (int c = 0; c < 4; ++c)
-                                    s[m0 + mt][nt][c] = fmaf(fmaf(unbias(acc[mt][nt][2][c]), 1.0f / 254.0f, unbias(acc[mt][nt][1][c])),
-                                                             1.0f / 254.0f, unbias(acc[mt][nt][0][c]));
+                                for (int c = 0; c < 4; ++c) s[m0 + mt][nt][c] = digits_sum(acc[mt][nt][0][c], acc[mt][nt][1][c], acc[mt][nt][2][c]);
                     } else {
                         float hi[ME][NT][4], lo[ME][NT][4];
 #pragma unroll
@@ -926,15 +932,16 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn(PagedAttnAr
                                     }
                                 }
 #pragma unroll
-                                for (int k = 0; k < MW; ++k) {
-                                    const int om = ((part * NP + np) * NW + w) * MW + k;
+                                for (int lo = 0; lo < (SPLIT ? 2 : 1); ++lo)
 #pragma unroll
-                                    for (int nt = 0; nt < NT; ++nt) {
-                                        mma_16816<BF16>(o[om][nt], va[k][0], va[k][1], va[k][2], va[k][3], ph[m0 + mt][nt][0], ph[m0 + mt][nt][1]);
-                                        if constexpr (SPLIT)
-                                            mma_16816<BF16>(o[om][nt], va[k][0], va[k][1], va[k][2], va[k][3], pl[m0 + mt][nt][0], pl[m0 + mt][nt][1]);
+                                    for (int k = 0; k < MW; ++k) {
+                                        const int om = ((part * NP + np) * NW + w) * MW + k;
+#pragma unroll
+                                        for (int nt = 0; nt < NT; ++nt) {
+                                            const uint32_t(&b)[2] = lo ? pl[m0 + mt][nt] : ph[m0 + mt][nt];
+                                            mma_16816<BF16>(o[om][nt], va[k][0], va[k][1], va[k][2], va[k][3], b[0], b[1]);
+                                        }
                                     }
-                                }
                             }
                         }
                 } else if constexpr (!I8) {
@@ -1057,10 +1064,10 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn(PagedAttnAr
 // The parts of each item that was cut, joined: CTA (c, y) has the one that main CTA c began, if there is one - its parts
 // are c's last and the first of c + 1, c + 2, .. - and a share of its values, `split` warps to a pair of m tiles of an
 // n tile: they take every split-th part, B in flight, and join their sums in shared memory.
-constexpr int kJoinThreads = 256;
+constexpr int kJoinThreads = 512;
 
 template <typename S>
-__global__ void __launch_bounds__(kJoinThreads, 2) k_paged_attn_join(PagedAttnArgs a, int split, int grid) {
+__global__ void __launch_bounds__(kJoinThreads, 1) k_paged_attn_join(PagedAttnArgs a, int split, int grid) {
     constexpr int OM = S::OM, W = kJoinThreads / 32;
     __shared__ float4 s_stat[W][2][4], s_v[W][2][32];
     __shared__ uint32_t s_cut[W];

@@ -31,7 +31,7 @@ inline PagedAttnPlan plan_paged_attn(const gcuda_paged_kv &kv, const gcuda_paged
         items = std::min(most, items * std::min(most, f));   // (capped at each step: no overflow)
     p.grid = static_cast<int>(std::min(most, items * std::min(most, per_seq + 32)));
     // (few items: many parts each)
-    p.split = items >= 64 ? 1 : items >= 16 ? 4 : 8;
+    p.split = items >= 64 ? 1 : items >= 16 ? 4 : 16;
     p.cuts = std::max(1, static_cast<int>(p.split == 1 ? p.grid - 1 : std::min<int64_t>(items, p.grid - 1)));
     auto take = [&](size_t bytes) {
         const size_t at = p.total;

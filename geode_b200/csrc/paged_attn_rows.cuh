@@ -130,68 +130,57 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn_rows(PagedA
         for (int i = 0; i < g.n; ++i) {
             const int tile0 = g.lo + (g.t0 + i) * S::CT, p0 = tile0 + warp * TP;
             const bool edge = tile0 < all_lo || tile0 + S::CT - 1 > all_hi;
-            // ---- S^T = K Q^T of this warp's 16 positions, two n tiles at a time
+            // ---- S^T = K Q^T of this warp's 16 positions
             const uint8_t *ent = next_entry(std::integral_constant<int, 0>{}) + warp * TP * RB;
             const KeyFragments<RB> keys(ent);
             float s[NT][4];
-            constexpr int NG = 2;
+            if constexpr (I8) {
+                // (sums on top of 1.5 * 2^23, whose float neighbours are the integers)
+                int32_t acc[NT][3][4];
 #pragma unroll
-            for (int n0 = 0; n0 < NT; n0 += NG) {
-                if constexpr (I8) {
-                    // (sums on top of 1.5 * 2^23, whose float neighbours are the integers)
-                    int32_t acc[NG][3][4];
+                for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                    for (int x = 0; x < NG; ++x)
+                    for (int y = 0; y < 3; ++y)
 #pragma unroll
-                        for (int y = 0; y < 3; ++y)
+                        for (int c = 0; c < 4; ++c) acc[nt][y][c] = static_cast<int32_t>(kBiasBits);
+#pragma unroll 2   // (unrolled whole, the kernel outgrows the instruction cache)
+                for (int ks = 0; ks < RB / 32; ++ks) {
+                    const uint4 k = keys(ks);
 #pragma unroll
-                            for (int c = 0; c < 4; ++c) acc[x][y][c] = static_cast<int32_t>(kBiasBits);
-#pragma unroll 4   // (unrolled whole, the kernel outgrows the instruction cache)
-                    for (int ks = 0; ks < RB / 32; ++ks) {
-                        const uint4 k = keys(ks);
-#pragma unroll
-                        for (int x = 0; x < NG; ++x) {
-                            if (n0 + x >= NT) continue;
-                            const int f = (ks * NT + n0 + x) * 32 + lane;
-                            const uint4 ab = q_two[f];
-                            const uint2 cc = q_one[f];
-                            mma_s8_16832(acc[x][0], k.x, k.y, k.z, k.w, ab.x, ab.y);
-                            mma_s8_16832(acc[x][1], k.x, k.y, k.z, k.w, ab.z, ab.w);
-                            mma_s8_16832(acc[x][2], k.x, k.y, k.z, k.w, cc.x, cc.y);
-                        }
+                    for (int nt = 0; nt < NT; ++nt) {
+                        const uint4 ab = q_two[(ks * NT + nt) * 32 + lane];
+                        const uint2 cc = q_one[(ks * NT + nt) * 32 + lane];
+                        mma_s8_16832(acc[nt][0], k.x, k.y, k.z, k.w, ab.x, ab.y);
+                        mma_s8_16832(acc[nt][1], k.x, k.y, k.z, k.w, ab.z, ab.w);
+                        mma_s8_16832(acc[nt][2], k.x, k.y, k.z, k.w, cc.x, cc.y);
                     }
-#pragma unroll
-                    for (int x = 0; x < NG; ++x)
-                        if (n0 + x < NT)
-#pragma unroll
-                            for (int c = 0; c < 4; ++c)
-                                s[n0 + x][c] = fmaf(fmaf(unbias(acc[x][2][c]), 1.0f / 254.0f, unbias(acc[x][1][c])), 1.0f / 254.0f,
-                                                    unbias(acc[x][0][c]));
-                } else {
-                    float hi[NG][4], lo[NG][4];
-#pragma unroll
-                    for (int x = 0; x < NG; ++x)
-#pragma unroll
-                        for (int c = 0; c < 4; ++c) hi[x][c] = lo[x][c] = 0.0f;
-#pragma unroll 4   // (unrolled whole, the kernel outgrows the instruction cache)
-                    for (int ks = 0; ks < RB / 32; ++ks) {
-                        const uint4 k = keys(ks);
-#pragma unroll
-                        for (int x = 0; x < NG; ++x) {
-                            if (n0 + x >= NT) continue;
-                            const int f = (ks * NT + n0 + x) * 32 + lane;
-                            const uint4 b2 = SPLIT ? q_two[f] : make_uint4(0, 0, 0, 0);
-                            const uint2 b = SPLIT ? make_uint2(b2.x, b2.y) : q_one[f];
-                            mma_16816<BF16>(hi[x], k.x, k.y, k.z, k.w, b.x, b.y);
-                            if constexpr (SPLIT) mma_16816<BF16>(lo[x], k.x, k.y, k.z, k.w, b2.z, b2.w);
-                        }
-                    }
-#pragma unroll
-                    for (int x = 0; x < NG; ++x)
-                        if (n0 + x < NT)
-#pragma unroll
-                            for (int c = 0; c < 4; ++c) s[n0 + x][c] = SPLIT ? hi[x][c] + lo[x][c] : hi[x][c];
                 }
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) s[nt][c] = digits_sum(acc[nt][0][c], acc[nt][1][c], acc[nt][2][c]);
+            } else {
+                float lo[NT][4];
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) s[nt][c] = lo[nt][c] = 0.0f;
+#pragma unroll 4
+                for (int ks = 0; ks < RB / 32; ++ks) {
+                    const uint4 k = keys(ks);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        const uint4 b2 = SPLIT ? q_two[(ks * NT + nt) * 32 + lane] : make_uint4(0, 0, 0, 0);
+                        const uint2 b = SPLIT ? make_uint2(b2.x, b2.y) : q_one[(ks * NT + nt) * 32 + lane];
+                        mma_16816<BF16>(s[nt], k.x, k.y, k.z, k.w, b.x, b.y);
+                        if constexpr (SPLIT) mma_16816<BF16>(lo[nt], k.x, k.y, k.z, k.w, b2.z, b2.w);
+                    }
+                }
+                if constexpr (SPLIT)
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) s[nt][c] += lo[nt][c];
             }
             // ---- scores in bits, masks, does a maximum grow far
             const uint8_t *sc = scales + tile_at * S::kScale;
@@ -370,10 +359,10 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn_rows(PagedA
                     for (int nt = 0; nt < NT; ++nt) {
                         const uint4 b = weights(kt, nt);
 #pragma unroll
-                        for (int k = 0; k < MW; ++k) {
-                            mma_16816<BF16>(o[k][nt], va[k][0], va[k][1], va[k][2], va[k][3], b.x, b.y);
-                            if constexpr (SPLIT) mma_16816<BF16>(o[k][nt], va[k][0], va[k][1], va[k][2], va[k][3], b.z, b.w);
-                        }
+                        for (int k = 0; k < MW; ++k) mma_16816<BF16>(o[k][nt], va[k][0], va[k][1], va[k][2], va[k][3], b.x, b.y);
+                        if constexpr (SPLIT)
+#pragma unroll
+                            for (int k = 0; k < MW; ++k) mma_16816<BF16>(o[k][nt], va[k][0], va[k][1], va[k][2], va[k][3], b.z, b.w);
                     }
                 }
             } else if constexpr (!I8) {
