@@ -36,7 +36,7 @@ __device__ __forceinline__ uint32_t bit_field(const uint32_t *w, int at, int n) 
 }
 
 template <typename T, int U>
-__global__ void __launch_bounds__(kAdjustThreads, 4) k_logits_adjust(AdjustArgs a) {
+__global__ void __launch_bounds__(kAdjustThreads, U == 2 ? 6 : 4) k_logits_adjust(AdjustArgs a) {
     using P = AdjustShape<T, U>;
     constexpr int VN = P::VN, NT = kAdjustThreads;
     extern __shared__ __align__(16) uint32_t adjust_sm[];
@@ -64,6 +64,13 @@ __global__ void __launch_bounds__(kAdjustThreads, 4) k_logits_adjust(AdjustArgs 
         }
         return q;
     };
+    constexpr uint32_t kAll = (1u << VN) - 1u;
+    auto mask_of = [&](int i) -> int {   // the row's mask (negative: none)
+        if (!r.mask || i >= rows) return -1;
+        const int64_t at = static_cast<int64_t>(s) * rows + i;
+        return r.mask_row ? r.mask_row[at] : static_cast<int>(at);
+    };
+    auto mask_words = [&](int m) { return m >= 0 && m < r.n_masks ? r.mask + m * r.mask_stride : nullptr; };
     uint4 next[U];
     auto fetch = [&](const Row &q) {
 #pragma unroll
@@ -72,6 +79,9 @@ __global__ void __launch_bounds__(kAdjustThreads, 4) k_logits_adjust(AdjustArgs 
     };
     Row row = row_at(0);
     fetch(row);
+    int mask_next = mask_of(0);   // (a row's mask is looked up a row ahead)
+    const float rep = r.repetition ? r.repetition[s] : 1.0f, fr = r.frequency ? r.frequency[s] : 0.0f,
+                pr = r.presence ? r.presence[s] : 0.0f;
 
     // the lists' first eight entries a thread, whatever their lengths (the rows are stride long): one trip to memory
     const int *hist = r.history + static_cast<int64_t>(s) * r.history_stride, *bid = r.bias_id + static_cast<int64_t>(s) * r.bias_stride;
@@ -111,8 +121,6 @@ __global__ void __launch_bounds__(kAdjustThreads, 4) k_logits_adjust(AdjustArgs 
     };
     each(hist, nh, th, [&](int t, int) { atomicAdd(&count[t], 1); });
     each(bid, nb, tb, [&](int t, int i) { atomicMax(&entry[t], i + 1); });
-    const float rep = r.repetition ? r.repetition[s] : 1.0f, fr = r.frequency ? r.frequency[s] : 0.0f,
-                pr = r.presence ? r.presence[s] : 0.0f;
     __syncthreads();
 
     auto adjusted = [&](float x, int t) {
@@ -137,26 +145,20 @@ __global__ void __launch_bounds__(kAdjustThreads, 4) k_logits_adjust(AdjustArgs 
                 atomicOr(a.status, kErrBadToken);
             }
         }
-        const uint32_t *mask = nullptr;
-        if (r.mask) {
-            const int64_t at = static_cast<int64_t>(s) * rows + i, m = r.mask_row ? r.mask_row[at] : at;
-            if (m >= r.n_masks) {
-                if (tid == 0) atomicOr(a.status, kErrBadShape);
-            } else if (m >= 0) {
-                mask = r.mask + m * r.mask_stride;
-            }
-        }
+        const uint32_t *mask = mask_words(mask_next);
+        if (r.mask && mask_next >= r.n_masks && tid == 0) atomicOr(a.status, kErrBadShape);
+        mask_next = mask_of(i + 1);
         const Row q = row;
         uint4 x[U];
         uint32_t allow[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             x[u] = next[u];
-            allow[u] = (1u << VN) - 1u;
+            allow[u] = kAll;
             const int j = tid + u * NT, t = v0 + q.head + j * VN;
             if (mask && j < q.body) {
                 const uint32_t lo = mask[t >> 5], hi = (t & 31) + VN > 32 ? mask[(t >> 5) + 1] : 0u;
-                allow[u] = __funnelshift_r(lo, hi, t & 31) & ((1u << VN) - 1u);
+                allow[u] = __funnelshift_r(lo, hi, t & 31) & kAll;
             }
         }
         if (i + 1 < rows) {
@@ -182,7 +184,7 @@ __global__ void __launch_bounds__(kAdjustThreads, 4) k_logits_adjust(AdjustArgs 
                         }
                     }
             }
-            if (allow[u] != (1u << VN) - 1u) {
+            if (allow[u] != kAll) {
 #pragma unroll
                 for (int e = 0; e < VN; ++e)
                     if (!(allow[u] >> e & 1)) {
