@@ -94,10 +94,10 @@ int gcuda_op_paged_append(const gcuda_paged_kv *kv, const gcuda_paged_batch *b, 
     const int half = x->rope_dim / 2;
     const size_t word = kv->type == GCUDA_I8 ? 8 : 4;   // the angles' and the odd halves' staging values
     const size_t smem = kAppendThreads * kAppendAhead * 8 * value_bytes(x->type) + kAppendWarps * half * 2 * word +
-                        (half % 8 ? kAppendThreads * 8 * word : 0);
+                        (half % 4 ? kAppendThreads * 8 * word : 0);
     const size_t es = value_bytes(x->type);
     auto vec = [&](const void *p, int64_t stride, int64_t head_stride) {
-        return p && !misaligned(p, 16) && stride * static_cast<int64_t>(es) % 16 == 0 && head_stride * static_cast<int64_t>(es) % 16 == 0;
+        return p && !misaligned(p, 4 * es) && stride % 4 == 0 && head_stride % 4 == 0;
     };
     AppendArgs a{*kv, *b, *x, warps, vec(x->q, x->q_stride, x->q_head_stride), vec(x->k, x->k_stride, 0),
                  vec(x->v, x->v_stride, 0), vec(x->q_out, x->q_out_stride, 0), device_status()};

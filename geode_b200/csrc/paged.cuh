@@ -45,9 +45,10 @@ __device__ __forceinline__ SeqRows seq_rows(const gcuda_paged_batch &b, int page
 }
 
 // ---------------------------------------------------------------------------------------------- append ----
-// One or more warps to a row, each on its own (no barrier): a head vector is 8 neighbouring values to a lane, so a warp's
-// turn is 1, 2 or 4 vectors of one kind (queries, keys, values), and a lane has the same dims of every head of its row, so
-// that the norm's weights and the rotary cosines and sines stay in registers. The turns' rows come through a ring in
+// One or more warps to a row, each on its own (no barrier): a head vector is 8 values to a lane, so a warp's turn is 1, 2 or
+// 4 vectors of one kind (queries, keys, values), and a lane has the same dims of every head of its row, so that the norm's
+// weights and the rotary cosines and sines stay in registers. The 8 are 4 neighbours and the 4 that these rotate with
+// (8 neighbours where nothing rotates), so a rotation needs no other lane. The turns' rows come through a ring in
 // shared memory, the first of them asked for before anything else; then the row's sequence is found (one round of loads
 // over up to 256 row_start entries), its length and page read and the angles taken. Angles are position * inv_freq in 64
 // bits (at position 10^6 a 32-bit angle is off by 0.03), reduced to a turn there. Queries and keys for a 16-bit cache go
@@ -58,7 +59,7 @@ struct AppendArgs {
     gcuda_paged_batch b;
     gcuda_append_rows x;
     int warps;                       // of a row
-    bool vec_q, vec_k, vec_v, vec_o; // 16-byte loads and stores of these rows
+    bool vec_q, vec_k, vec_v, vec_o; // loads and stores of these rows by 4 values
     uint32_t *status;
 };
 
@@ -119,22 +120,9 @@ __device__ __forceinline__ double head_factor(const double (&v)[8], double eps) 
     return rsqrt(ss * (1.0 / HD) + eps);
 }
 
-// Rotation of a lane's 8 values at `at`, trig the row's (cos, sin) [half]. A half of whole lanes: partners by shuffles;
-// else through st, a vector's HD values of shared memory.
+// Rotation where half is no multiple of 4: through st, a vector's HD values of shared memory; a lane's values lie at `at`
 template <typename T, typename T2>
-__device__ __forceinline__ void head_rotate(T (&v)[8], int at, int half, const T2 *trig, T *st) {
-    const int lane = threadIdx.x & 31;
-    if (half % 8 == 0) {
-        const bool mine = at < 2 * half, low = at < half;
-        const int other = mine ? (low ? lane + half / 8 : lane - half / 8) : lane;
-        const T2 *t = trig + (mine ? (low ? at : at - half) : 0);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const T p = __shfl_sync(0xffffffffu, v[i], other);
-            if (mine) v[i] = low ? v[i] * T(t[i].x) - p * T(t[i].y) : v[i] * T(t[i].x) + p * T(t[i].y);
-        }
-        return;
-    }
+__device__ __forceinline__ void rotate_odd(T (&v)[8], int at, int half, const T2 *trig, T *st) {
     __syncwarp();
 #pragma unroll
     for (int i = 0; i < 8; ++i) st[at + i] = v[i];
@@ -178,22 +166,25 @@ __global__ void __launch_bounds__(kAppendThreads, 3) k_paged_append(AppendArgs a
     using Trig = std::conditional_t<I8, double2, float2>;
     using Wide = std::conditional_t<I8, double, float>;
     extern __shared__ __align__(16) uint8_t append_sm[];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane / LV, at = lane % LV * 8;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane / LV, j = lane % LV;
     const int64_t work = static_cast<int64_t>(blockIdx.x) * kAppendWarps + warp;
     const int row = static_cast<int>(work / a.warps), first = static_cast<int>(work % a.warps);
     const int nh = a.x.n_heads, nkv = a.kv.n_kv_heads, half = a.x.rope_dim / 2;
     const int tq = (nh + VW - 1) / VW, tk = (nkv + VW - 1) / VW, turns = tq + 2 * tk;
     if (row >= a.b.n_rows) return;
+    // the lane's dims: at[0] .. + 3 and at[1] .. + 3, which rotate with each other on the first half / 4 lanes
+    const bool paired = half % 4 == 0, rotates = paired && j < half / 4;
+    const int at0 = !paired ? 8 * j : rotates ? 4 * j : 8 * j, at1 = rotates ? half + 4 * j : at0 + 4;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;");
 
-    constexpr int U = sizeof(TA) * 8 / 16;   // 16-byte pieces of 8 values
+    constexpr int CB = 4 * sizeof(TA);   // bytes of 4 values
     struct __align__(16) Raw {
-        uint4 w[U];
+        TA v[8];
     };
     Raw *ring = reinterpret_cast<Raw *>(append_sm) + (warp * kAppendAhead) * 32 + lane;   // [turn][lane]: a lane's own
-    const TA *src_q = static_cast<const TA *>(a.x.q) + row * a.x.q_stride + at, *src_k = static_cast<const TA *>(a.x.k) + row * a.x.k_stride + at,
-             *src_v = static_cast<const TA *>(a.x.v) + row * a.x.v_stride + at;
+    const TA *src_q = static_cast<const TA *>(a.x.q) + row * a.x.q_stride, *src_k = static_cast<const TA *>(a.x.k) + row * a.x.k_stride,
+             *src_v = static_cast<const TA *>(a.x.v) + row * a.x.v_stride;
     auto fetch = [&](int turn, int slot) {
         if (turn < turns) {
             const TA *src;
@@ -212,12 +203,16 @@ __global__ void __launch_bounds__(kAppendThreads, 3) k_paged_append(AppendArgs a
             if (!in) {
                 *dst = Raw{};
             } else if (vec) {
-#pragma unroll
-                for (int u = 0; u < U; ++u)
-                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_addr(&dst->w[u])), "l"(reinterpret_cast<const uint4 *>(src) + u) : "memory");
+                if constexpr (CB == 16) {
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_addr(dst->v)), "l"(src + at0) : "memory");
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_addr(dst->v + 4)), "l"(src + at1) : "memory");
+                } else {
+                    asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(smem_addr(dst->v)), "l"(src + at0) : "memory");
+                    asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(smem_addr(dst->v + 4)), "l"(src + at1) : "memory");
+                }
             } else {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) reinterpret_cast<TA *>(dst)[i] = src[i];
+                for (int i = 0; i < 4; ++i) dst->v[i] = src[at0 + i], dst->v[4 + i] = src[at1 + i];
             }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
@@ -257,30 +252,46 @@ __global__ void __launch_bounds__(kAppendThreads, 3) k_paged_append(AppendArgs a
         asm volatile("cp.async.wait_group 0;" ::: "memory");
         return;
     }
-    // whole halves: a lane's cosines and (signed) sines, (1, 0) where it does not rotate, and its partner
-    const bool whole = half % 8 == 0, mine = at < 2 * half, low = at < half;
-    const int other = mine ? (low ? lane + half / 8 : lane - half / 8) : lane;
-    float cs[8], sn[8], wq[8];
+    // queries: lo' = lo A - hi B, hi' = hi C + lo D with the norm's weights in the factors
+    float fa[4], fb[4], fc[4], fd[4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const bool turn = whole && mine;
-        const Trig t = turn ? trig[(low ? at : at - half) + i] : Trig{1, 0};
-        cs[i] = static_cast<float>(t.x);
-        sn[i] = static_cast<float>(turn && low ? -t.y : t.y);
-        wq[i] = a.x.q_norm ? 1.0f + a.x.q_norm[at + i] : 1.0f;
+    for (int i = 0; i < 4; ++i) {
+        const Trig t = rotates ? trig[4 * j + i] : Trig{1, 0};
+        const float c = static_cast<float>(t.x), n = static_cast<float>(t.y);
+        const float wl = a.x.q_norm ? 1.0f + a.x.q_norm[at0 + i] : 1.0f, wh = a.x.q_norm ? 1.0f + a.x.q_norm[at1 + i] : 1.0f;
+        fa[i] = wl * c, fb[i] = wh * n, fc[i] = wh * c, fd[i] = wl * n;
     }
-    auto rotate = [&](float (&v)[8]) {
-        if (half == 0) return;
-        if (whole) {
+    // keys: the norm, then the rotation, in T
+    auto key = [&](auto (&v)[8]) {
+        using T = std::remove_reference_t<decltype(v[0])>;
+        if (a.x.k_norm) {
+            const T f = head_factor<HD>(v, static_cast<T>(a.x.eps));
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = fmaf(v[i], cs[i], __shfl_sync(0xffffffffu, v[i], other) * sn[i]);
+            for (int i = 0; i < 8; ++i) v[i] = v[i] * f * (T(1) + static_cast<T>(a.x.k_norm[(i < 4 ? at0 : at1 - 4) + i]));
+        }
+        if (rotates)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const T c = static_cast<T>(trig[4 * j + i].x), n = static_cast<T>(trig[4 * j + i].y), lo = v[i], hi = v[4 + i];
+                v[i] = lo * c - hi * n;
+                v[4 + i] = hi * c + lo * n;
+            }
+        if (!paired) rotate_odd<T>(v, at0, half, trig, reinterpret_cast<T *>(st));
+    };
+    // a lane's 8 values as two groups of 4 (dst: the vector's start)
+    auto put = [&](auto *dst, const auto (&y)[8], bool vec) {
+        using Group = std::conditional_t<sizeof(y[0]) == 4, uint4, std::conditional_t<sizeof(y[0]) == 2, uint2, uint32_t>>;
+        if (vec) {
+            *reinterpret_cast<Group *>(dst + at0) = *reinterpret_cast<const Group *>(y);
+            *reinterpret_cast<Group *>(dst + at1) = *reinterpret_cast<const Group *>(y + 4);
         } else {
-            head_rotate<float>(v, at, half, trig, reinterpret_cast<float *>(st));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) dst[at0 + i] = y[i], dst[at1 + i] = y[4 + i];
         }
     };
-    const int64_t place = stored ? page * a.kv.page_stride + in_page * a.kv.pos_stride + at : 0;
+    const int64_t place = stored ? page * a.kv.page_stride + in_page * a.kv.pos_stride : 0;
     const int64_t place_s = stored ? page * a.kv.scale_page_stride + in_page * a.kv.scale_pos_stride : 0;
-    TA *out = static_cast<TA *>(a.x.q_out) + row * a.x.q_out_stride + at;
+    TA *out = static_cast<TA *>(a.x.q_out) + row * a.x.q_out_stride;
     int slot = 0;
 #pragma unroll 1
     for (int turn = first; turn < turns; turn += a.warps) {
@@ -289,32 +300,25 @@ __global__ void __launch_bounds__(kAppendThreads, 3) k_paged_append(AppendArgs a
         float v[8];
         {
             const Raw r = ring[slot * 32];
-            const TA *x = reinterpret_cast<const TA *>(&r);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = to_float(x[i]);
+            for (int i = 0; i < 8; ++i) v[i] = to_float(r.v[i]);
         }
         slot = slot + 1 == kAppendAhead ? 0 : slot + 1;
         if (turn < tq) {
             const int h = turn * VW + sub;
-            if (a.x.q_norm) {
-                const float f = head_factor<HD>(v, a.x.eps);
+            const float f = a.x.q_norm ? head_factor<HD>(v, a.x.eps) : 1.0f;
+            alignas(16) TA y[8];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] *= f * wq[i];
+            for (int i = 0; i < 4; ++i) {
+                const float lo = v[i], hi = v[4 + i];
+                v[i] = f * (rotates ? fmaf(lo, fa[i], -(hi * fb[i])) : lo * fa[i]);   // (an infinity stays one where nothing rotates)
+                v[4 + i] = f * (rotates ? fmaf(hi, fc[i], lo * fd[i]) : hi * fc[i]);
             }
-            rotate(v);
+            if (!paired) rotate_odd<float>(v, at0, half, trig, reinterpret_cast<float *>(st));
             if (h >= nh) continue;
-            Raw o;
-            TA *y = reinterpret_cast<TA *>(&o);
 #pragma unroll
             for (int i = 0; i < 8; ++i) y[i] = from_float<TA>(v[i]);
-            TA *dst = out + h * HD;
-            if (a.vec_o) {
-#pragma unroll
-                for (int u = 0; u < U; ++u) reinterpret_cast<uint4 *>(dst)[u] = o.w[u];
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) dst[i] = y[i];
-            }
+            put(out + h * HD, y, a.vec_o);
             continue;
         }
         if (!stored) continue;
@@ -325,21 +329,11 @@ __global__ void __launch_bounds__(kAppendThreads, 3) k_paged_append(AppendArgs a
                 double y[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) y[i] = v[i];
-                if (a.x.k_norm) {
-                    const double f = head_factor<HD>(y, static_cast<double>(a.x.eps));
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) y[i] = y[i] * f * (1.0 + static_cast<double>(a.x.k_norm[at + i]));
-                }
-                if (half) head_rotate<double>(y, at, half, trig, st);
+                key(y);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) v[i] = static_cast<float>(y[i]);
             } else {
-                if (a.x.k_norm) {
-                    const float f = head_factor<HD>(v, a.x.eps);
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) v[i] *= f * (1.0f + a.x.k_norm[at + i]);
-                }
-                rotate(v);
+                key(v);
             }
         }
         const int64_t to = place + h * a.kv.head_stride;
@@ -351,18 +345,19 @@ __global__ void __launch_bounds__(kAppendThreads, 3) k_paged_append(AppendArgs a
 #pragma unroll
             for (int o = LV / 2; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
             if (h >= nkv) continue;
-            *reinterpret_cast<uint2 *>(static_cast<int8_t *>(base) + to) = codes_of(v, top);
+            const uint2 codes = codes_of(v, top);
+            *reinterpret_cast<uint32_t *>(static_cast<int8_t *>(base) + to + at0) = codes.x;
+            *reinterpret_cast<uint32_t *>(static_cast<int8_t *>(base) + to + at1) = codes.y;
             if (lane % LV == 0)
                 (is_k ? a.kv.k_scale : a.kv.v_scale)[place_s + h * a.kv.scale_head_stride] =
                     static_cast<float>(static_cast<double>(top) / 127.0);
         } else {
             using TC = std::conditional_t<CACHE == GCUDA_BF16, __nv_bfloat16, __half>;
             if (h >= nkv) continue;
-            uint4 o;
-            TC *y = reinterpret_cast<TC *>(&o);
+            alignas(16) TC y[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) y[i] = from_float<TC>(v[i]);
-            *reinterpret_cast<uint4 *>(static_cast<TC *>(base) + to) = o;
+            put(static_cast<TC *>(base) + to, y, true);
         }
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
