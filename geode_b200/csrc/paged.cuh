@@ -160,7 +160,7 @@ __device__ __forceinline__ int find_sequence(const gcuda_paged_batch &b, int row
 }
 
 template <int HD, typename TA, int CACHE>
-__global__ void __launch_bounds__(kAppendThreads, 3) k_paged_append(AppendArgs a) {
+__global__ void __launch_bounds__(kAppendThreads, 4) k_paged_append(AppendArgs a) {
     constexpr int LV = HD / 8, VW = 32 / LV;   // lanes of a vector, vectors of a turn
     constexpr bool I8 = CACHE == GCUDA_I8;
     using Trig = std::conditional_t<I8, double2, float2>;

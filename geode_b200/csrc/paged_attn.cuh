@@ -15,9 +15,10 @@
 //
 // Arithmetic: over an int8 cache a query row is its largest value times (65536 a + 256 b + c) / (127 * 65536) with int8 a, b,
 // c: every value to 2^-24 of the row's largest, each sum of products exact. Over a 16-bit cache queries are in the cache's
-// type (f16: scaled by a power of two per row); float activations, and f16 ones over bf16, are held as a sum of two such
-// numbers. Weights are rounded once to 16 bits, an error of at most half a step relative to each, below the output's own
-// rounding; for float activations they are a sum of two (22 bits, 16 for bf16).
+// type (f16: scaled by a power of two per row); float activations, and f16 ones over bf16, are held as a sum of such
+// numbers: two f16 (22 bits) or three bf16 (24 bits; two would leave an error of 4e-6, three times a float product's).
+// Weights are rounded once to 16 bits, an error of at most half a step relative to each, below the output's own rounding;
+// for float activations they are such sums too.
 // int8 rows' value scales go into the weight's exponent: w = 2^(s + log2 vs - m'), with a maximum m' of its own, so that
 // rows of any scale keep their bits. Scores, sums, maxima and outputs are float.
 #pragma once
@@ -54,9 +55,10 @@ struct PagedBase {
     static constexpr int HD = HD_, CACHE = CACHE_, NT = NT_, kRows = 8 * NT;
     static constexpr bool SPLIT = SPLIT_, I8 = CACHE == GCUDA_I8, BF16 = CACHE == GCUDA_BF16;
     static constexpr int ES = I8 ? 1 : 2, RB = HD * ES, OM = HD / 16;
-    // the queries' fragments: int8 three digits a value in k steps of 32 dims, else one or two numbers in k steps of 16
-    static constexpr int kQ = I8 ? HD / 32 * NT * 32 * 24 : HD / 16 * NT * 32 * 8 * (SPLIT ? 2 : 1);
-    static constexpr int kQTwo = I8 ? HD / 32 * NT * 32 * 16 : 0;   // (int8: where the third digits start)
+    static constexpr bool THREE = SPLIT && BF16;                 // floats as three numbers
+    // the queries' fragments: int8 three digits a value in k steps of 32 dims, else one to three numbers in k steps of 16
+    static constexpr int kQ = I8 ? HD / 32 * NT * 32 * 24 : HD / 16 * NT * 32 * 8 * (THREE ? 3 : SPLIT ? 2 : 1);
+    static constexpr int kQTwo = I8 ? HD / 32 * NT * 32 * 16 : THREE ? HD / 16 * NT * 32 * 16 : 0;   // (where the third ones start)
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -468,7 +470,7 @@ __device__ __forceinline__ void build_queries(const PagedAttnArgs &a, const Page
     constexpr bool I8 = S::I8, BF16 = S::BF16, SPLIT = S::SPLIT;
     constexpr int HD = S::HD, N = HD / 32, B = S::kRows / 4 < 5 ? S::kRows / 4 : 5;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, G = a.x.n_heads / a.kv.n_kv_heads, R = g.rows * G;
-    uint2 *q_one = reinterpret_cast<uint2 *>(sm_q + S::kQTwo);   // (int8: the third digits)
+    uint2 *q_one = reinterpret_cast<uint2 *>(sm_q + S::kQTwo);   // (the third numbers, or the only ones)
     uint4 *q_two = reinterpret_cast<uint4 *>(sm_q);              // two numbers a value (SPLIT, and int8's first digits)
     for (int i0 = warp; i0 < S::kRows; i0 += 4 * B) {
         float vs[B][N];
@@ -530,7 +532,13 @@ __device__ __forceinline__ void build_queries(const PagedAttnArgs &a, const Page
                     if constexpr (SPLIT) {
                         const float2 h = unpack2<BF16>(hi);
                         reinterpret_cast<uint32_t *>(q_two + f)[half] = hi;
-                        reinterpret_cast<uint32_t *>(q_two + f)[2 + half] = pack2<BF16>(v[k] - h.x, v[k + 1] - h.y);
+                        const float x = v[k] - h.x, y = v[k + 1] - h.y;
+                        const uint32_t mid = pack2<BF16>(x, y);
+                        reinterpret_cast<uint32_t *>(q_two + f)[2 + half] = mid;
+                        if constexpr (S::THREE) {
+                            const float2 m = unpack2<BF16>(mid);
+                            reinterpret_cast<uint32_t *>(q_one + f)[half] = pack2<BF16>(x - m.x, y - m.y);
+                        }
                     } else {
                         reinterpret_cast<uint32_t *>(q_one + f)[half] = hi;
                     }
@@ -686,7 +694,8 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn(PagedAttnAr
 
         for (int i = 0; i < g.n; ++i) {
             const int p0 = g.lo + (g.t0 + i) * S::CT + warp * TP;
-            uint32_t ph[MT][NT][2], pl[MT][NT][2];   // the weights as fragments: (b0, b1), and what is left of them
+            constexpr int PN = S::THREE ? 3 : SPLIT ? 2 : 1;
+            uint32_t pw[PN][MT][NT][2];   // the weights as fragments (b0, b1), and what is left of them
             bool edge;
             {
                 // ---- S^T = K Q^T
@@ -748,6 +757,7 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn(PagedAttnAr
                                     const uint4 k = keys(mt, ks);
                                     mma_16816<BF16>(hi[mt][nt], k.x, k.y, k.z, k.w, b.x, b.y);
                                     if constexpr (SPLIT) mma_16816<BF16>(lo[mt][nt], k.x, k.y, k.z, k.w, b2.z, b2.w);
+                                    if constexpr (S::THREE) mma_16816<BF16>(lo[mt][nt], k.x, k.y, k.z, k.w, q_one[f].x, q_one[f].y);
                                 }
                             }
 #pragma unroll
@@ -855,11 +865,13 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn(PagedAttnAr
                         }
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
-                            const uint32_t hi = pack2<BF16>(w[2 * h], w[2 * h + 1]);
-                            ph[mt][nt][h] = move_trans(hi);
-                            if constexpr (SPLIT) {
-                                const float2 b = unpack2<BF16>(hi);
-                                pl[mt][nt][h] = move_trans(pack2<BF16>(w[2 * h] - b.x, w[2 * h + 1] - b.y));
+                            float x = w[2 * h], y = w[2 * h + 1];
+#pragma unroll
+                            for (int n = 0; n < PN; ++n) {
+                                const uint32_t part = pack2<BF16>(x, y);
+                                pw[n][mt][nt][h] = move_trans(part);
+                                const float2 b = unpack2<BF16>(part);
+                                x -= b.x, y -= b.y;
                             }
                         }
                     }
@@ -932,14 +944,13 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn(PagedAttnAr
                                     }
                                 }
 #pragma unroll
-                                for (int lo = 0; lo < (SPLIT ? 2 : 1); ++lo)
+                                for (int n = 0; n < PN; ++n)
 #pragma unroll
                                     for (int k = 0; k < MW; ++k) {
                                         const int om = ((part * NP + np) * NW + w) * MW + k;
 #pragma unroll
                                         for (int nt = 0; nt < NT; ++nt) {
-                                            const uint32_t(&b)[2] = lo ? pl[m0 + mt][nt] : ph[m0 + mt][nt];
-                                            mma_16816<BF16>(o[om][nt], va[k][0], va[k][1], va[k][2], va[k][3], b[0], b[1]);
+                                            mma_16816<BF16>(o[om][nt], va[k][0], va[k][1], va[k][2], va[k][3], pw[n][m0 + mt][nt][0], pw[n][m0 + mt][nt][1]);
                                         }
                                     }
                             }
@@ -972,8 +983,9 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn(PagedAttnAr
                                         float d[4];
 #pragma unroll
                                         for (int x4 = 0; x4 < 4; ++x4) d[x4] = o[(part * NP + np) * NW + w][nt][x4];
-                                        mma_16816<BF16>(d, va[0], va[1], va[2], va[3], ph[m0 + mt][nt][0], ph[m0 + mt][nt][1]);
-                                        if constexpr (SPLIT) mma_16816<BF16>(d, va[0], va[1], va[2], va[3], pl[m0 + mt][nt][0], pl[m0 + mt][nt][1]);
+#pragma unroll
+                                        for (int n = 0; n < PN; ++n)
+                                            mma_16816<BF16>(d, va[0], va[1], va[2], va[3], pw[n][m0 + mt][nt][0], pw[n][m0 + mt][nt][1]);
 #pragma unroll
                                         for (int x4 = 0; x4 < 4; ++x4)
                                             if (lim[nt][x4 & 1] - p0 == hi_p && lim[nt][x4 & 1] >= 0) o[(part * NP + np) * NW + w][nt][x4] = d[x4];

@@ -16,13 +16,14 @@ struct PagedRowsShape : PagedBase<HD_, CACHE_, SPLIT_, NT_> {
     using B = PagedBase<HD_, CACHE_, SPLIT_, NT_>;
     using B::HD, B::RB, B::I8, B::OM, B::ES, B::NT, B::SPLIT, B::kRows;
     static constexpr int TP = 16, CT = 4 * TP;                    // positions of a warp, of a CTA's tile
-    static constexpr int kItemCost = 65536 / (2 * CT * RB) > 0 ? 65536 / (2 * CT * RB) : 1;
+    static constexpr int kItemCost = 131072 / (2 * CT * RB) > 0 ? 131072 / (2 * CT * RB) : 1;
     static constexpr int kEntry = CT * RB;                        // a tile's K or V rows
     static constexpr int E = 65536 / kEntry < 3 ? 3 : 65536 / kEntry > 8 ? 8 : 65536 / kEntry;
     static constexpr int TS = E / 2 + 2, kSegs = E / 2 + 5;
     static constexpr int kScale = (I8 ? 2 * TP * 4 : 0) + 16;
     static constexpr int DL = HD / 32, MW = HD / 64;              // dims of a lane, m tiles of a warp in the second product
-    static constexpr int kP = 4 * NT * 32 * (SPLIT ? 16 : 8);     // the weights [16 positions][n tile][lane]
+    static constexpr int kP = 4 * NT * 32 * (B::THREE ? 24 : SPLIT ? 16 : 8);   // the weights [16 positions][n tile][lane]
+    static constexpr int kPTwo = B::THREE ? 4 * NT * 32 * 16 : 0;                // (where their third numbers start)
     static constexpr int o_ring = 0, o_q = o_ring + E * kEntry, o_p = o_q + B::kQ, o_scale = o_p + kP;
     static constexpr int o_col = o_scale + 4 * TS * kScale;       // [kRows] column factor, then the last position seen
     static constexpr int o_seg = o_col + kRows * 8;
@@ -174,6 +175,10 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn_rows(PagedA
                         const uint2 b = SPLIT ? make_uint2(b2.x, b2.y) : q_one[(ks * NT + nt) * 32 + lane];
                         mma_16816<BF16>(s[nt], k.x, k.y, k.z, k.w, b.x, b.y);
                         if constexpr (SPLIT) mma_16816<BF16>(lo[nt], k.x, k.y, k.z, k.w, b2.z, b2.w);
+                        if constexpr (S::THREE) {
+                            const uint2 b3 = q_one[(ks * NT + nt) * 32 + lane];
+                            mma_16816<BF16>(lo[nt], k.x, k.y, k.z, k.w, b3.x, b3.y);
+                        }
                     }
                 }
                 if constexpr (SPLIT)
@@ -276,16 +281,23 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn_rows(PagedA
 #pragma unroll
                     for (int x = 0; x < 4; ++x)
                         if (hidden >> (4 * nt + x) & 1) w[x] = 0.0f;
-                const uint32_t h0 = pack2<BF16>(w[0], w[1]), h1 = pack2<BF16>(w[2], w[3]);
-                const uint32_t b0 = move_trans(h0), b1 = move_trans(h1);
-                const int f = (warp * NT + nt) * 32 + lane;
-                if constexpr (SPLIT) {
-                    const float2 x = unpack2<BF16>(h0), y = unpack2<BF16>(h1);
-                    const uint32_t c0 = move_trans(pack2<BF16>(w[0] - x.x, w[1] - x.y)), c1 = move_trans(pack2<BF16>(w[2] - y.x, w[3] - y.y));
-                    reinterpret_cast<uint4 *>(sm + S::o_p)[f] = make_uint4(b0, b1, c0, c1);
-                } else {
-                    reinterpret_cast<uint2 *>(sm + S::o_p)[f] = make_uint2(b0, b1);
+                constexpr int PN = S::THREE ? 3 : SPLIT ? 2 : 1;
+                uint32_t part[PN][2];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    float x = w[2 * h], y = w[2 * h + 1];
+#pragma unroll
+                    for (int n = 0; n < PN; ++n) {
+                        const uint32_t b = pack2<BF16>(x, y);
+                        part[n][h] = move_trans(b);
+                        const float2 held = unpack2<BF16>(b);
+                        x -= held.x, y -= held.y;
+                    }
                 }
+                const int f = (warp * NT + nt) * 32 + lane;
+                if constexpr (SPLIT) reinterpret_cast<uint4 *>(sm + S::o_p)[f] = make_uint4(part[0][0], part[0][1], part[1][0], part[1][1]);
+                if constexpr (!SPLIT || S::THREE)
+                    reinterpret_cast<uint2 *>(sm + S::o_p + S::kPTwo)[f] = make_uint2(part[PN - 1][0], part[PN - 1][1]);
             }
             // ---- O^T += V^T P^T of this warp's dims
             const uint8_t *ev = next_entry(std::integral_constant<int, 1>{});   // (its barrier: the weights are there too)
@@ -330,6 +342,7 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn_rows(PagedA
                 const uint2 b = reinterpret_cast<const uint2 *>(sm + S::o_p)[f];
                 return make_uint4(b.x, b.y, 0, 0);
             };
+            auto third = [&](int kt, int nt) { return reinterpret_cast<const uint2 *>(sm + S::o_p + S::kPTwo)[(kt * NT + nt) * 32 + lane]; };
             // (values that a row does not see: as in k_paged_attn)
             bool apart = false;
             if constexpr (!I8) {
@@ -363,6 +376,11 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn_rows(PagedA
                         if constexpr (SPLIT)
 #pragma unroll
                             for (int k = 0; k < MW; ++k) mma_16816<BF16>(o[k][nt], va[k][0], va[k][1], va[k][2], va[k][3], b.z, b.w);
+                        if constexpr (S::THREE) {
+                            const uint2 c = third(kt, nt);
+#pragma unroll
+                            for (int k = 0; k < MW; ++k) mma_16816<BF16>(o[k][nt], va[k][0], va[k][1], va[k][2], va[k][3], c.x, c.y);
+                        }
                     }
                 }
             } else if constexpr (!I8) {
@@ -389,6 +407,10 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn_rows(PagedA
                                 float d[4] = {o[k][nt][0], o[k][nt][1], o[k][nt][2], o[k][nt][3]};
                                 mma_16816<BF16>(d, va[k][0], va[k][1], va[k][2], va[k][3], b.x, b.y);
                                 if constexpr (SPLIT) mma_16816<BF16>(d, va[k][0], va[k][1], va[k][2], va[k][3], b.z, b.w);
+                                if constexpr (S::THREE) {
+                                    const uint2 c = third(kt, nt);
+                                    mma_16816<BF16>(d, va[k][0], va[k][1], va[k][2], va[k][3], c.x, c.y);
+                                }
 #pragma unroll
                                 for (int y = 0; y < 4; ++y)
                                     if ((y & 1 ? lim.y : lim.x) == last && last >= 0) o[k][nt][y] = d[y];
