@@ -85,6 +85,7 @@ int gcuda_op_paged_append(const gcuda_paged_kv *kv, const gcuda_paged_batch *b, 
         x->rope_dim % 2 || x->rope_dim > kv->head_dim || (x->rope_dim > 0 && !x->inv_freq) || !(x->eps >= 0.0f) ||
         (x->q && x->q == x->q_out && (x->q_stride != x->q_out_stride || x->q_head_stride != kv->head_dim)))
         return GCUDA_E_ARG;
+    if (!on_current_device(kv->k, x->k)) return GCUDA_E_ARG;
     // A row's warps: one where the rows alone make three CTAs an SM, else more, up to a turn for every warp
     const int per_turn = 256 / kv->head_dim;   // vectors
     const int turns = (x->n_heads + per_turn - 1) / per_turn + 2 * ((kv->n_kv_heads + per_turn - 1) / per_turn);
@@ -123,6 +124,7 @@ int gcuda_op_paged_attn(const gcuda_paged_kv *kv, const gcuda_paged_batch *b, co
         return GCUDA_E_ARG;
     const size_t need = gcuda_op_paged_attn_work_bytes(kv, b, x->n_heads);
     if (need == 0 || work_bytes < need) return GCUDA_E_ARG;
+    if (!on_current_device(kv->k, x->out)) return GCUDA_E_ARG;
     const PagedAttnPlan p = plan_paged_attn(*kv, *b, x->n_heads);
     uint8_t *w = static_cast<uint8_t *>(d_work);
     // p / page_size by a multiplication, exact for p < 2^31: with 2^l >= page_size the multiplier is less than
@@ -142,7 +144,7 @@ int gcuda_op_paged_attn(const gcuda_paged_kv *kv, const gcuda_paged_batch *b, co
 
 int gcuda_op_logits_adjust(const gcuda_logit_rules *r, const void *d_in, void *d_out, int type, int S, int k, int V,
                            int64_t in_stride, int64_t out_stride, void *stream) {
-    if (!r || !d_in || !d_out || !activation(type) || S < 1 || S > (1 << 20) || k < 0 || k > 64 || V < 1 || in_stride < V ||
+    if (!r || !d_in || !d_out || !activation(type) || S < 1 || S > (1 << 20) || k < 0 || k > 64 || V < 1 || V > (1 << 30) || in_stride < V ||
         out_stride < V)
         return GCUDA_E_ARG;
     const int64_t rows = static_cast<int64_t>(S) * (k + 1);
@@ -156,6 +158,7 @@ int gcuda_op_logits_adjust(const gcuda_logit_rules *r, const void *d_in, void *d
     const int64_t es = static_cast<int64_t>(value_bytes(type)), ib = ((rows - 1) * in_stride + V) * es,
                   ob = ((rows - 1) * out_stride + V) * es;
     if (i0 == o0 ? in_stride != out_stride : (i0 < o0 + ob && o0 < i0 + ib)) return GCUDA_E_ARG;
+    if (!on_current_device(d_in, d_out)) return GCUDA_E_ARG;
     AdjustArgs a{*r, d_in, d_out, S, k, V, 0, in_stride, out_stride, device_status()};
     if (!a.status) return GCUDA_E_CUDA;
     cudaStream_t st = static_cast<cudaStream_t>(stream);

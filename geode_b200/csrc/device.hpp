@@ -57,6 +57,22 @@ inline int sm_count() {
     return d.sms[dev];
 }
 
+// Whether the pointers are memory of the current device (a kernel that follows one of another device faults where no
+// peer access was set up).
+template <typename... P>
+inline bool on_current_device(const P *...p) {
+    const int dev = current_device();
+    auto here = [&](const void *q) {
+        cudaPointerAttributes at{};
+        if (cudaPointerGetAttributes(&at, q) != cudaSuccess) {
+            cudaGetLastError();   // (the failure is the answer)
+            return false;
+        }
+        return (at.type == cudaMemoryTypeDevice || at.type == cudaMemoryTypeManaged) && at.device == dev;
+    };
+    return dev >= 0 && (here(p) && ...);
+}
+
 // The operators' status word on the current device (device memory, zeroed once): kernels OR error flags into it.
 // The first call on a device may come while the caller captures a stream, so the word is made outside any capture:
 // the thread's capture mode relaxed for the allocation, the zeroing on a stream of its own.
