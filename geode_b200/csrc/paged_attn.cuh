@@ -1076,13 +1076,14 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn(PagedAttnAr
 // The parts of each item that was cut, joined: CTA (c, y) has the one that main CTA c began, if there is one - its parts
 // are c's last and the first of c + 1, c + 2, .. - and a share of its values, `split` warps to a pair of m tiles of an
 // n tile: they take every split-th part, B in flight, and join their sums in shared memory.
-constexpr int kJoinThreads = 512;
+constexpr int kJoinThreads = 512;   // (split 1: 256 of them)
 
 template <typename S>
 __global__ void __launch_bounds__(kJoinThreads, 1) k_paged_attn_join(PagedAttnArgs a, int split, int grid) {
-    constexpr int OM = S::OM, W = kJoinThreads / 32;
-    __shared__ float4 s_stat[W][2][4], s_v[W][2][32];
-    __shared__ uint32_t s_cut[W];
+    constexpr int OM = S::OM;
+    __shared__ float4 s_stat[kJoinThreads / 32][2][4], s_v[kJoinThreads / 32][2][32];
+    __shared__ uint32_t s_cut[kJoinThreads / 32];
+    const int W = blockDim.x / 32;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, tig = lane & 3, gid = lane >> 2;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;");
@@ -1090,7 +1091,7 @@ __global__ void __launch_bounds__(kJoinThreads, 1) k_paged_attn_join(PagedAttnAr
     if (split > 1) {   // (few items: a CTA for each of them, not for each main CTA)
         int left = blockIdx.x;
         c = -1;
-        for (int c0 = 0; c0 < grid && c < 0; c0 += kJoinThreads) {
+        for (int c0 = 0; c0 < grid && c < 0; c0 += blockDim.x) {
             const uint32_t held = __ballot_sync(0xffffffffu, c0 + tid < grid && a.cut[c0 + tid].x != 0);
             if (lane == 0) s_cut[warp] = held;
             __syncthreads();

@@ -14,8 +14,8 @@ int launch_paged_shape(const PagedAttnArgs &a, const PagedAttnPlan &p, cudaStrea
     if (!shared_opt_in<kern>(S::kSmem)) return GCUDA_E_CUDA;
     if (launch_ex(kern, dim3(p.grid), dim3(kPagedAttnThreads), S::kSmem, st, true, a) != cudaSuccess) return GCUDA_E_CUDA;
     if (p.grid == 1) return GCUDA_OK;   // (nothing is cut)
-    const int units = S::NT * S::OM / 2, per = kJoinThreads / 32 / p.split;
-    return launch_ex(k_paged_attn_join<S>, dim3(p.cuts, (units + per - 1) / per), dim3(kJoinThreads), 0, st, true, a, p.split, p.grid) ==
+    const int units = S::NT * S::OM / 2, threads = p.split == 1 ? kJoinThreads / 2 : kJoinThreads, per = threads / 32 / p.split;
+    return launch_ex(k_paged_attn_join<S>, dim3(p.cuts, (units + per - 1) / per), dim3(threads), 0, st, true, a, p.split, p.grid) ==
                    cudaSuccess
                ? GCUDA_OK
                : GCUDA_E_CUDA;
