@@ -5,6 +5,10 @@
 // its k+1 rows, the tokens of the slice counted in shared memory (integer atomics: their order does not matter, and of
 // an id's bias entries the largest index wins). Then each row's slice is one round of 16-byte loads and stores, the next
 // row's loads in flight while one is finished, the first row's and the lists' while the counts are cleared.
+//
+// Measured: 64 x 5 rows of 248320 floats (641 MB) 129 us, 5.0 TB/s; 100 rows of 50257 bf16 (21 MB) 15 us, two waves of slices
+// that are each a chain lists -> atomics -> row; one row of 248320 floats 6.8 us, the same chain. A value at a time with 8 bytes
+// of counts read for each: 449, 25 and 13 us.
 #pragma once
 
 #include "paged.cuh"

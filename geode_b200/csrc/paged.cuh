@@ -54,6 +54,10 @@ __device__ __forceinline__ SeqRows seq_rows(const gcuda_paged_batch &b, int page
 // bits (at position 10^6 a 32-bit angle is off by 0.03), reduced to a turn there. Queries and keys for a 16-bit cache go
 // through float; keys for the int8 cache through double up to the rounding to float, so that their codes are those of the
 // definition (a float rounding moves one code in about 10^5).
+//
+// What bounds it: for few rows the chain row -> sequence -> length -> page -> angle (8 us for one row, 16 us for 1280 rows of
+// 16/2 heads of 256 to int8, 3.0 TB/s); for prompts instruction issue (9645 bf16 rows of 32/8 heads of 128: 56 us, 4.2 TB/s;
+// 6151 f16 rows to int8: 47 us, 2.6 TB/s). One CTA per row with barriers between those steps: 24, 90 and 90 us.
 struct AppendArgs {
     gcuda_paged_kv kv;
     gcuda_paged_batch b;

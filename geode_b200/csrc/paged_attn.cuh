@@ -1,17 +1,18 @@
 // paged_attn.cuh - attention of each sequence's newest rows over its pages (flash decoding over a paged cache).
 //
-// An item is one (sequence, key head, block of query rows): the sequence's T rows times the G query heads that share the
-// key head, R = T * G rows in blocks of kRows = 8 (k_paged_attn), 16 or 40 (k_paged_attn_rows, paged_attn_rows.cuh). Items are cut into tiles of positions and the tiles of all items, laid end
-// to end with a few tiles' time for each item's beginning, are dealt out evenly to the resident CTAs (each CTA finds its
-// share by a scan over the lengths on the device: whatever the lengths, every CTA has the same work). What a CTA holds
-// of an item that it does not finish goes to the scratch and k_paged_attn_join adds the parts up. The copies run ahead
-// of the products across tiles and items alike, so memory is not left idle while an item ends and the next begins.
+// An item is one (sequence, key head, block of query rows): the sequence's T rows times the G query heads that share the key
+// head, R = T * G rows in blocks of 8 (k_paged_attn), 16 or 40 (k_paged_attn_rows, paged_attn_rows.cuh). Items are cut into
+// tiles of positions and the tiles of all items, laid end to end with a few tiles' time for each item's beginning, are dealt
+// out evenly to the resident CTAs (each finds its share by a scan over the lengths on the device: whatever the lengths, every
+// CTA has the same work). What a CTA holds of an item that it does not finish goes to the scratch and k_paged_attn_join adds
+// the parts up. The copies run ahead of the products across tiles and items alike, so memory is not left idle while an item
+// ends and the next begins.
 //
-// Both products run on the tensor cores (mma.sync m16n8k16, float sums) with the cache as the 16-row operand and the
-// query rows as the 8-column one, so that one token's few rows fill the instruction: S^T = K Q^T, then O^T = V^T P^T.
-// K's fragments come by ldmatrix as they lie; V's by rows, positions interleaved by byte permutation (the order of dims in
-// O^T is free): no staging of transposed or widened rows. int8 keys are multiplied
-// as they are (m16n8k32, integer sums); int8 values are widened to f16 in registers (exact).
+// Both products run on the tensor cores (mma.sync, float sums) with the cache as the 16-row operand and the query rows as the
+// 8-column one, so that one token's few rows fill the instruction: S^T = K Q^T, then O^T = V^T P^T. K's fragments come by
+// ldmatrix as they lie; V's by rows, positions interleaved by byte permutation (the order of dims in O^T is free): no staging
+// of transposed or widened rows. int8 keys are multiplied as they are (m16n8k32, integer sums); int8 values are widened to
+// f16 in registers (exact).
 //
 // Arithmetic: over an int8 cache a query row is its largest value times (65536 a + 256 b + c) / (127 * 65536) with int8 a, b,
 // c: every value to 2^-24 of the row's largest, each sum of products exact. Over a 16-bit cache queries are in the cache's
@@ -21,6 +22,11 @@
 // for float activations they are such sums too.
 // int8 rows' value scales go into the weight's exponent: w = 2^(s + log2 vs - m'), with a maximum m' of its own, so that
 // rows of any scale keep their bits. Scores, sums, maxima and outputs are float.
+//
+// Measured, main kernel and join (8 query rows a key head): 64 ragged conversations of up to 8192 positions over an int8
+// cache of 2 heads of 256 (278 MB) 61 us, each further 278 MB 41 us (6.8 TB/s); 2 x 131072 positions of bf16 72 us (5.3
+// TB/s); 128 of up to 1000 in f16, 8 heads of 128, 66 us (items of four tiles: their beginnings and ends); one conversation
+// of 8192 positions 16 us (latency: the scan and the first copies 4.7, a tile 2.5, the join 5).
 #pragma once
 
 #include <utility>

@@ -5,6 +5,11 @@
 // four warps multiplies its 16 with all rows' queries (S^T = K Q^T), the weights go through shared memory as ready
 // fragments, and in the second product each warp has a quarter of the dims for all rows and all 64 positions. The running
 // maxima are the CTA's: a tile on which none grows far (nearly all but the first) costs one vote, folded into the barrier.
+//
+// Measured: 32 ragged verify batches of 5 rows (40 rows an item), up to 8192 positions of int8, 2 heads of 256, float
+// activations: 105 us (142 MB; 72 us for each further 142 MB). The tensor pipe is busy 41% of the time: a warp and tile has 280
+// products (at the 8.2 cycles of mma.sync the pipe's floor is 35 us) among 1900 instructions in dependent phases, two warps a
+// scheduler.
 #pragma once
 
 #include "paged_attn.cuh"
