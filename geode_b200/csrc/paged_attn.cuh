@@ -18,13 +18,14 @@
 // c: every value to 2^-24 of the row's largest, each sum of products exact. Over a 16-bit cache queries are in the cache's
 // type (f16: scaled by a power of two per row); float activations, and f16 ones over bf16, are held as a sum of such
 // numbers: two f16 (22 bits) or three bf16 (24 bits; two would leave an error of 4e-6, three times a float product's).
-// Weights are rounded once to 16 bits, an error of at most half a step relative to each, below the output's own rounding;
-// for float activations they are such sums too.
+// Weights are rounded once to f16, an error of at most 2^-11 relative to each, below the output's own rounding; for float
+// activations they are such sums too, and over a bf16 cache two numbers (one would add as much error as rounding the output
+// to bf16 does).
 // int8 rows' value scales go into the weight's exponent: w = 2^(s + log2 vs - m'), with a maximum m' of its own, so that
 // rows of any scale keep their bits. Scores, sums, maxima and outputs are float.
 //
 // Measured, main kernel and join (8 query rows a key head): 64 ragged conversations of up to 8192 positions over an int8
-// cache of 2 heads of 256 (278 MB) 61 us, each further 278 MB 41 us (6.8 TB/s); 2 x 131072 positions of bf16 72 us (5.3
+// cache of 2 heads of 256 (278 MB) 61 us, each further 278 MB 41 us (6.8 TB/s); 2 x 131072 positions of bf16 73 us (5.2
 // TB/s); 128 of up to 1000 in f16, 8 heads of 128, 66 us (items of four tiles: their beginnings and ends); one conversation
 // of 8192 positions 16 us (latency: the scan and the first copies 4.7, a tile 2.5, the join 5).
 #pragma once
@@ -62,6 +63,7 @@ struct PagedBase {
     static constexpr bool SPLIT = SPLIT_, I8 = CACHE == GCUDA_I8, BF16 = CACHE == GCUDA_BF16;
     static constexpr int ES = I8 ? 1 : 2, RB = HD * ES, OM = HD / 16;
     static constexpr bool THREE = SPLIT && BF16;                 // floats as three numbers
+    static constexpr int PN = THREE ? 3 : SPLIT || BF16 ? 2 : 1;  // numbers of a weight
     // the queries' fragments: int8 three digits a value in k steps of 32 dims, else one to three numbers in k steps of 16
     static constexpr int kQ = I8 ? HD / 32 * NT * 32 * 24 : HD / 16 * NT * 32 * 8 * (THREE ? 3 : SPLIT ? 2 : 1);
     static constexpr int kQTwo = I8 ? HD / 32 * NT * 32 * 16 : THREE ? HD / 16 * NT * 32 * 16 : 0;   // (where the third ones start)
@@ -700,7 +702,7 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn(PagedAttnAr
 
         for (int i = 0; i < g.n; ++i) {
             const int p0 = g.lo + (g.t0 + i) * S::CT + warp * TP;
-            constexpr int PN = S::THREE ? 3 : SPLIT ? 2 : 1;
+            constexpr int PN = S::PN;
             uint32_t pw[PN][MT][NT][2];   // the weights as fragments (b0, b1), and what is left of them
             bool edge;
             {

@@ -27,7 +27,7 @@ struct PagedRowsShape : PagedBase<HD_, CACHE_, SPLIT_, NT_> {
     static constexpr int TS = E / 2 + 2, kSegs = E / 2 + 5;
     static constexpr int kScale = (I8 ? 2 * TP * 4 : 0) + 16;
     static constexpr int DL = HD / 32, MW = HD / 64;              // dims of a lane, m tiles of a warp in the second product
-    static constexpr int kP = 4 * NT * 32 * (B::THREE ? 24 : SPLIT ? 16 : 8);   // the weights [16 positions][n tile][lane]
+    static constexpr int kP = 4 * NT * 32 * 8 * B::PN;              // the weights [16 positions][n tile][lane]
     static constexpr int kPTwo = B::THREE ? 4 * NT * 32 * 16 : 0;                // (where their third numbers start)
     static constexpr int o_ring = 0, o_q = o_ring + E * kEntry, o_p = o_q + B::kQ, o_scale = o_p + kP;
     static constexpr int o_col = o_scale + 4 * TS * kScale;       // [kRows] column factor, then the last position seen
@@ -41,6 +41,7 @@ template <typename S>
 __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn_rows(PagedAttnArgs a) {
     constexpr int NT = S::NT, RB = S::RB, E = S::E, OM = S::OM, MW = S::MW, TP = S::TP;
     constexpr bool I8 = S::I8, BF16 = S::BF16, SPLIT = S::SPLIT;
+    constexpr int PN = S::PN;
     extern __shared__ __align__(1024) uint8_t sm[];   // (a row of the ring starts on a multiple of its size)
     __shared__ PagedWalkShared sh;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gid = lane >> 2, tig = lane & 3;
@@ -286,7 +287,6 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn_rows(PagedA
 #pragma unroll
                     for (int x = 0; x < 4; ++x)
                         if (hidden >> (4 * nt + x) & 1) w[x] = 0.0f;
-                constexpr int PN = S::THREE ? 3 : SPLIT ? 2 : 1;
                 uint32_t part[PN][2];
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
@@ -300,8 +300,8 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn_rows(PagedA
                     }
                 }
                 const int f = (warp * NT + nt) * 32 + lane;
-                if constexpr (SPLIT) reinterpret_cast<uint4 *>(sm + S::o_p)[f] = make_uint4(part[0][0], part[0][1], part[1][0], part[1][1]);
-                if constexpr (!SPLIT || S::THREE)
+                if constexpr (PN > 1) reinterpret_cast<uint4 *>(sm + S::o_p)[f] = make_uint4(part[0][0], part[0][1], part[1][0], part[1][1]);
+                if constexpr (PN != 2)
                     reinterpret_cast<uint2 *>(sm + S::o_p + S::kPTwo)[f] = make_uint2(part[PN - 1][0], part[PN - 1][1]);
             }
             // ---- O^T += V^T P^T of this warp's dims
@@ -343,7 +343,7 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn_rows(PagedA
             };
             auto weights = [&](int kt, int nt) {
                 const int f = (kt * NT + nt) * 32 + lane;
-                if constexpr (SPLIT) return reinterpret_cast<const uint4 *>(sm + S::o_p)[f];
+                if constexpr (PN > 1) return reinterpret_cast<const uint4 *>(sm + S::o_p)[f];
                 const uint2 b = reinterpret_cast<const uint2 *>(sm + S::o_p)[f];
                 return make_uint4(b.x, b.y, 0, 0);
             };
@@ -378,7 +378,7 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn_rows(PagedA
                         const uint4 b = weights(kt, nt);
 #pragma unroll
                         for (int k = 0; k < MW; ++k) mma_16816<BF16>(o[k][nt], va[k][0], va[k][1], va[k][2], va[k][3], b.x, b.y);
-                        if constexpr (SPLIT)
+                        if constexpr (PN > 1)
 #pragma unroll
                             for (int k = 0; k < MW; ++k) mma_16816<BF16>(o[k][nt], va[k][0], va[k][1], va[k][2], va[k][3], b.z, b.w);
                         if constexpr (S::THREE) {
@@ -411,7 +411,7 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn_rows(PagedA
                             for (int k = 0; k < MW; ++k) {
                                 float d[4] = {o[k][nt][0], o[k][nt][1], o[k][nt][2], o[k][nt][3]};
                                 mma_16816<BF16>(d, va[k][0], va[k][1], va[k][2], va[k][3], b.x, b.y);
-                                if constexpr (SPLIT) mma_16816<BF16>(d, va[k][0], va[k][1], va[k][2], va[k][3], b.z, b.w);
+                                if constexpr (PN > 1) mma_16816<BF16>(d, va[k][0], va[k][1], va[k][2], va[k][3], b.z, b.w);
                                 if constexpr (S::THREE) {
                                     const uint2 c = third(kt, nt);
                                     mma_16816<BF16>(d, va[k][0], va[k][1], va[k][2], va[k][3], c.x, c.y);
