@@ -133,8 +133,9 @@ int gcuda_op_paged_attn(const gcuda_paged_kv *kv, const gcuda_paged_batch *b, co
     while ((1ll << l) < kv->page_size) ++l;
     const uint64_t d = static_cast<uint64_t>(kv->page_size);
     const uint32_t mul = static_cast<uint32_t>(((1ull << (31 + l)) + d - 1) / d);
-    const PagedAttnArgs a{*kv, *b, *x, device_status(), mul, 31 + l, reinterpret_cast<int4 *>(w + p.cut),
+    PagedAttnArgs a{*kv, *b, *x, device_status(), mul, 31 + l, reinterpret_cast<int4 *>(w + p.cut),
                           reinterpret_cast<float4 *>(w + p.stats), reinterpret_cast<float4 *>(w + p.part)};
+    if (a.x.window >= 1 << 30) a.x.window = 0;   // (no sequence is longer: all positions; the differences stay in 32 bits)
     if (!a.status) return GCUDA_E_CUDA;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (kv->type == GCUDA_I8) return launch_paged_attn_i8(a, p, st);

@@ -5,6 +5,7 @@
 // process each get their own.
 #pragma once
 
+#include <cuda.h>
 #include <cuda_runtime.h>
 
 #include <atomic>
@@ -58,17 +59,14 @@ inline int sm_count() {
 }
 
 // Whether the pointers are memory of the current device (a kernel that follows one of another device faults where no
-// peer access was set up).
+// peer access was set up). The driver's single attribute: the runtime's query of all of them takes 2.5 us a pointer.
 template <typename... P>
 inline bool on_current_device(const P *...p) {
     const int dev = current_device();
     auto here = [&](const void *q) {
-        cudaPointerAttributes at{};
-        if (cudaPointerGetAttributes(&at, q) != cudaSuccess) {
-            cudaGetLastError();   // (the failure is the answer)
-            return false;
-        }
-        return (at.type == cudaMemoryTypeDevice || at.type == cudaMemoryTypeManaged) && at.device == dev;
+        int at = -1;
+        return cuPointerGetAttribute(&at, CU_POINTER_ATTRIBUTE_DEVICE_ORDINAL, reinterpret_cast<CUdeviceptr>(q)) == CUDA_SUCCESS &&
+               at == dev;
     };
     return dev >= 0 && (here(p) && ...);
 }

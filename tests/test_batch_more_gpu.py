@@ -85,6 +85,18 @@ def test_append_every_shape(L, dim, rope, cache, act):
     assert L.gcuda_op_status(1) == 0
 
 
+@pytest.mark.parametrize("window", [2**31 - 1, 2**30, 2**30 - 1, 300, 7])
+def test_windows(L, window):
+    """Windows beyond any sequence see everything; the difference of a position and a window stays in 32 bits."""
+    plan = Plan([8, 2, 3], [200, 2, 0], 16, 2, 64, "i8", seed=9)
+    plan.randomize(10)
+    for tokens in (2, 16):   # (1 and 8 query heads a key head: both kernels)
+        x = attn_inputs(L, plan, "f32", tokens, 11, window=window)
+        assert run_attn(L, plan, x) == 0
+        torch.cuda.synchronize()
+        check_attn(plan, x, "f32", tokens)
+
+
 def test_append_many_sequences(L):
     """More sequences than one round of the search looks at, some without rows."""
     rows = [(i * 7) % 3 for i in range(1500)]
