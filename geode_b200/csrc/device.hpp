@@ -59,16 +59,28 @@ inline int sm_count() {
 }
 
 // Whether the pointers are memory of the current device (a kernel that follows one of another device faults where no
-// peer access was set up). The driver's single attribute: the runtime's query of all of them takes 2.5 us a pointer.
+// peer access was set up). The driver's single attribute: the runtime's query of all of them takes 2.5 us a pointer. The
+// driver's function comes through the runtime, so the library loads where no driver is installed.
+inline decltype(&cuPointerGetAttribute) pointer_attribute() {
+    static const auto fn = [] {
+        void *f = nullptr;
+        cudaDriverEntryPointQueryResult found = cudaDriverEntryPointSymbolNotFound;
+        if (cudaGetDriverEntryPoint("cuPointerGetAttribute", &f, cudaEnableDefault, &found) != cudaSuccess || found != cudaDriverEntryPointSuccess)
+            f = nullptr;
+        return reinterpret_cast<decltype(&cuPointerGetAttribute)>(f);
+    }();
+    return fn;
+}
 template <typename... P>
 inline bool on_current_device(const P *...p) {
     const int dev = current_device();
+    if (dev < 0 || !pointer_attribute()) return false;
     auto here = [&](const void *q) {
         int at = -1;
-        return cuPointerGetAttribute(&at, CU_POINTER_ATTRIBUTE_DEVICE_ORDINAL, reinterpret_cast<CUdeviceptr>(q)) == CUDA_SUCCESS &&
+        return pointer_attribute()(&at, CU_POINTER_ATTRIBUTE_DEVICE_ORDINAL, reinterpret_cast<CUdeviceptr>(q)) == CUDA_SUCCESS &&
                at == dev;
     };
-    return dev >= 0 && (here(p) && ...);
+    return (here(p) && ...);
 }
 
 // The operators' status word on the current device (device memory, zeroed once): kernels OR error flags into it.

@@ -1,11 +1,12 @@
 """The refusals of the operators for many conversations at once: every bad argument is an error before anything is
 launched, so they are checked without a GPU (the pointers are never followed)."""
 import ctypes as C
+import subprocess
 
 import pytest
 
 from geode_b200 import batch as gb
-from geode_b200 import cuda_lib
+from geode_b200 import CUDA_SO, cuda_lib
 
 E_ARG = -1
 P = 1 << 20   # an aligned address
@@ -47,6 +48,12 @@ BAD_ROWS = [dict(type=gb.I8), dict(type=7), dict(n_heads=-1), dict(n_heads=5000)
             dict(q_out=None), dict(n_heads=0), dict(rope_dim=31), dict(rope_dim=66), dict(rope_dim=-2), dict(inv_freq=None),
             dict(eps=-1.0), dict(eps=float("nan")), dict(q_out=P, q_out_stride=512), dict(q_out=P, q_head_stride=128)]
 BAD_ATTN = [dict(type=gb.I8), dict(n_heads=0), dict(n_heads=3), dict(n_heads=2000), dict(window=-1), dict(q=None), dict(out=None)]
+
+
+def test_library_loads_without_a_driver():
+    """The driver's library is looked up where a call needs it, never linked: a machine without a GPU has none."""
+    needed = subprocess.run(["readelf", "-d", CUDA_SO], capture_output=True, text=True, check=True).stdout
+    assert "libcudart" in needed and "libcuda.so" not in needed
 
 
 def ids(d):
