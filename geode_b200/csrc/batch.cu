@@ -19,18 +19,43 @@ namespace {
 bool activation(int type) { return type == GCUDA_F32 || type == GCUDA_BF16 || type == GCUDA_F16; }
 bool misaligned(const void *p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n != 0; }
 size_t value_bytes(int type) { return type == GCUDA_F32 ? 4 : type == GCUDA_I8 ? 1 : 2; }
+template <typename... P>
+bool words(const P *...p) { return !(misaligned(p, 4) || ...); }   // (32-bit values; NULL passes)
+
+// Whether n rows of two buffers, `width` values `stride` apart, share no value: apart as a whole, or columns of the same
+// rows (the parts of a fused q | k | v row).
+struct RowSpan {
+    const void *p;
+    int64_t stride, width;
+};
+bool apart(const RowSpan &a, const RowSpan &b, int64_t n, int64_t bytes) {
+    auto low = [&](const RowSpan &r) { return static_cast<int64_t>(reinterpret_cast<uintptr_t>(r.p)) + std::min<int64_t>(0, (n - 1) * r.stride) * bytes; };
+    auto high = [&](const RowSpan &r) { return static_cast<int64_t>(reinterpret_cast<uintptr_t>(r.p)) + (std::max<int64_t>(0, (n - 1) * r.stride) + r.width) * bytes; };
+    if (high(a) <= low(b) || high(b) <= low(a)) return true;
+    const int64_t step = (a.stride < 0 ? -a.stride : a.stride) * bytes;
+    if (a.stride != b.stride || step == 0) return false;
+    const int64_t d = ((static_cast<int64_t>(reinterpret_cast<uintptr_t>(b.p)) - static_cast<int64_t>(reinterpret_cast<uintptr_t>(a.p))) % step + step) % step;
+    return d >= a.width * bytes && d + b.width * bytes <= step;
+}
+// query rows, whose heads lie head_stride apart
+RowSpan query_rows(const void *q, int type, int64_t stride, int64_t head_stride, int n_heads, int head_dim) {
+    const int64_t over = (n_heads - 1) * head_stride;
+    return {static_cast<const uint8_t *>(q) + std::min<int64_t>(0, over) * static_cast<int64_t>(value_bytes(type)), stride, (over < 0 ? -over : over) + head_dim};
+}
 
 // The geometry alone (what the scratch's size follows from); then with the pointers
 bool good_geometry(const gcuda_paged_kv *kv, const gcuda_paged_batch *b) {
     return kv && b && (kv->type == GCUDA_I8 || kv->type == GCUDA_BF16 || kv->type == GCUDA_F16) && kv->n_pages >= 1 &&
            kv->page_size >= 1 && kv->n_kv_heads >= 1 && kv->n_kv_heads <= 1024 &&
            (kv->head_dim == 64 || kv->head_dim == 128 || kv->head_dim == 256) && b->n_seq >= 1 && b->n_rows >= 1 &&
+           b->n_seq <= (1 << 30) && b->n_rows <= (1 << 30) &&
            b->max_rows >= 1 && b->max_pages >= 1 && b->pages_stride >= 0 &&
            static_cast<int64_t>(b->max_pages) * kv->page_size <= (1ll << 30);
 }
 bool good_cache(const gcuda_paged_kv *kv, const gcuda_paged_batch *b) {
     if (!good_geometry(kv, b) || !kv->k || !kv->v || !b->row_start || !b->length || !b->pages) return false;
     if ((kv->type == GCUDA_I8) != (kv->k_scale != nullptr) || (kv->type == GCUDA_I8) != (kv->v_scale != nullptr)) return false;
+    if (!words(kv->k_scale, kv->v_scale, b->row_start, b->length, b->pages)) return false;
     const int64_t unit = 16 / static_cast<int64_t>(value_bytes(kv->type));
     return !misaligned(kv->k, 16) && !misaligned(kv->v, 16) && kv->page_stride % unit == 0 && kv->pos_stride % unit == 0 &&
            kv->head_stride % unit == 0 && kv->page_stride >= 0 && kv->pos_stride >= 0 && kv->head_stride >= 0;
@@ -85,7 +110,18 @@ int gcuda_op_paged_append(const gcuda_paged_kv *kv, const gcuda_paged_batch *b, 
         x->rope_dim % 2 || x->rope_dim > kv->head_dim || (x->rope_dim > 0 && !x->inv_freq) || !(x->eps >= 0.0f) ||
         (x->q && x->q == x->q_out && (x->q_stride != x->q_out_stride || x->q_head_stride != kv->head_dim)))
         return GCUDA_E_ARG;
-    if (!on_current_device(kv->k, x->k)) return GCUDA_E_ARG;
+    const size_t es = value_bytes(x->type);
+    if (misaligned(x->q, es) || misaligned(x->k, es) || misaligned(x->v, es) || misaligned(x->q_out, es) ||
+        !words(x->q_norm, x->k_norm, x->inv_freq))
+        return GCUDA_E_ARG;
+    if (x->q) {   // q_out is q itself or apart from all that is read
+        const int64_t kv_width = static_cast<int64_t>(kv->n_kv_heads) * kv->head_dim;
+        const RowSpan out{x->q_out, x->q_out_stride, static_cast<int64_t>(x->n_heads) * kv->head_dim};
+        if ((x->q != x->q_out && !apart(query_rows(x->q, x->type, x->q_stride, x->q_head_stride, x->n_heads, kv->head_dim), out, b->n_rows, es)) ||
+            !apart({x->k, x->k_stride, kv_width}, out, b->n_rows, es) || !apart({x->v, x->v_stride, kv_width}, out, b->n_rows, es))
+            return GCUDA_E_ARG;
+    }
+    if (const int rc = on_current_device(kv->k, x->k)) return rc;
     // A row's warps: one where the rows alone make three CTAs an SM, else more, up to a turn for every warp
     const int per_turn = 256 / kv->head_dim;   // vectors
     const int turns = (x->n_heads + per_turn - 1) / per_turn + 2 * ((kv->n_kv_heads + per_turn - 1) / per_turn);
@@ -96,7 +132,6 @@ int gcuda_op_paged_append(const gcuda_paged_kv *kv, const gcuda_paged_batch *b, 
     const size_t word = kv->type == GCUDA_I8 ? 8 : 4;   // the angles' and the odd halves' staging values
     const size_t smem = kAppendThreads * kAppendAhead * 8 * value_bytes(x->type) + kAppendWarps * half * 2 * word +
                         (half % 4 ? kAppendThreads * 8 * word : 0);
-    const size_t es = value_bytes(x->type);
     auto vec = [&](const void *p, int64_t stride, int64_t head_stride) {
         return p && !misaligned(p, 4 * es) && stride % 4 == 0 && head_stride % 4 == 0;
     };
@@ -124,7 +159,12 @@ int gcuda_op_paged_attn(const gcuda_paged_kv *kv, const gcuda_paged_batch *b, co
         return GCUDA_E_ARG;
     const size_t need = gcuda_op_paged_attn_work_bytes(kv, b, x->n_heads);
     if (need == 0 || work_bytes < need) return GCUDA_E_ARG;
-    if (!on_current_device(kv->k, x->out)) return GCUDA_E_ARG;
+    const size_t es = value_bytes(x->type);
+    if (misaligned(x->q, es) || misaligned(x->out, es) || !words(x->lse) ||
+        !apart(query_rows(x->q, x->type, x->q_stride, x->q_head_stride, x->n_heads, kv->head_dim),
+               {x->out, x->out_stride, static_cast<int64_t>(x->n_heads) * kv->head_dim}, b->n_rows, es))
+        return GCUDA_E_ARG;
+    if (const int rc = on_current_device(kv->k, x->out)) return rc;
     const PagedAttnPlan p = plan_paged_attn(*kv, *b, x->n_heads);
     uint8_t *w = static_cast<uint8_t *>(d_work);
     // p / page_size by a multiplication, exact for p < 2^31: with 2^l >= page_size the multiplier is less than
@@ -151,15 +191,18 @@ int gcuda_op_logits_adjust(const gcuda_logit_rules *r, const void *d_in, void *d
     const int64_t rows = static_cast<int64_t>(S) * (k + 1);
     if ((r->history != nullptr) != (r->history_len != nullptr) || (r->bias_id != nullptr) != (r->bias != nullptr) ||
         (r->bias_id != nullptr) != (r->bias_len != nullptr) || (r->drafts && k == 0) || r->history_stride < 0 ||
-        r->bias_stride < 0 || (r->mask_row && !r->mask) ||
+        r->bias_stride < 0 || r->history_stride > (1 << 30) || r->bias_stride > (1 << 30) || (r->mask_row && !r->mask) ||
         (r->mask && (r->n_masks < 1 || r->mask_stride < (V + 31) / 32 || (!r->mask_row && r->n_masks < rows))))
+        return GCUDA_E_ARG;
+    if (misaligned(d_in, value_bytes(type)) || misaligned(d_out, value_bytes(type)) ||
+        !words(r->history, r->history_len, r->drafts, r->repetition, r->frequency, r->presence, r->bias_id, r->bias, r->bias_len, r->mask, r->mask_row))
         return GCUDA_E_ARG;
     // in place row for row, or apart
     const char *i0 = static_cast<const char *>(d_in), *o0 = static_cast<const char *>(d_out);
     const int64_t es = static_cast<int64_t>(value_bytes(type)), ib = ((rows - 1) * in_stride + V) * es,
                   ob = ((rows - 1) * out_stride + V) * es;
     if (i0 == o0 ? in_stride != out_stride : (i0 < o0 + ob && o0 < i0 + ib)) return GCUDA_E_ARG;
-    if (!on_current_device(d_in, d_out)) return GCUDA_E_ARG;
+    if (const int rc = on_current_device(d_in, d_out)) return rc;
     AdjustArgs a{*r, d_in, d_out, S, k, V, 0, in_stride, out_stride, device_status()};
     if (!a.status) return GCUDA_E_CUDA;
     cudaStream_t st = static_cast<cudaStream_t>(stream);

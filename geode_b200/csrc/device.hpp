@@ -58,8 +58,8 @@ inline int sm_count() {
     return d.sms[dev];
 }
 
-// Whether the pointers are memory of the current device (a kernel that follows one of another device faults where no
-// peer access was set up). The driver's single attribute: the runtime's query of all of them takes 2.5 us a pointer. The
+// GCUDA_OK where the pointers are memory of the current device, else GCUDA_E_ARG (a kernel that follows one of another
+// device faults where no peer access was set up); GCUDA_E_CUDA without a device. The driver's single attribute: the runtime's query of all of them takes 2.5 us a pointer. The
 // driver's function comes through the runtime, so the library loads where no driver is installed.
 inline decltype(&cuPointerGetAttribute) pointer_attribute() {
     static const auto fn = [] {
@@ -72,15 +72,15 @@ inline decltype(&cuPointerGetAttribute) pointer_attribute() {
     return fn;
 }
 template <typename... P>
-inline bool on_current_device(const P *...p) {
+inline int on_current_device(const P *...p) {
     const int dev = current_device();
-    if (dev < 0 || !pointer_attribute()) return false;
+    if (dev < 0 || !pointer_attribute()) return GCUDA_E_CUDA;
     auto here = [&](const void *q) {
         int at = -1;
         return pointer_attribute()(&at, CU_POINTER_ATTRIBUTE_DEVICE_ORDINAL, reinterpret_cast<CUdeviceptr>(q)) == CUDA_SUCCESS &&
                at == dev;
     };
-    return (here(p) && ...);
+    return (here(p) && ...) ? GCUDA_OK : GCUDA_E_ARG;
 }
 
 // The operators' status word on the current device (device memory, zeroed once): kernels OR error flags into it.

@@ -357,8 +357,8 @@ int gcuda_op_spec_reject_static(const float *d_target, const float *d_draft, con
  * gcuda_op_greedy_verify or the rejection samplers then accept from. No counterpart in the reference, which holds one
  * conversation in one contiguous cache (its arithmetic per row: engine/src/model.cpp:3705-3797, 3815-4019, and the
  * presence penalty of engine/src/geode.cpp:234-255).
- * They run on the current device; a cache, rows or logits that are not that device's memory are refused (GCUDA_E_ARG), a
- * stream of another device fails (GCUDA_E_CUDA). None allocates, waits or needs a call before a stream capture.
+ * They run on the current device; a cache, rows or logits that are not that device's memory are refused (GCUDA_E_ARG), as
+ * is any array that is not aligned to its values; a stream of another device fails (GCUDA_E_CUDA). None allocates, waits or needs a call before a stream capture.
  *
  * Types of values: activations and 16-bit cache rows are read and written as these; GCUDA_I8 rows are int8 codes with
  * one float scale per (position, head), as the engine's cache (value = code * scale). */
@@ -382,11 +382,11 @@ typedef struct {
 
 /* The step's rows: sequence s owns rows row_start[s] .. row_start[s+1]-1 (at most max_rows) of the step's buffers of
  * n_rows rows; its cache holds length[s] positions, its rows the last of them; position p lies on page
- * pages[s * pages_stride + p / page_size], p / page_size < max_pages (max_pages * page_size at most 2^30). The three
- * arrays are device memory (int32), so a
- * captured step follows its plan from replay to replay. Rows of no sequence (behind row_start[n_seq]) are not written. What is out of range on the device raises the status word's flag 2 (gcuda_op_status): a sequence whose
- * rows or length are out of range is left out whole; a position on a page id outside [0, n_pages) is not stored and
- * not attended to. */
+ * pages[s * pages_stride + p / page_size], p / page_size < max_pages (max_pages * page_size, n_seq and n_rows at most
+ * 2^30). The three arrays are device memory (int32), so a captured step follows its plan from replay to replay. Rows of
+ * no sequence (behind row_start[n_seq]) are not written. What is out of range on the device raises the status word's
+ * flag 2 (gcuda_op_status): a sequence whose rows or length are out of range is left out whole; a position on a page id
+ * outside [0, n_pages) is not stored and not attended to. */
 typedef struct {
     int n_seq, n_rows, max_rows, max_pages;
     const int *row_start, *length, *pages;
@@ -398,7 +398,8 @@ typedef struct {
  * and key heads go through the zero-centred RMSNorm x / sqrt(mean x^2 + eps) * (1 + w) with w = q_norm / k_norm
  * [head_dim] (NULL: no norm) and the rotate-half rotary embedding over the first rope_dim values (even; 0: none), the
  * angle position * inv_freq[i] (float [rope_dim / 2]) taken in 64 bits. q_out [n_rows][n_heads][head_dim], rows
- * q_out_stride apart: the queries after both, in `type` (q_out may be q itself with the same strides; n_heads 0, q and
+ * q_out_stride apart: the queries after both, in `type` (q_out may be q itself with the same strides, or else overlaps
+ * neither q, k nor v: elsewhere, or other columns of rows with one stride; n_heads 0, q and
  * q_out NULL: keys and values only). Keys and values are rounded once to a 16-bit cache; into an int8 cache the row
  * rounded to float, its scale amax / 127 and its codes the nearest of 127 x / amax, the even one of two (an all-zero
  * row: zeros), computed in 64 bits. type: GCUDA_F32, GCUDA_BF16 or GCUDA_F16, of q, k, v and q_out alike. */
@@ -420,7 +421,7 @@ int gcuda_op_paged_append(const gcuda_paged_kv *kv, const gcuda_paged_batch *b, 
  * p = length[s] - T + i attends to the positions 0 .. p (the last `window` of them when window > 0):
  * out = sum softmax(scale * q . k) v, lse = log sum exp(scale * q . k). A row that sees no position (an empty
  * sequence, p < 0) gives zeros and lse -inf. Values at positions a row does not see do not touch it, whatever they
- * are. out must not overlap q. type: of q and out. */
+ * are. out must not overlap q (elsewhere, or other columns of rows with one stride). type: of q and out. */
 typedef struct {
     int type, n_heads, window;
     float scale;
@@ -463,7 +464,7 @@ typedef struct {
 } gcuda_logit_rules;
 /* d_out row = the rules in this order (biases, penalties, mask) on d_in row, for S sequences of k+1 rows of V logits
  * (rows s * (k+1) + i, in_stride and out_stride values apart), computed in float and rounded once to `type`
- * (GCUDA_F32, GCUDA_BF16 or GCUDA_F16); k at most 64, V at most 2^30. d_out may be d_in with the same stride; otherwise they
+ * (GCUDA_F32, GCUDA_BF16 or GCUDA_F16); k at most 64; V, history_stride and bias_stride at most 2^30. d_out may be d_in with the same stride; otherwise they
  * must not overlap. */
 int gcuda_op_logits_adjust(const gcuda_logit_rules *r, const void *d_in, void *d_out, int type, int S, int k, int V,
                            int64_t in_stride, int64_t out_stride, void *stream);

@@ -4,6 +4,7 @@ import ctypes as C
 import subprocess
 
 import pytest
+import torch
 
 from geode_b200 import batch as gb
 from geode_b200 import CUDA_SO, cuda_lib
@@ -30,7 +31,7 @@ def rows(**kw):
 
 
 def attn(**kw):
-    d = dict(type=gb.F32, n_heads=4, window=0, scale=0.1, q=P, out=P, lse=None, q_stride=256, q_head_stride=64, out_stride=256)
+    d = dict(type=gb.F32, n_heads=4, window=0, scale=0.1, q=P, out=1 << 40, lse=None, q_stride=256, q_head_stride=64, out_stride=256)
     return gb.AttnRows(**{**d, **kw})
 
 
@@ -41,13 +42,18 @@ def by(x):
 BAD_CACHE = [dict(k=None), dict(v=None), dict(k_scale=None), dict(v_scale=None), dict(type=gb.F32), dict(type=9),
              dict(type=gb.F16), dict(n_pages=0), dict(page_size=0), dict(n_kv_heads=0), dict(n_kv_heads=2000),
              dict(head_dim=96), dict(head_dim=512), dict(k=P + 8), dict(v=P + 1), dict(page_stride=16 * 128 + 8),
-             dict(pos_stride=120), dict(head_stride=8), dict(pos_stride=-128)]
+             dict(pos_stride=120), dict(head_stride=8), dict(pos_stride=-128),
+             dict(k_scale=P + 2), dict(v_scale=P + 1)]
 BAD_BATCH = [dict(n_seq=0), dict(n_rows=0), dict(max_rows=0), dict(max_pages=0), dict(row_start=None), dict(length=None),
-             dict(pages=None), dict(pages_stride=-1)]
+             dict(pages=None), dict(pages_stride=-1), dict(n_seq=(1 << 30) + 1), dict(n_rows=(1 << 30) + 1),
+             dict(row_start=P + 2), dict(length=P + 1), dict(pages=P + 3)]
 BAD_ROWS = [dict(type=gb.I8), dict(type=7), dict(n_heads=-1), dict(n_heads=5000), dict(k=None), dict(v=None), dict(q=None),
             dict(q_out=None), dict(n_heads=0), dict(rope_dim=31), dict(rope_dim=66), dict(rope_dim=-2), dict(inv_freq=None),
-            dict(eps=-1.0), dict(eps=float("nan")), dict(q_out=P, q_out_stride=512), dict(q_out=P, q_head_stride=128)]
-BAD_ATTN = [dict(type=gb.I8), dict(n_heads=0), dict(n_heads=3), dict(n_heads=2000), dict(window=-1), dict(q=None), dict(out=None)]
+            dict(eps=-1.0), dict(eps=float("nan")), dict(q_out=P, q_out_stride=512), dict(q_out=P, q_head_stride=128),
+            dict(q=P + 2), dict(k=P + 1), dict(v=P + 3), dict(q_out=2 * P + 2), dict(q_norm=P + 2), dict(k_norm=P + 1),
+            dict(inv_freq=P + 2), dict(q_out=P + 4), dict(q_out=P - 4), dict(k=2 * P + 1020), dict(v=2 * P - 508)]
+BAD_ATTN = [dict(type=gb.I8), dict(n_heads=0), dict(n_heads=3), dict(n_heads=2000), dict(window=-1), dict(q=None), dict(out=None),
+            dict(q=P + 1), dict(out=P + 2 + (1 << 30)), dict(lse=P + 2), dict(out=P), dict(out=P + 1020), dict(out=P - 1020)]
 
 
 def test_library_loads_without_a_driver():
@@ -84,6 +90,25 @@ def test_attn_refused(bad):
     assert cuda_lib().gcuda_op_paged_attn(by(cache()), by(batch()), by(attn(**bad)), P, 1 << 40, None) == E_ARG
 
 
+@pytest.mark.skipif(torch.cuda.is_available(), reason="the addresses are followed where there is a device")
+def test_good_calls_pass_the_checks():
+    """What the refusals start from, and rows side by side in one buffer (q | k | v, with and without other rows
+    between): not refused, but without a device they go no further."""
+    L = cuda_lib()
+    E_CUDA = L.gcuda_op_logits_adjust(C.byref(gb.LogitRules()), P, 1 << 40, gb.F32, 1, 0, 8, 8, 8, None)
+    assert E_CUDA not in (0, E_ARG)
+    many = batch(n_rows=5, max_rows=5)
+    for r in (rows(), rows(q_out=P, k=P + 1024, v=P + 1536, q_stride=512, k_stride=512, v_stride=512, q_out_stride=512),
+              rows(q_out=P + 4 * 1024, k=P + 1024, v=P + 1536, q_stride=2048, k_stride=2048, v_stride=2048, q_out_stride=2048),
+              rows(n_heads=0, q=None, q_out=None), rows(q_stride=0)):
+        assert L.gcuda_op_paged_append(by(cache()), by(many), by(r), None) == E_CUDA
+    for a in (attn(), attn(out=P + 1024, q_stride=512, out_stride=512), attn(out=P - 1024, q_stride=512, out_stride=512), attn(q_stride=0)):
+        assert L.gcuda_op_paged_attn(by(cache()), by(many), by(a), P, 1 << 40, None) == E_CUDA
+    for a in (attn(out=P + 1024, q_stride=512, out_stride=520), attn(out=P + 1020, q_stride=512, out_stride=512),
+              attn(out=P + 1028, q_stride=512, out_stride=512)):
+        assert L.gcuda_op_paged_attn(by(cache()), by(many), by(a), P, 1 << 40, None) == E_ARG
+
+
 def test_attn_scratch_and_rows_refused():
     L = cuda_lib()
     need = L.gcuda_op_paged_attn_work_bytes(by(cache()), by(batch()), 4)
@@ -118,7 +143,11 @@ def test_adjust_refused():
                                    dict(n_masks=0), dict(mask_stride=3), dict(mask_row=None, n_masks=5))]
     bad += [dict(d_in=None), dict(d_out=None), dict(type=gb.I8), dict(type=-1), dict(S=0), dict(k=-1), dict(k=65), dict(V=0),
             dict(si=99), dict(so=99), dict(S=1 << 21), dict(k=0), dict(d_out=P, so=104), dict(d_out=P + 400),
-            dict(d_out=P - 400)]
+            dict(d_out=P - 400), dict(d_in=P + 2), dict(d_out=far + 1)]
+    bad += [dict(rules={n: P + 2}) for n in ("history", "history_len", "drafts", "repetition", "frequency", "presence", "bias_id",
+                                            "bias", "bias_len", "mask", "mask_row")]
+    bad += [dict(rules={n: (1 << 30) + 1}) for n in ("history_stride", "bias_stride")]
+    assert torch.cuda.is_available() or call() not in (0, E_ARG)
     for b in bad:
         assert call(**b) == E_ARG, b
     assert L.gcuda_op_logits_adjust(None, P, far, gb.F32, 1, 0, 8, 8, 8, None) == E_ARG
