@@ -81,8 +81,14 @@ __device__ __forceinline__ float max_nan(float a, float b) {   // (a NaN among t
 
 // The nearest integers to 127 y / top, the even one of two, as bytes: by a float product where that is sure (it is within
 // 10^-4 of the quotient; added to 1.5 * 2^23 its low bits are the integer), next to a half by comparing 2 * 127 |y| with
-// (2 k + 1) top, both exact in double
-__device__ __forceinline__ uint2 codes_of(const float (&y)[8], float top) {
+// (2 k + 1) top, both exact in double. Rows of values so small that 127 / top has no float (below 2^-121) are scaled by a
+// power of two first, which is exact: y is theirs afterwards.
+__device__ __forceinline__ uint2 codes_of(float (&y)[8], float top) {
+    if (top < 0x1p-100f) {
+        top *= 0x1p100f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] *= 0x1p100f;
+    }
     const float inv = top > 0.0f ? 127.0f / top : 0.0f;
     uint32_t w[2] = {0, 0}, near = 0;
 #pragma unroll
