@@ -16,8 +16,8 @@
 //
 // Arithmetic: over an int8 cache a query row is its largest value times (65536 a + 256 b + c) / (127 * 65536) with int8 a, b,
 // c: every value to 2^-24 of the row's largest, each sum of products exact. Over a 16-bit cache queries are in the cache's
-// type (f16: scaled by a power of two per row); float activations, and f16 ones over bf16, are held as a sum of such
-// numbers: two f16 (22 bits) or three bf16 (24 bits; two would leave an error of 4e-6, three times a float product's).
+// type (f16, and floats in any: scaled by a power of two per row); float activations, and f16 ones over bf16, are held as a sum
+// of such numbers: two f16 (22 bits) or three bf16 (24 bits; two would leave an error of 4e-6, three times a float product's).
 // Weights are rounded once to f16, an error of at most 2^-11 relative to each, below the output's own rounding; for float
 // activations they are such sums too, and over a bf16 cache two numbers (one would add as much error as rounding the output
 // to bf16 does).
@@ -500,9 +500,16 @@ __device__ __forceinline__ void build_queries(const PagedAttnArgs &a, const Page
 #pragma unroll
                 for (int x = 16; x > 0; x >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, x));
                 // (the nearest integer n to 127 * 65536 v / top; the bytes of n + 0x808080, their top bits flipped, are its
-                // signed digits)
+                // signed digits. Rows so small that the quotient or the factor has no normal float: times a power of two)
+                float down = 1.0f;
+                if (top < 0x1p-60f) {
+                    top *= 0x1p60f;
+                    down = 0x1p-60f;
+#pragma unroll
+                    for (int k = 0; k < N; ++k) v[k] *= 0x1p60f;
+                }
                 const float inv = top > 0.0f ? 8323072.0f / top : 0.0f;
-                if (lane == 0) col[i] = a.x.scale * 1.44269504088896341f * (top * (1.0f / 8323072.0f));
+                if (lane == 0) col[i] = a.x.scale * 1.44269504088896341f * down * (top * (1.0f / 8323072.0f));
                 uint32_t n[N];
 #pragma unroll
                 for (int k = 0; k < N; ++k) n[k] = static_cast<uint32_t>(__float2int_rn(v[k] * inv)) + 0x808080u;
@@ -522,7 +529,7 @@ __device__ __forceinline__ void build_queries(const PagedAttnArgs &a, const Page
                 }
             } else {
                 int ex = 0;
-                if constexpr (!BF16) {
+                if constexpr (!BF16 || SPLIT) {   // (bf16 queries over bf16 keep their bits as they are)
 #pragma unroll
                     for (int k = 0; k < N; ++k) top = fmaxf(top, fabsf(v[k]));
                     top = warp_max(top);

@@ -58,3 +58,16 @@ def test_append_tiny_rows(L, act, heads):
     assert L.gcuda_op_paged_append(ref(plan.kv), ref(plan.batch), ref(x["desc"]), stream()) == 0
     torch.cuda.synchronize()
     check_append(plan, x, act, heads, False, before, scales)
+
+
+@pytest.mark.parametrize("cache", ["i8", "bf16", "f16"])
+@pytest.mark.parametrize("act", ["f32", "bf16"])
+@pytest.mark.parametrize("tokens", [1, 5])
+def test_attend_tiny_queries(L, act, cache, tokens):
+    """Queries far below 1 under a softmax scale that makes up for it."""
+    plan = Plan([tokens, 1], [70, 9], 16, 2, 64, cache, seed=2)
+    plan.randomize(3)
+    x = attn_inputs(L, plan, act, 16, 4, q_scale=3e-37, scale=4e35)
+    assert run_attn(L, plan, x) == 0
+    torch.cuda.synchronize()
+    check_attn(plan, x, act, 16)
