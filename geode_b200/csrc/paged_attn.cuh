@@ -1053,7 +1053,8 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn(PagedAttnAr
             for (int w = 0; w < 4; ++w)
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
-                    Ls[c] += st[w][c].x == -INFINITY ? 0.0f : st[w][c].y * ex2(st[w][c].x - M[c]);
+                    // (a sum of 0: nothing seen. One that is no number stays so, though no maximum came with it)
+                    Ls[c] += st[w][c].y == 0.0f ? 0.0f : st[w][c].y * ex2(st[w][c].x - M[c]);
                     f[w][c] = st[w][c].z == -INFINITY ? 0.0f : ex2(st[w][c].z - Mo[c]);
                 }
             const float inv0 = row_factor(M[0], Ls[0], Mo[0]), inv1 = row_factor(M[1], Ls[1], Mo[1]);
@@ -1154,7 +1155,7 @@ __global__ void __launch_bounds__(kJoinThreads, 1) k_paged_attn_join(PagedAttnAr
             float f[2];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                L[h] += st[b][h].x == -INFINITY ? 0.0f : st[b][h].y * ex2(st[b][h].x - M[h]);
+                L[h] += st[b][h].y == 0.0f ? 0.0f : st[b][h].y * ex2(st[b][h].x - M[h]);   // (as at a segment's end)
                 f[h] = st[b][h].z == -INFINITY ? 0.0f : ex2(st[b][h].z - Mo[h]);
             }
 #pragma unroll

@@ -37,6 +37,19 @@ def status_clear(L):
     assert L.gcuda_op_status(1) == 0   # (a test that raises flags clears them itself)
 
 
+class LongPlan(Plan):
+    """A plan whose sequences are long or many: their values by one gather each."""
+
+    def values(self, s, which, upto):
+        P = self.page
+        pos = torch.arange(upto)
+        page = torch.from_numpy(self.table_host[s].astype(np.int64))[pos // P]
+        x = self.view[page.to(self.device), which, (pos % P).to(self.device)].cpu().double()
+        if self.scale_view is not None:
+            x = x * self.scale_view[page.to(self.device), which, (pos % P).to(self.device)].cpu().double()[..., None]
+        return x
+
+
 # ------------------------------------------------------------------------------------------- tiny values ----
 @pytest.mark.parametrize("act", ["f32", "bf16"])
 @pytest.mark.parametrize("heads", [0, 2])
@@ -71,3 +84,44 @@ def test_attend_tiny_queries(L, act, cache, tokens):
     assert run_attn(L, plan, x) == 0
     torch.cuda.synchronize()
     check_attn(plan, x, act, 16)
+
+
+# ---------------------------------------------------------------------------------------- rows of no numbers ----
+@pytest.mark.parametrize("act,cache", [("f32", "i8"), ("bf16", "i8"), ("bf16", "bf16"), ("f32", "bf16"), ("f16", "f16"), ("f32", "f16")])
+@pytest.mark.parametrize("tokens,heads", [(1, 8), (5, 8), (2, 1), (2, 8)])
+@pytest.mark.parametrize("length", [5, 6001])
+def test_attend_nan_query(L, act, cache, tokens, heads, length):
+    """A query that is no number gives none, neither out nor lse, whether its item is cut or not; the others' bits stay."""
+    plan = LongPlan([tokens, 1], [length, 40], 16, 1, 64, cache, seed=3)
+    plan.randomize(4)
+    x = attn_inputs(L, plan, act, heads, 5)
+    assert run_attn(L, plan, x) == 0
+    torch.cuda.synchronize()
+    out, lse = x["out"].clone(), x["lse"].clone()
+    row, head = tokens - 1, heads // 2
+    x["q"][row, head, 17] = math.nan
+    assert run_attn(L, plan, x) == 0
+    torch.cuda.synchronize()
+    assert torch.isnan(x["out"][row, head].float()).all() and torch.isnan(x["lse"][row, head])
+    x["out"][row, head], x["lse"][row, head] = out[row, head], lse[row, head]
+    assert torch.equal(x["out"], out) and torch.equal(x["lse"], lse)
+
+
+@pytest.mark.parametrize("act,cache", [("f32", "i8"), ("bf16", "bf16"), ("f16", "f16")])
+@pytest.mark.parametrize("tokens", [1, 5])
+@pytest.mark.parametrize("length", [1, 33, 6001])
+def test_attend_nan_key(L, act, cache, tokens, length):
+    """A key that is no number, alone in its warp's positions: out and lse of the rows that see it are no numbers."""
+    length = max(length, tokens)
+    plan = LongPlan([tokens], [length], 16, 1, 64, cache, seed=5)
+    plan.randomize(6)
+    x = attn_inputs(L, plan, act, 8, 7)
+    p = length - tokens   # (every row sees it)
+    at = (int(plan.table_host[0, p // 16]), 0, p % 16)
+    if cache == "i8":
+        plan.scale_view[at] = math.nan
+    else:
+        plan.view[at] = math.nan
+    assert run_attn(L, plan, x) == 0
+    torch.cuda.synchronize()
+    assert torch.isnan(x["out"].float()).all() and torch.isnan(x["lse"]).all()
