@@ -121,7 +121,9 @@ int gcuda_op_paged_append(const gcuda_paged_kv *kv, const gcuda_paged_batch *b, 
             !apart({x->k, x->k_stride, kv_width}, out, b->n_rows, es) || !apart({x->v, x->v_stride, kv_width}, out, b->n_rows, es))
             return GCUDA_E_ARG;
     }
-    if (const int rc = on_current_device(kv->k, x->k)) return rc;
+    if (const int rc = on_current_device(kv->k, kv->v, kv->k_scale, kv->v_scale, b->row_start, b->length, b->pages, x->q, x->k, x->v, x->q_out,
+                                         x->q_norm, x->k_norm, x->rope_dim > 0 ? x->inv_freq : nullptr))
+        return rc;
     // A row's warps: one where the rows alone make three CTAs an SM, else more, up to a turn for every warp
     const int per_turn = 256 / kv->head_dim;   // vectors
     const int turns = (x->n_heads + per_turn - 1) / per_turn + 2 * ((kv->n_kv_heads + per_turn - 1) / per_turn);
@@ -164,7 +166,8 @@ int gcuda_op_paged_attn(const gcuda_paged_kv *kv, const gcuda_paged_batch *b, co
         !apart(query_rows(x->q, x->type, x->q_stride, x->q_head_stride, x->n_heads, kv->head_dim),
                {x->out, x->out_stride, static_cast<int64_t>(x->n_heads) * kv->head_dim}, b->n_rows, es))
         return GCUDA_E_ARG;
-    if (const int rc = on_current_device(kv->k, x->out)) return rc;
+    if (const int rc = on_current_device(kv->k, kv->v, kv->k_scale, kv->v_scale, b->row_start, b->length, b->pages, x->q, x->out, x->lse, d_work))
+        return rc;
     const PagedAttnPlan p = plan_paged_attn(*kv, *b, x->n_heads);
     uint8_t *w = static_cast<uint8_t *>(d_work);
     // p / page_size by a multiplication, exact for p < 2^31: with 2^l >= page_size the multiplier is less than
@@ -202,7 +205,9 @@ int gcuda_op_logits_adjust(const gcuda_logit_rules *r, const void *d_in, void *d
     const int64_t es = static_cast<int64_t>(value_bytes(type)), ib = ((rows - 1) * in_stride + V) * es,
                   ob = ((rows - 1) * out_stride + V) * es;
     if (i0 == o0 ? in_stride != out_stride : (i0 < o0 + ob && o0 < i0 + ib)) return GCUDA_E_ARG;
-    if (const int rc = on_current_device(d_in, d_out)) return rc;
+    if (const int rc = on_current_device(d_in, d_out, r->history, r->history_len, r->drafts, r->repetition, r->frequency, r->presence, r->bias_id,
+                                         r->bias, r->bias_len, r->mask, r->mask_row))
+        return rc;
     AdjustArgs a{*r, d_in, d_out, S, k, V, 0, in_stride, out_stride, device_status()};
     if (!a.status) return GCUDA_E_CUDA;
     cudaStream_t st = static_cast<cudaStream_t>(stream);

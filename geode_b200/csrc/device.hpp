@@ -58,9 +58,10 @@ inline int sm_count() {
     return d.sms[dev];
 }
 
-// GCUDA_OK where the pointers are memory of the current device, else GCUDA_E_ARG (a kernel that follows one of another
-// device faults where no peer access was set up); GCUDA_E_CUDA without a device. The driver's single attribute: the runtime's query of all of them takes 2.5 us a pointer. The
-// driver's function comes through the runtime, so the library loads where no driver is installed.
+// GCUDA_OK where the pointers (NULL: passed over) can be followed on the current device - its own memory, page-locked host
+// memory, managed memory - else GCUDA_E_ARG (a kernel that follows memory of another device, or an ordinary host address,
+// faults); GCUDA_E_CUDA without a device. The driver's single attribute, 29 ns a pointer: the runtime's query of all of them
+// takes 2.5 us. The driver's function comes through the runtime, so the library loads where no driver is installed.
 inline decltype(&cuPointerGetAttribute) pointer_attribute() {
     static const auto fn = [] {
         void *f = nullptr;
@@ -75,10 +76,13 @@ template <typename... P>
 inline int on_current_device(const P *...p) {
     const int dev = current_device();
     if (dev < 0 || !pointer_attribute()) return GCUDA_E_CUDA;
+    auto ask = [](const void *q, CUpointer_attribute what) {   // (-1: unknown to the driver)
+        int v = 0;
+        return pointer_attribute()(&v, what, reinterpret_cast<CUdeviceptr>(q)) == CUDA_SUCCESS ? v : -1;
+    };
     auto here = [&](const void *q) {
-        int at = -1;
-        return pointer_attribute()(&at, CU_POINTER_ATTRIBUTE_DEVICE_ORDINAL, reinterpret_cast<CUdeviceptr>(q)) == CUDA_SUCCESS &&
-               at == dev;
+        return !q || ask(q, CU_POINTER_ATTRIBUTE_DEVICE_ORDINAL) == dev || ask(q, CU_POINTER_ATTRIBUTE_MEMORY_TYPE) == CU_MEMORYTYPE_HOST ||
+               ask(q, CU_POINTER_ATTRIBUTE_IS_MANAGED) == 1;
     };
     return (here(p) && ...) ? GCUDA_OK : GCUDA_E_ARG;
 }

@@ -357,8 +357,9 @@ int gcuda_op_spec_reject_static(const float *d_target, const float *d_draft, con
  * gcuda_op_greedy_verify or the rejection samplers then accept from. No counterpart in the reference, which holds one
  * conversation in one contiguous cache (its arithmetic per row: engine/src/model.cpp:3705-3797, 3815-4019, and the
  * presence penalty of engine/src/geode.cpp:234-255).
- * They run on the current device; a cache, rows or logits that are not that device's memory are refused (GCUDA_E_ARG), as
- * is any array that is not aligned to its values; a stream of another device fails (GCUDA_E_CUDA). None allocates, waits or needs a call before a stream capture.
+ * They run on the current device. Every array must be memory that it can follow: its own, page-locked host memory or managed
+ * memory; any other address is refused (GCUDA_E_ARG), as is any array that is not aligned to its values. A stream of another
+ * device fails (GCUDA_E_CUDA). None allocates, waits or needs a call before a stream capture.
  *
  * Types of values: activations and 16-bit cache rows are read and written as these; GCUDA_I8 rows are int8 codes with
  * one float scale per (position, head), as the engine's cache (value = code * scale). */

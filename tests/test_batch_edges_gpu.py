@@ -125,3 +125,67 @@ def test_attend_nan_key(L, act, cache, tokens, length):
     assert run_attn(L, plan, x) == 0
     torch.cuda.synchronize()
     assert torch.isnan(x["out"].float()).all() and torch.isnan(x["lse"]).all()
+
+
+# ------------------------------------------------------------------------------------------------- the device ----
+def host_address(keep):
+    """An address of ordinary host memory, 256-byte aligned."""
+    a = np.zeros(1 << 16, np.uint8)
+    keep.append(a)
+    return (a.ctypes.data + 255) // 256 * 256
+
+
+def test_every_buffer_elsewhere_is_refused(L):
+    """Each array that a kernel would follow, as host memory: refused before anything is launched."""
+    keep = []
+    plan = Plan([2], [5], 16, 2, 64, "i8")
+    x = attn_inputs(L, plan, "f32", 4, 1)
+    y = append_inputs(plan, "f32", 4, 64, True, 1)
+
+    def swapped(d, name, f):
+        was = getattr(d, name)
+        setattr(d, name, host_address(keep))
+        rc = f()
+        setattr(d, name, was)
+        return rc
+
+    attend = lambda: run_attn(L, plan, x)  # noqa: E731
+    append = lambda: L.gcuda_op_paged_append(ref(plan.kv), ref(plan.batch), ref(y["desc"]), stream())  # noqa: E731
+    for name in ("k", "v", "k_scale", "v_scale"):
+        assert swapped(plan.kv, name, attend) == -1 and swapped(plan.kv, name, append) == -1, name
+    for name in ("row_start", "length", "pages"):
+        assert swapped(plan.batch, name, attend) == -1 and swapped(plan.batch, name, append) == -1, name
+    for name in ("q", "out", "lse"):
+        assert swapped(x["desc"], name, attend) == -1, name
+    for name in ("q", "k", "v", "q_out", "q_norm", "k_norm", "inv_freq"):
+        assert swapped(y["desc"], name, append) == -1, name
+    work = host_address(keep)
+    assert L.gcuda_op_paged_attn(ref(plan.kv), ref(plan.batch), ref(x["desc"]), work, x["need"], stream()) == -1
+    h, t, r = rules_for(2, 2, 500, 3)
+    src, dst = torch.zeros(6, 500, device="cuda"), torch.zeros(6, 500, device="cuda")
+    adjust = lambda a, b: L.gcuda_op_logits_adjust(ref(r), a, b, gb.F32, 2, 2, 500, 500, 500, stream())  # noqa: E731
+    for name in ("history", "history_len", "drafts", "repetition", "frequency", "presence", "bias_id", "bias", "bias_len", "mask", "mask_row"):
+        assert swapped(r, name, lambda: adjust(src.data_ptr(), dst.data_ptr())) == -1, name
+    assert adjust(host_address(keep), dst.data_ptr()) == -1 and adjust(src.data_ptr(), host_address(keep)) == -1
+    assert attend() == 0 and append() == 0 and adjust(src.data_ptr(), dst.data_ptr()) == 0
+    torch.cuda.synchronize()
+
+
+def test_page_locked_and_managed_memory_is_taken(L):
+    """Host memory that the device can follow: a plan may lie there, and the outputs in managed memory."""
+    plan = Plan([2], [5], 16, 2, 64, "bf16")
+    plan.randomize(1)
+    x = attn_inputs(L, plan, "bf16", 4, 1)
+    pinned = [t.cpu().pin_memory() for t in (plan.row_start, plan.length, plan.table)]
+    plan.batch.row_start, plan.batch.length, plan.batch.pages = (t.data_ptr() for t in pinned)
+    assert run_attn(L, plan, x) == 0
+    torch.cuda.synchronize()
+    check_attn(plan, x, "bf16", 4)
+    p = C.c_void_p()
+    assert L.cudaMallocManaged(C.byref(p), C.c_size_t(4096), 1) == 0   # (of the runtime that the library is linked with)
+    x["desc"].lse = p.value
+    assert run_attn(L, plan, x) == 0
+    torch.cuda.synchronize()
+    lse = np.ctypeslib.as_array(C.cast(p, C.POINTER(C.c_float)), (2, 4)).copy()
+    assert L.cudaFree(p) == 0
+    assert np.array_equal(lse, x["lse"].cpu().numpy())
