@@ -189,3 +189,42 @@ def test_page_locked_and_managed_memory_is_taken(L):
     lse = np.ctypeslib.as_array(C.cast(p, C.POINTER(C.c_float)), (2, 4)).copy()
     assert L.cudaFree(p) == 0
     assert np.array_equal(lse, x["lse"].cpu().numpy())
+
+
+THREADS = """
+import sys, threading
+sys.path[:0] = [{root!r}, {tests!r}]
+import torch
+import batch_helpers as bh
+from geode_b200 import batch as gb, cuda_lib
+from test_batch_gpu import append_inputs, attn_inputs, run_attn, check_attn
+L = cuda_lib()
+plan = bh.Plan([1, 2], [40, 70], 16, 2, 64, "i8")
+plan.randomize(1)
+x = attn_inputs(L, plan, "f32", 4, 2)
+y = append_inputs(plan, "f32", 4, 32, True, 1)
+src, dst = torch.randn(2, 100, device="cuda"), torch.zeros(2, 100, device="cuda")
+r = gb.LogitRules()
+st = torch.cuda.current_stream().cuda_stream
+torch.cuda.synchronize()
+rc = []
+def call(which):
+    if which == 0: rc.append(run_attn(L, plan, x, st))
+    if which == 1: rc.append(L.gcuda_op_paged_append(bh.ref(plan.kv), bh.ref(plan.batch), bh.ref(y["desc"]), st))
+    if which == 2: rc.append(L.gcuda_op_logits_adjust(bh.ref(r), src.data_ptr(), dst.data_ptr(), gb.F32, 2, 0, 100, 100, 100, st))
+for which in (0, 1, 2):
+    t = threading.Thread(target=call, args=(which,))
+    t.start(); t.join()
+torch.cuda.synchronize()
+assert rc == [0, 0, 0], rc
+assert torch.equal(src, dst)
+print("threads")
+"""
+
+
+def test_first_call_of_a_thread(L):
+    """A thread's first call into CUDA may be one of these."""
+    here = os.path.dirname(os.path.abspath(__file__))
+    code = THREADS.format(root=os.path.dirname(here), tests=here)
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "threads" in r.stdout, r.stderr[-2000:]
