@@ -228,3 +228,47 @@ def test_first_call_of_a_thread(L):
     code = THREADS.format(root=os.path.dirname(here), tests=here)
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and "threads" in r.stdout, r.stderr[-2000:]
+
+
+# ---------------------------------------------------------------------------------------------- wrong plans ----
+def left_out(plan, bad):
+    """The plan as the operators see it: the bad sequences own nothing."""
+    for s in bad:
+        plan.rows[s] = 0
+
+
+BAD_PLANS = [
+    # lengths, row_start (None: as it should be), the sequences that are left out
+    ([49, 17, 9], None, [0]), ([5, -3, 9], None, [1]), ([5, 17, 2**31 - 1], None, [2]), ([-2**31, 17, 33], None, [0, 2]),
+    ([5, 17, 9], [0, 9, 2, 3], [0, 1]), ([5, 17, 9], [-2, 1, 2, 3], [0]), ([5, 17, 9], [0, 1, 2, 99], [2]),
+    ([5, 17, 9], [0, 1, 2, 4], [2]), ([5, 17, 9], [2**31 - 1, 1, 2, 3], [0]), ([5, 17, 9], [0, 2, 2, 3], [0, 1]),
+]
+
+
+@pytest.mark.parametrize("lengths,starts,bad", BAD_PLANS, ids=str)
+@pytest.mark.parametrize("cache", ["i8", "bf16"])
+def test_wrong_plans(L, lengths, starts, bad, cache):
+    """Sequences whose rows or lengths are out of range are left out whole, flagged, and the others served: rows, cache and
+    outputs exactly."""
+    plan = Plan([1, 1, 1], [5, 17, 9], 16, 2, 64, cache, seed=2)
+    plan.batch.n_rows = 3
+    before, scales = plan.randomize(3)
+    plan.length.copy_(torch.tensor(lengths, dtype=torch.int32))
+    if starts:
+        plan.row_start.copy_(torch.tensor(starts, dtype=torch.int32))
+        plan.start_host = np.array(starts, np.int32)
+    left_out(plan, bad)
+    act = "f32" if cache == "i8" else "bf16"
+    y = attn_inputs(L, plan, act, 4, 5)
+    assert run_attn(L, plan, y) == 0
+    torch.cuda.synchronize()
+    assert L.gcuda_op_status(1) == 2
+    check_attn(plan, y, act, 4)      # (rows of no good sequence: as they were)
+    x = append_inputs(plan, act, 2, 32, True, 4)
+    assert L.gcuda_op_paged_append(ref(plan.kv), ref(plan.batch), ref(x["desc"]), stream()) == 0
+    torch.cuda.synchronize()
+    assert L.gcuda_op_status(1) in (0, 2)   # (a bad sequence that no row falls to is not met)
+    check_append(plan, x, act, 2, True, before, scales)
+    owned = {int(plan.start_host[s]) for s in range(3) if plan.rows[s]}
+    for row in range(3):
+        assert (x["q_out"][row] == 77.0).all() == (row not in owned)
