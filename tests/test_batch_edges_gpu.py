@@ -272,3 +272,41 @@ def test_wrong_plans(L, lengths, starts, bad, cache):
     owned = {int(plan.start_host[s]) for s in range(3) if plan.rows[s]}
     for row in range(3):
         assert (x["q_out"][row] == 77.0).all() == (row not in owned)
+
+
+# ---------------------------------------------------------------------------------------------- unseen values ----
+@pytest.mark.parametrize("heads,tokens", [(1, 4), (1, 8), (2, 4), (4, 4), (8, 5), (16, 4)])   # rows an item: 4, 8, 8, 16, 40, 64
+@pytest.mark.parametrize("act,cache", [("bf16", "bf16"), ("f32", "bf16"), ("f16", "f16"), ("f32", "f16"), ("bf16", "i8"), ("f32", "i8")])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_unseen_values_in_every_shape(L, heads, tokens, act, cache, dim, bad):
+    """The newest position, which only the last row sees, and (under a window) the oldest one, which only the first row
+    sees: whatever they hold, the other rows' bits stay."""
+    for window in (0, 21):
+        plan = LongPlan([tokens, tokens], [130 + tokens, tokens], 16, 1, dim, cache, seed=8)
+        plan.randomize(9)
+        x = attn_inputs(L, plan, act, heads, 10, window=window)
+        assert run_attn(L, plan, x) == 0
+        torch.cuda.synchronize()
+        clean, clean_lse = x["out"].clone(), x["lse"].clone()
+        check_attn(plan, x, act, heads)
+        places = [(0, plan.lengths[0] - 1, tokens - 1), (1, plan.lengths[1] - 1, 2 * tokens - 1)]
+        if window:
+            places.append((0, plan.lengths[0] - tokens + 1 - window, 0))
+        for which in (0, 1):   # keys, values
+            target = plan.scale_view if cache == "i8" else plan.view
+            kept = target.clone()
+            touched = set()
+            for s, p, row in places:
+                target[int(plan.table_host[s, p // 16]), which, p % 16] = bad
+                touched.add(row)
+            assert run_attn(L, plan, x) == 0
+            torch.cuda.synchronize()
+            target.copy_(kept)
+            # (a key's scale of inf makes scores of -inf, weights of 0, as well as inf: nothing to say about the rows that see it)
+            either = which == 0 and cache == "i8" and bad == math.inf
+            for row in range(2 * tokens):
+                if row not in touched:
+                    assert torch.equal(x["out"][row], clean[row]) and torch.equal(x["lse"][row], clean_lse[row]), (window, which, row)
+                elif not either:
+                    assert not torch.isfinite(x["out"][row].float()).any(), (window, which, row)
