@@ -310,3 +310,156 @@ def test_unseen_values_in_every_shape(L, heads, tokens, act, cache, dim, bad):
                     assert torch.equal(x["out"][row], clean[row]) and torch.equal(x["lse"][row], clean_lse[row]), (window, which, row)
                 elif not either:
                     assert not torch.isfinite(x["out"][row].float()).any(), (window, which, row)
+
+
+# ----------------------------------------------------------------------------------------- many tiles, many items ----
+@pytest.mark.parametrize("act,cache", [("f32", "i8"), ("bf16", "i8"), ("f16", "i8"), ("bf16", "bf16"), ("f32", "bf16"), ("f16", "f16"), ("f32", "f16")])
+@pytest.mark.parametrize("tokens", [1, 2, 5])   # of 8 query heads a key head: 8, 16 and 40 rows
+@pytest.mark.parametrize("dim", [64, 256])
+def test_many_items_a_cta(L, act, cache, tokens, dim):
+    """128 ragged sequences of two key heads: 256 items of several tiles each, more than the CTAs: a CTA goes from tile to
+    tile and from item to item, and items are cut between CTAs."""
+    rng = np.random.default_rng(dim + tokens)
+    n = 128
+    rows = [int(v) for v in rng.integers(1, tokens + 1, n)]
+    lengths = [max(r, int(v)) for r, v in zip(rows, rng.integers(1, 1500 if dim == 64 else 700, n))]
+    plan = LongPlan(rows, lengths, 32, 2, dim, cache, seed=dim, max_rows=tokens)
+    plan.randomize(11)
+    x = attn_inputs(L, plan, act, 16, 12, q_scale=2.0)
+    assert run_attn(L, plan, x) == 0
+    torch.cuda.synchronize()
+    check_attn(plan, x, act, 16)
+    again = x["out"].clone(), x["lse"].clone()
+    for _ in range(4):   # the same bits run after run, whatever the scratch held
+        x["work"].random_(0, 256)
+        x["out"].fill_(3.0)
+        assert run_attn(L, plan, x) == 0
+        torch.cuda.synchronize()
+        assert torch.equal(again[0], x["out"]) and torch.equal(again[1], x["lse"])
+
+
+@pytest.mark.parametrize("act,cache,tokens,dim", [("f32", "i8", 1, 128), ("f32", "i8", 5, 128), ("bf16", "bf16", 1, 128), ("bf16", "bf16", 3, 64),
+                                                  ("f16", "f16", 5, 128), ("f16", "f16", 1, 64)])
+def test_many_tiles_a_cta(L, act, cache, tokens, dim):
+    """One sequence of 100000 positions with scores that climb: a CTA's running maxima are carried, and grow, from tile to
+    tile."""
+    n = 100_000
+    plan = LongPlan([tokens], [n], 64, 1, dim, cache, seed=5)
+    plan.randomize(6)
+    x = attn_inputs(L, plan, act, 8, 7)
+    # a direction that all queries share, along which the keys grow with the position
+    P = plan.page
+    u = torch.zeros(dim)
+    u[:8] = 1.0
+    climb = torch.linspace(0, 1, n)
+    pos = torch.arange(n)
+    page = torch.from_numpy(plan.table_host[0].astype(np.int64))[pos // P]
+    if cache == "i8":
+        codes = plan.view[page.cuda(), 0, (pos % P).cuda()]
+        codes[:, 0] = (codes[:, 0].float() * 0.3 + (90 * climb[:, None] * u).cuda()).round().clamp(-127, 127).to(torch.int8)
+        plan.view[page.cuda(), 0, (pos % P).cuda()] = codes
+    else:
+        k = plan.view[page.cuda(), 0, (pos % P).cuda()].float()
+        k[:, 0] += (4 * climb[:, None] * u).cuda()
+        plan.view[page.cuda(), 0, (pos % P).cuda()] = k.to(plan.view.dtype)
+    x["q"][..., :8] += 6.0
+    assert run_attn(L, plan, x) == 0
+    torch.cuda.synchronize()
+    check_attn(plan, x, act, 8)
+
+
+# ------------------------------------------------------------------------------------------- many turns a warp ----
+@pytest.mark.parametrize("act,cache,heads,nkv,dim,rope,norm", [("bf16", "bf16", 16, 4, 128, 128, False), ("f16", "i8", 32, 4, 128, 128, True),
+                                                             ("f32", "i8", 16, 2, 256, 64, True), ("f32", "f16", 24, 3, 64, 36, True),
+                                                             ("bf16", "i8", 9, 5, 256, 256, False)])
+def test_append_many_turns(L, act, cache, heads, nkv, dim, rope, norm):
+    """Prompts: more rows than warps, so that a warp goes through all of a row's turns and its ring is used over and over;
+    every row against the definition."""
+    rows, lengths = [1500, 1, 2300], [1500, 90, 4001]
+    plan = Plan(rows, lengths, 32, nkv, dim, cache, seed=1, spare=3)
+    plan.randomize(2)
+    before, scales = plan.view.clone(), None if plan.scale_view is None else plan.scale_view.clone()
+    x = append_inputs(plan, act, heads, rope, norm, 3)
+    assert L.gcuda_op_paged_append(ref(plan.kv), ref(plan.batch), ref(x["desc"]), stream()) == 0
+    torch.cuda.synchronize()
+    N = sum(rows)
+    pos = torch.cat([torch.arange(n - r, n) for r, n in zip(rows, lengths)])
+    page = torch.cat([torch.from_numpy(plan.table_host[s].astype(np.int64))[torch.arange(n - r, n) // 32] for s, (r, n) in enumerate(zip(rows, lengths))])
+    angle = pos.double()[:, None, None] * x["freq"].cpu().double()
+    h = rope // 2
+
+    def vectors(v, w):   # [row][head][dim] in 64 bits
+        v = v.double()
+        if norm:
+            v = v / (v.square().mean(-1, keepdim=True) + float(np.float32(1e-6))).sqrt() * (1.0 + w.cpu().double())
+        a, b = v[..., :h], v[..., h:2 * h]
+        return torch.cat([a * angle.cos() - b * angle.sin(), b * angle.cos() + a * angle.sin(), v[..., 2 * h:]], -1)
+
+    def size(y):   # a rotation's two products of values up to the pair's size
+        p = y.abs().clone()
+        p[..., :h] = 2 * torch.hypot(y[..., :h], y[..., h:2 * h])
+        p[..., h:2 * h] = p[..., :h]
+        return p
+
+    arithmetic = ((dim + 5) / 2 + 12) * 2.0**-24
+    q = vectors(x["q"][:N, :, :dim].cpu(), x["qn"])
+    got = x["q_out"].cpu().double()
+    assert ((got[:N] - q).abs() <= arithmetic * size(q) + HALF_STEP[act] * 1.01 * q.abs() + 1e-7 * HALF_STEP[act]).all()
+    assert (got[N:] == 77.0).all()
+    k = vectors(x["k"][:N, :nkv * dim].cpu().view(N, nkv, dim), x["kn"])
+    v = x["v"][:N].cpu().double().view(N, nkv, dim)
+    at = (page.cuda(), slice(None), (pos % 32).cuda())
+    held = plan.view[at].cpu()
+    for which, y in ((0, k), (1, v)):
+        if cache == "i8":
+            y = y.float().double()
+            top = y.abs().amax(-1, keepdim=True)
+            codes = torch.round(y * 127.0 / top).to(torch.int8)   # (to even)
+            # the definition in 64 bits rounds to float first; this one's own 64-bit roundings may tip a value there
+            off = held[:, which] != codes
+            assert off.float().mean() <= 1e-6 and (held[:, which].int() - codes.int()).abs().max() <= 1
+            got_scale = plan.scale_view[at].cpu()[:, which]
+            want_scale = (top[..., 0] / 127.0).float()
+            assert ((got_scale - want_scale).abs() <= want_scale * 2.0**-23).all()
+        else:
+            tol = arithmetic * size(y) if which == 0 else torch.zeros_like(y)
+            assert ((held[:, which].double() - y).abs() <= tol + HALF_STEP[cache] * 1.01 * y.abs() + 2.0**-25).all()
+    # the rest of the cache as it was
+    plan.view[at] = before[at]
+    assert torch.equal(plan.view.nan_to_num(-1) if cache != "i8" else plan.view, before.nan_to_num(-1) if cache != "i8" else before)
+    if scales is not None:
+        plan.scale_view[at] = scales[at]
+        assert torch.equal(plan.scale_view.nan_to_num(-1), scales.nan_to_num(-1))
+
+
+# ------------------------------------------------------------------------------ wide vocabularies, long lists ----
+@pytest.mark.parametrize("act,S,k,V", [("f32", 24, 1, 50257), ("bf16", 30, 0, 50257), ("f16", 30, 2, 50001), ("f32", 5, 4, 248320)])
+@pytest.mark.parametrize("layout", ["apart", "in place", "strided"])
+def test_adjust_wide(L, act, S, k, V, layout):
+    """Enough slices of 4096 tokens for every SM (the kernels of large batches), lists longer than a thread's first eight
+    entries, tokens all over the vocabulary."""
+    rows, history, biases = S * (k + 1), 5000, 2300
+    h, t, r = rules_for(S, k, V, 5, history, biases, True, True)
+    rng = np.random.default_rng(6)
+    # words of all sizes, the same ones over and over
+    h["history"][:] = np.minimum(V - 1, (np.float64(V + 1) ** rng.random((S, history)) - 1)).astype(np.int32)
+    h["history"][:, 1] = -1
+    h["bias_id"][:] = rng.integers(0, V, (S, biases))
+    h["bias_id"][:, -40:] = h["bias_id"][:, :40]   # entries of one id far apart
+    h["drafts"][:] = rng.integers(0, V, h["drafts"].shape)
+    h["history_len"][:] = rng.integers(4000, history + 1, S)
+    h["bias_len"][:] = biases
+    h["history_len"][0], h["bias_len"][0] = 2048, 2049
+    for n in ("history", "bias_id", "drafts", "history_len", "bias_len"):
+        t[n].copy_(torch.from_numpy(h[n]))
+    g = torch.Generator().manual_seed(7)
+    x = (4 * torch.randn(rows, V, generator=g)).to(TORCH[act])
+    pad_in, pad_out = (5, 3) if layout == "strided" else (0, 0)
+    src = torch.full((rows, V + pad_in), 9.0, dtype=TORCH[act], device="cuda")
+    src[:, :V] = x.cuda()
+    dst = src if layout == "in place" else torch.full((rows, V + pad_out), 7.0, dtype=TORCH[act], device="cuda")
+    assert L.gcuda_op_logits_adjust(ref(r), src.data_ptr(), dst.data_ptr(), CODE[act], S, k, V, src.stride(0), dst.stride(0), stream()) == 0
+    torch.cuda.synchronize()
+    got = dst.cpu()
+    assert (got[:, V:] == 7.0).all()
+    check_adjust(x, got[:, :V], act, S, k, V, h, history, biases, True, True, (True, True, True))
