@@ -32,7 +32,7 @@ int launch_paged_rows(const PagedAttnArgs &a, const PagedAttnPlan &p, cudaStream
 }
 template <int CACHE, int HD>
 int launch_paged_split(const PagedAttnArgs &a, const PagedAttnPlan &p, cudaStream_t st) {
-    const bool split = a.x.type == GCUDA_F32 || (a.x.type == GCUDA_F16 && CACHE == GCUDA_BF16);
+    const bool split = a.x.type == GCUDA_F32 || (a.x.type == GCUDA_F16 && CACHE != GCUDA_F16);   // (over int8: weights of two numbers)
     return split ? launch_paged_rows<CACHE, HD, true>(a, p, st) : launch_paged_rows<CACHE, HD, false>(a, p, st);
 }
 template <int CACHE>

@@ -127,6 +127,36 @@ def test_attend_nan_key(L, act, cache, tokens, length):
     assert torch.isnan(x["out"].float()).all() and torch.isnan(x["lse"]).all()
 
 
+# --------------------------------------------------------------------------------------------------- weights ----
+@pytest.mark.parametrize("cache", ["i8", "f16"])
+@pytest.mark.parametrize("tokens", [1, 2, 5])
+@pytest.mark.parametrize("dim", [64, 256])
+def test_attend_f16_weights(L, cache, tokens, dim):
+    """f16 activations: what the weights are rounded to is finer than the output's own rounding (values that cancel show
+    it). The bound is check_attn's with weights of two f16 numbers: each to 2^-22."""
+    plan = LongPlan([tokens] * 6, [tokens + 1, tokens + 2, 40, 200, 70, 1000], 16, 2, dim, cache, seed=7)
+    plan.randomize(8)
+    if cache == "f16":   # neighbours that nearly cancel
+        for s in range(6):
+            for p in range(0, plan.lengths[s] - 1, 2):
+                a, b = ((int(plan.table_host[s, q // 16]), 1, q % 16) for q in (p, p + 1))
+                plan.view[b] = -plan.view[a] * 0.75
+    x = attn_inputs(L, plan, "f16", 16, 9, q_scale=0.3)
+    assert run_attn(L, plan, x) == 0
+    torch.cuda.synchronize()
+    out = x["out"].cpu().double()
+    scale = float(x["desc"].scale)
+    for s, n in enumerate(plan.rows):
+        keys, values = plan.values(s, 0, plan.lengths[s]), plan.values(s, 1, plan.lengths[s])
+        for i in range(n):
+            row, end = int(plan.start_host[s]) + i, plan.lengths[s] - n + i + 1
+            q = x["q"][row].cpu().double()
+            o, _, size, mag = bh.attend(q, keys[:end], values[:end], scale)
+            ds = mag * (dim + 10) * 2.0**-24 + 2.0**-21 * q.abs().amax(-1) * keys[:end].abs().sum(-1).amax() * abs(scale)
+            tol = size * (2 * ds[:, None] + 2.0**-21 + (end + 40) * 2.0**-24) + HALF_STEP["f16"] * 1.01 * o.abs() + 2.0**-25
+            assert ((out[row] - o).abs() <= tol).all(), (s, i, float(((out[row] - o).abs() / tol).max()))
+
+
 # ------------------------------------------------------------------------------------------------- the device ----
 def host_address(keep):
     """An address of ordinary host memory, 256-byte aligned."""
