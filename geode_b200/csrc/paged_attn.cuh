@@ -18,9 +18,9 @@
 // c: every value to 2^-24 of the row's largest, each sum of products exact. Over a 16-bit cache queries are in the cache's
 // type (f16, and floats in any: scaled by a power of two per row); float activations, and f16 ones over bf16, are held as a sum
 // of such numbers: two f16 (22 bits) or three bf16 (24 bits; two would leave an error of 4e-6, three times a float product's).
-// Weights are held in two numbers of the product's 16-bit type (three bf16 for float activations over bf16): one would add as
-// much error as rounding the output to that type does. For bf16 activations over int8 they are one f16, an error of at most
-// 2^-11 of each, an eighth of the output's own rounding.
+// Weights are held in two numbers of the product's 16-bit type, f16 over int8 (three bf16 for float activations over bf16): one
+// would add as much error as rounding the output to that type does, and turn one in eleven of bf16 outputs over int8 to the
+// neighbouring number (two: one in a thousand; the second number costs 2% there, up to 9% where the products weigh).
 // int8 rows' value scales go into the weight's exponent: w = 2^(s + log2 vs - m'), with a maximum m' of its own, so that
 // rows of any scale keep their bits. Scores, sums, maxima and outputs are float.
 //
@@ -63,7 +63,7 @@ struct PagedBase {
     static constexpr bool SPLIT = SPLIT_, I8 = CACHE == GCUDA_I8, BF16 = CACHE == GCUDA_BF16;
     static constexpr int ES = I8 ? 1 : 2, RB = HD * ES, OM = HD / 16;
     static constexpr bool THREE = SPLIT && BF16;                 // floats as three numbers
-    static constexpr int PN = THREE ? 3 : SPLIT || !I8 ? 2 : 1;  // numbers of a weight
+    static constexpr int PN = THREE ? 3 : 2;                     // numbers of a weight
     // the queries' fragments: int8 three digits a value in k steps of 32 dims, else one to three numbers in k steps of 16
     static constexpr int kQ = I8 ? HD / 32 * NT * 32 * 24 : HD / 16 * NT * 32 * 8 * (THREE ? 3 : SPLIT ? 2 : 1);
     static constexpr int kQTwo = I8 ? HD / 32 * NT * 32 * 16 : THREE ? HD / 16 * NT * 32 * 16 : 0;   // (where the third ones start)

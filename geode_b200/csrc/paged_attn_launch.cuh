@@ -32,8 +32,12 @@ int launch_paged_rows(const PagedAttnArgs &a, const PagedAttnPlan &p, cudaStream
 }
 template <int CACHE, int HD>
 int launch_paged_split(const PagedAttnArgs &a, const PagedAttnPlan &p, cudaStream_t st) {
-    const bool split = a.x.type == GCUDA_F32 || (a.x.type == GCUDA_F16 && CACHE != GCUDA_F16);   // (over int8: weights of two numbers)
-    return split ? launch_paged_rows<CACHE, HD, true>(a, p, st) : launch_paged_rows<CACHE, HD, false>(a, p, st);
+    if constexpr (CACHE == GCUDA_I8) {
+        return launch_paged_rows<CACHE, HD, false>(a, p, st);   // (the queries' digits are the same for all activations)
+    } else {
+        const bool split = a.x.type == GCUDA_F32 || (a.x.type == GCUDA_F16 && CACHE == GCUDA_BF16);
+        return split ? launch_paged_rows<CACHE, HD, true>(a, p, st) : launch_paged_rows<CACHE, HD, false>(a, p, st);
+    }
 }
 template <int CACHE>
 int launch_paged_cache(const PagedAttnArgs &a, const PagedAttnPlan &p, cudaStream_t st) {

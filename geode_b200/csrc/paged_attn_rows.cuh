@@ -300,9 +300,8 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn_rows(PagedA
                     }
                 }
                 const int f = (warp * NT + nt) * 32 + lane;
-                if constexpr (PN > 1) reinterpret_cast<uint4 *>(sm + S::o_p)[f] = make_uint4(part[0][0], part[0][1], part[1][0], part[1][1]);
-                if constexpr (PN != 2)
-                    reinterpret_cast<uint2 *>(sm + S::o_p + S::kPTwo)[f] = make_uint2(part[PN - 1][0], part[PN - 1][1]);
+                reinterpret_cast<uint4 *>(sm + S::o_p)[f] = make_uint4(part[0][0], part[0][1], part[1][0], part[1][1]);
+                if constexpr (S::THREE) reinterpret_cast<uint2 *>(sm + S::o_p + S::kPTwo)[f] = make_uint2(part[2][0], part[2][1]);
             }
             // ---- O^T += V^T P^T of this warp's dims
             const uint8_t *ev = next_entry(std::integral_constant<int, 1>{});   // (its barrier: the weights are there too)
@@ -341,12 +340,7 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn_rows(PagedA
                         }
                     }
             };
-            auto weights = [&](int kt, int nt) {
-                const int f = (kt * NT + nt) * 32 + lane;
-                if constexpr (PN > 1) return reinterpret_cast<const uint4 *>(sm + S::o_p)[f];
-                const uint2 b = reinterpret_cast<const uint2 *>(sm + S::o_p)[f];
-                return make_uint4(b.x, b.y, 0, 0);
-            };
+            auto weights = [&](int kt, int nt) { return reinterpret_cast<const uint4 *>(sm + S::o_p)[(kt * NT + nt) * 32 + lane]; };
             auto third = [&](int kt, int nt) { return reinterpret_cast<const uint2 *>(sm + S::o_p + S::kPTwo)[(kt * NT + nt) * 32 + lane]; };
             // (values that a row does not see: as in k_paged_attn)
             bool apart = false;
@@ -378,9 +372,8 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn_rows(PagedA
                         const uint4 b = weights(kt, nt);
 #pragma unroll
                         for (int k = 0; k < MW; ++k) mma_16816<BF16>(o[k][nt], va[k][0], va[k][1], va[k][2], va[k][3], b.x, b.y);
-                        if constexpr (PN > 1)
 #pragma unroll
-                            for (int k = 0; k < MW; ++k) mma_16816<BF16>(o[k][nt], va[k][0], va[k][1], va[k][2], va[k][3], b.z, b.w);
+                        for (int k = 0; k < MW; ++k) mma_16816<BF16>(o[k][nt], va[k][0], va[k][1], va[k][2], va[k][3], b.z, b.w);
                         if constexpr (S::THREE) {
                             const uint2 c = third(kt, nt);
 #pragma unroll
@@ -411,7 +404,7 @@ __global__ void __launch_bounds__(kPagedAttnThreads, 2) k_paged_attn_rows(PagedA
                             for (int k = 0; k < MW; ++k) {
                                 float d[4] = {o[k][nt][0], o[k][nt][1], o[k][nt][2], o[k][nt][3]};
                                 mma_16816<BF16>(d, va[k][0], va[k][1], va[k][2], va[k][3], b.x, b.y);
-                                if constexpr (PN > 1) mma_16816<BF16>(d, va[k][0], va[k][1], va[k][2], va[k][3], b.z, b.w);
+                                mma_16816<BF16>(d, va[k][0], va[k][1], va[k][2], va[k][3], b.z, b.w);
                                 if constexpr (S::THREE) {
                                     const uint2 c = third(kt, nt);
                                     mma_16816<BF16>(d, va[k][0], va[k][1], va[k][2], va[k][3], c.x, c.y);

@@ -128,11 +128,11 @@ def test_attend_nan_key(L, act, cache, tokens, length):
 
 
 # --------------------------------------------------------------------------------------------------- weights ----
-@pytest.mark.parametrize("cache", ["i8", "f16"])
+@pytest.mark.parametrize("act,cache", [("f16", "i8"), ("f16", "f16"), ("bf16", "i8"), ("bf16", "f16")])
 @pytest.mark.parametrize("tokens", [1, 2, 5])
 @pytest.mark.parametrize("dim", [64, 256])
-def test_attend_f16_weights(L, cache, tokens, dim):
-    """f16 activations: what the weights are rounded to is finer than the output's own rounding (values that cancel show
+def test_attend_16_bit_weights(L, act, cache, tokens, dim):
+    """16-bit activations: what the weights are rounded to is finer than the output's own rounding (values that cancel show
     it). The bound is check_attn's with weights of two f16 numbers: each to 2^-22."""
     plan = LongPlan([tokens] * 6, [tokens + 1, tokens + 2, 40, 200, 70, 1000], 16, 2, dim, cache, seed=7)
     plan.randomize(8)
@@ -141,7 +141,7 @@ def test_attend_f16_weights(L, cache, tokens, dim):
             for p in range(0, plan.lengths[s] - 1, 2):
                 a, b = ((int(plan.table_host[s, q // 16]), 1, q % 16) for q in (p, p + 1))
                 plan.view[b] = -plan.view[a] * 0.75
-    x = attn_inputs(L, plan, "f16", 16, 9, q_scale=0.3)
+    x = attn_inputs(L, plan, act, 16, 9, q_scale=0.3)
     assert run_attn(L, plan, x) == 0
     torch.cuda.synchronize()
     out = x["out"].cpu().double()
@@ -153,7 +153,7 @@ def test_attend_f16_weights(L, cache, tokens, dim):
             q = x["q"][row].cpu().double()
             o, _, size, mag = bh.attend(q, keys[:end], values[:end], scale)
             ds = mag * (dim + 10) * 2.0**-24 + 2.0**-21 * q.abs().amax(-1) * keys[:end].abs().sum(-1).amax() * abs(scale)
-            tol = size * (2 * ds[:, None] + 2.0**-21 + (end + 40) * 2.0**-24) + HALF_STEP["f16"] * 1.01 * o.abs() + 2.0**-25
+            tol = size * (2 * ds[:, None] + 2.0**-21 + (end + 40) * 2.0**-24) + HALF_STEP[act] * 1.01 * o.abs() + 2.0**-25
             assert ((out[row] - o).abs() <= tol).all(), (s, i, float(((out[row] - o).abs() / tol).max()))
 
 
