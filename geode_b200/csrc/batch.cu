@@ -43,6 +43,23 @@ RowSpan query_rows(const void *q, int type, int64_t stride, int64_t head_stride,
     return {static_cast<const uint8_t *>(q) + std::min<int64_t>(0, over) * static_cast<int64_t>(value_bytes(type)), stride, (over < 0 ? -over : over) + head_dim};
 }
 
+// Whether a stretch of memory meets any of n rows of `width` bytes, `step` bytes apart.
+struct Stretch {
+    const void *p;
+    int64_t bytes;   // (nothing at NULL)
+};
+bool meets(const Stretch &a, const void *rows, int64_t step, int64_t width, int64_t n) {
+    if (!a.p) return false;
+    __int128 base = reinterpret_cast<uintptr_t>(rows), w = width, d = step;
+    const __int128 lo = reinterpret_cast<uintptr_t>(a.p), hi = lo + a.bytes;
+    if (d < 0) base += (n - 1) * d, d = -d;
+    if (d == 0 || n == 1) return base < hi && lo < base + w;
+    const __int128 first = lo - w < base ? 0 : (lo - w - base) / d + 1, end = hi <= base ? 0 : (hi - base + d - 1) / d;   // rows that end behind lo; that begin before hi
+    return first < (end < n ? end : n);
+}
+// rows that are written: none over another
+bool rows_apart(const RowSpan &r, int64_t n) { return n == 1 || (r.stride < 0 ? -r.stride : r.stride) >= r.width; }
+
 // The geometry alone (what the scratch's size follows from); then with the pointers
 bool good_geometry(const gcuda_paged_kv *kv, const gcuda_paged_batch *b) {
     return kv && b && (kv->type == GCUDA_I8 || kv->type == GCUDA_BF16 || kv->type == GCUDA_F16) && kv->n_pages >= 1 &&
@@ -118,7 +135,8 @@ int gcuda_op_paged_append(const gcuda_paged_kv *kv, const gcuda_paged_batch *b, 
         const int64_t kv_width = static_cast<int64_t>(kv->n_kv_heads) * kv->head_dim;
         const RowSpan out{x->q_out, x->q_out_stride, static_cast<int64_t>(x->n_heads) * kv->head_dim};
         if ((x->q != x->q_out && !apart(query_rows(x->q, x->type, x->q_stride, x->q_head_stride, x->n_heads, kv->head_dim), out, b->n_rows, es)) ||
-            !apart({x->k, x->k_stride, kv_width}, out, b->n_rows, es) || !apart({x->v, x->v_stride, kv_width}, out, b->n_rows, es))
+            !apart({x->k, x->k_stride, kv_width}, out, b->n_rows, es) || !apart({x->v, x->v_stride, kv_width}, out, b->n_rows, es) ||
+            !rows_apart(out, b->n_rows))
             return GCUDA_E_ARG;
     }
     if (const int rc = on_current_device(kv->k, kv->v, kv->k_scale, kv->v_scale, b->row_start, b->length, b->pages, x->q, x->k, x->v, x->q_out,
@@ -162,10 +180,14 @@ int gcuda_op_paged_attn(const gcuda_paged_kv *kv, const gcuda_paged_batch *b, co
     const size_t need = gcuda_op_paged_attn_work_bytes(kv, b, x->n_heads);
     if (need == 0 || work_bytes < need) return GCUDA_E_ARG;
     const size_t es = value_bytes(x->type);
-    if (misaligned(x->q, es) || misaligned(x->out, es) || !words(x->lse) ||
-        !apart(query_rows(x->q, x->type, x->q_stride, x->q_head_stride, x->n_heads, kv->head_dim),
-               {x->out, x->out_stride, static_cast<int64_t>(x->n_heads) * kv->head_dim}, b->n_rows, es))
-        return GCUDA_E_ARG;
+    if (misaligned(x->q, es) || misaligned(x->out, es) || !words(x->lse)) return GCUDA_E_ARG;
+    // out and lse apart from each other and from q
+    const RowSpan q = query_rows(x->q, x->type, x->q_stride, x->q_head_stride, x->n_heads, kv->head_dim),
+                  out{x->out, x->out_stride, static_cast<int64_t>(x->n_heads) * kv->head_dim};
+    if (!apart(q, out, b->n_rows, es) || !rows_apart(out, b->n_rows)) return GCUDA_E_ARG;
+    for (const RowSpan &r : {q, out})
+        if (meets({x->lse, static_cast<int64_t>(b->n_rows) * x->n_heads * 4}, r.p, r.stride * static_cast<int64_t>(es), r.width * static_cast<int64_t>(es), b->n_rows))
+            return GCUDA_E_ARG;
     if (const int rc = on_current_device(kv->k, kv->v, kv->k_scale, kv->v_scale, b->row_start, b->length, b->pages, x->q, x->out, x->lse, d_work))
         return rc;
     const PagedAttnPlan p = plan_paged_attn(*kv, *b, x->n_heads);
@@ -205,6 +227,12 @@ int gcuda_op_logits_adjust(const gcuda_logit_rules *r, const void *d_in, void *d
     const int64_t es = static_cast<int64_t>(value_bytes(type)), ib = ((rows - 1) * in_stride + V) * es,
                   ob = ((rows - 1) * out_stride + V) * es;
     if (i0 == o0 ? in_stride != out_stride : (i0 < o0 + ob && o0 < i0 + ib)) return GCUDA_E_ARG;
+    const int64_t n = S, lists = n * r->history_stride * 4, biases = n * r->bias_stride * 4;
+    for (const Stretch &a : {Stretch{r->history, lists}, Stretch{r->history_len, n * 4}, Stretch{r->drafts, n * k * 4}, Stretch{r->repetition, n * 4},
+                             Stretch{r->frequency, n * 4}, Stretch{r->presence, n * 4}, Stretch{r->bias_id, biases}, Stretch{r->bias, biases},
+                             Stretch{r->bias_len, n * 4}, Stretch{r->mask, r->mask ? ((r->n_masks - 1) * r->mask_stride + (V + 31) / 32) * 4 : 0},
+                             Stretch{r->mask_row, rows * 4}})
+        if (meets(a, d_out, out_stride * es, V * es, rows)) return GCUDA_E_ARG;
     if (const int rc = on_current_device(d_in, d_out, r->history, r->history_len, r->drafts, r->repetition, r->frequency, r->presence, r->bias_id,
                                          r->bias, r->bias_len, r->mask, r->mask_row))
         return rc;

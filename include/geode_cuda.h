@@ -360,6 +360,9 @@ int gcuda_op_spec_reject_static(const float *d_target, const float *d_draft, con
  * They run on the current device. Every array must be memory that it can follow: its own, page-locked host memory or managed
  * memory; any other address is refused (GCUDA_E_ARG), as is any array that is not aligned to its values. A stream of another
  * device fails (GCUDA_E_CUDA). None allocates, waits or needs a call before a stream capture.
+ * What a call writes must not lie over itself or over anything else that it reads or writes, but where the operator says so.
+ * Refused is what can be told on the host: outputs over the call's rows, lse and lists, rows of an output over each other; not
+ * told are a cache's pages and scales, the plan and the scratch.
  *
  * Types of values: activations and 16-bit cache rows are read and written as these; GCUDA_I8 rows are int8 codes with
  * one float scale per (position, head), as the engine's cache (value = code * scale). */
@@ -422,7 +425,8 @@ int gcuda_op_paged_append(const gcuda_paged_kv *kv, const gcuda_paged_batch *b, 
  * p = length[s] - T + i attends to the positions 0 .. p (the last `window` of them when window > 0):
  * out = sum softmax(scale * q . k) v, lse = log sum exp(scale * q . k). A row that sees no position (an empty
  * sequence, p < 0) gives zeros and lse -inf. Values at positions a row does not see do not touch it, whatever they
- * are. out must not overlap q (elsewhere, or other columns of rows with one stride). type: of q and out. */
+ * are; where a row does see a score that is no number, its outputs and lse are none. out must not overlap q (elsewhere, or
+ * other columns of rows with one stride), lse neither. type: of q and out. */
 typedef struct {
     int type, n_heads, window;
     float scale;
