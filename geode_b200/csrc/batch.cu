@@ -227,7 +227,8 @@ int gcuda_op_logits_adjust(const gcuda_logit_rules *r, const void *d_in, void *d
     const int64_t es = static_cast<int64_t>(value_bytes(type)), ib = ((rows - 1) * in_stride + V) * es,
                   ob = ((rows - 1) * out_stride + V) * es;
     if (i0 == o0 ? in_stride != out_stride : (i0 < o0 + ob && o0 < i0 + ib)) return GCUDA_E_ARG;
-    const int64_t n = S, lists = n * r->history_stride * 4, biases = n * r->bias_stride * 4;
+    // (of the lists' last rows the first entry: how many are used is on the device, and the rows may be columns of a wider array)
+    const int64_t n = S, lists = ((n - 1) * r->history_stride + 1) * 4, biases = ((n - 1) * r->bias_stride + 1) * 4;
     for (const Stretch &a : {Stretch{r->history, lists}, Stretch{r->history_len, n * 4}, Stretch{r->drafts, n * k * 4}, Stretch{r->repetition, n * 4},
                              Stretch{r->frequency, n * 4}, Stretch{r->presence, n * 4}, Stretch{r->bias_id, biases}, Stretch{r->bias, biases},
                              Stretch{r->bias_len, n * 4}, Stretch{r->mask, r->mask ? ((r->n_masks - 1) * r->mask_stride + (V + 31) / 32) * 4 : 0},

@@ -87,15 +87,6 @@ __global__ void __launch_bounds__(kAdjustThreads, U == 2 ? 6 : 4) k_logits_adjus
     const float rep = r.repetition ? r.repetition[s] : 1.0f, fr = r.frequency ? r.frequency[s] : 0.0f,
                 pr = r.presence ? r.presence[s] : 0.0f;
 
-    // the lists' first eight entries a thread, whatever their lengths (the rows are stride long): one trip to memory
-    const int *hist = r.history + static_cast<int64_t>(s) * r.history_stride, *bid = r.bias_id + static_cast<int64_t>(s) * r.bias_stride;
-    auto ahead = [&](const int *list, int64_t stride, int (&t)[8]) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) t[j] = list && tid + j * NT < stride ? list[tid + j * NT] : -1;
-    };
-    int th[8], tb[8];
-    ahead(r.history ? hist : nullptr, r.history_stride, th);
-    ahead(r.bias_id ? bid : nullptr, r.bias_stride, tb);
     auto checked = [&](int n, int64_t most) {
         if (n >= 0 && n <= most) return n;
         if (tid == 0) atomicOr(a.status, kErrBadShape);
@@ -103,6 +94,17 @@ __global__ void __launch_bounds__(kAdjustThreads, U == 2 ? 6 : 4) k_logits_adjus
     };
     const int nh = r.history ? checked(r.history_len[s], r.history_stride) : 0;
     const int nb = r.bias_id ? checked(r.bias_len[s], r.bias_stride) : 0;
+    // the lists' first eight entries a thread, whatever their lengths (another row follows within a stride): one trip to
+    // memory. The last row may end with its used entries (columns of a wider array): those only, a second trip.
+    const int *hist = r.history + static_cast<int64_t>(s) * r.history_stride, *bid = r.bias_id + static_cast<int64_t>(s) * r.bias_stride;
+    auto ahead = [&](const int *list, int64_t stride, int n, int (&t)[8]) {
+        const int64_t most = s + 1 < a.S ? stride : n;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) t[j] = list && tid + j * NT < most ? list[tid + j * NT] : -1;
+    };
+    int th[8], tb[8];
+    ahead(r.history ? hist : nullptr, r.history_stride, nh, th);
+    ahead(r.bias_id ? bid : nullptr, r.bias_stride, nb, tb);
     for (int i = tid; i < P::smem / 16; i += NT) reinterpret_cast<uint4 *>(adjust_sm)[i] = make_uint4(0, 0, 0, 0);
     __syncthreads();
     // f(token in the slice, place in the list)

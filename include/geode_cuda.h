@@ -452,7 +452,8 @@ int gcuda_op_paged_attn(const gcuda_paged_kv *kv, const gcuda_paged_batch *b, co
  *   token v is allowed: the others become -inf. mask_row [n_seq * (k+1)]: the mask of each row, negative: none
  *   (NULL: row i has mask i, n_masks >= n_seq * (k+1)).
  * Negative ids are padding and are passed over; ids >= V are left out and raise the status word's flag 4; a length
- * outside [0, stride] is clamped, a mask_row >= n_masks leaves its row unmasked, and both raise flag 2. */
+ * outside [0, stride] is clamped, a mask_row >= n_masks leaves its row unmasked, and both raise flag 2. The lists may be
+ * columns of a wider array: nothing behind the last sequence's used entries is read. */
 typedef struct {
     const int *history, *history_len;
     int64_t history_stride;

@@ -493,3 +493,24 @@ def test_adjust_wide(L, act, S, k, V, layout):
     got = dst.cpu()
     assert (got[:, V:] == 7.0).all()
     check_adjust(x, got[:, :V], act, S, k, V, h, history, biases, True, True, (True, True, True))
+
+
+def test_adjust_lists_in_a_wider_array(L):
+    """Lists that are the last columns of a wider array (an answer's tokens behind its prompt's): the other columns, and what is
+    behind the used entries, do not count; the last row ends with its used entries."""
+    S, k, V = 3, 1, 700
+    h, t, r = rules_for(S, k, V, 11, history=25, biases=9)
+    wide = {}
+    for name, skip, width in (("history", 2000, 2025), ("bias_id", 7, 16), ("bias", 7, 16)):
+        w = torch.full((S, width), V + 5 if name != "bias" else 3.0, dtype=t[name].dtype, device="cuda")
+        n = h["history_len" if name == "history" else "bias_len"]
+        for s in range(S):
+            w[s, skip:skip + int(n[s])] = t[name][s, :int(n[s])]
+        wide[name] = w.flatten()[:(S - 1) * width + skip + int(n[S - 1])].clone()
+        setattr(r, name, wide[name].data_ptr() + 4 * skip)
+    r.history_stride, r.bias_stride = 2025, 16
+    x = torch.randn(S * (k + 1), V)
+    src, dst = x.cuda(), torch.empty(S * (k + 1), V, device="cuda")
+    assert L.gcuda_op_logits_adjust(ref(r), src.data_ptr(), dst.data_ptr(), gb.F32, S, k, V, V, V, stream()) == 0
+    torch.cuda.synchronize()
+    check_adjust(x, dst.cpu(), "f32", S, k, V, h, 25, 9, True, True, (True, True, True))

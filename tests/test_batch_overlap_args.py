@@ -55,9 +55,10 @@ def test_attn_outputs_over_rows(good, d, refused):
     assert rc == (E_ARG if refused else good)
 
 
-@pytest.mark.parametrize("name,bytes_", [("history", 2 * 7 * 4), ("history_len", 8), ("drafts", 2 * 2 * 4), ("repetition", 8), ("frequency", 8), ("presence", 8),
-                                         ("bias_id", 2 * 5 * 4), ("bias", 2 * 5 * 4), ("bias_len", 8), ("mask", (2 * 6 + 4) * 4), ("mask_row", 6 * 4)])
+@pytest.mark.parametrize("name,bytes_", [("history", (7 + 1) * 4), ("history_len", 8), ("drafts", 2 * 2 * 4), ("repetition", 8), ("frequency", 8), ("presence", 8),
+                                         ("bias_id", (5 + 1) * 4), ("bias", (5 + 1) * 4), ("bias_len", 8), ("mask", (2 * 6 + 4) * 4), ("mask_row", 6 * 4)])
 def test_adjust_output_over_its_rules(good, name, bytes_):
+    """(Of the lists' last rows the first entry counts: where their used entries end is not known on the host.)"""
     L = cuda_lib()
     S, k, V = 2, 2, 100
     d = dict(history=P, history_len=P, history_stride=7, drafts=P, repetition=P, frequency=P, presence=P, bias_id=P, bias=P, bias_len=P,
