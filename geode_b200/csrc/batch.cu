@@ -107,9 +107,9 @@ int launch_adjust_slices(AdjustArgs a, cudaStream_t st) {
     if (!shared_opt_in<k_logits_adjust<T, U>>(P::smem)) return GCUDA_E_CUDA;
     return launched(launch_ex(k_logits_adjust<T, U>, dim3(a.S * a.slices), dim3(kAdjustThreads), P::smem, st, true, a));
 }
-// Slices of 4096 tokens (33 KB of counts: six CTAs an SM) where they make two CTAs an SM or more, of one load a thread
-// otherwise. 64 x 5 rows of 248320 floats: 242 us with one load a thread, 154 with two, 128 with four; 100 rows of 50257
-// bf16: 21, 17 and 18.
+// Slices of 4096 tokens (33 KB of counts; four CTAs an SM for floats, six for 16 bits) where they make two CTAs an SM or more, of
+// one load a thread otherwise. With one, two and four loads a thread: 64 x 5 rows of 248320 floats 234, 131 and 130 us, of bf16
+// 134, 94 and 145; 100 rows of 50257 bf16 21.4, 15.7 and 19.0; one row of 248320 floats (61 slices of 4096) 10.7, 11.0 and 12.2.
 template <typename T>
 int launch_adjust(const AdjustArgs &a, cudaStream_t st) {
     constexpr int U = sizeof(T) == 4 ? 4 : 2;
@@ -142,7 +142,9 @@ int gcuda_op_paged_append(const gcuda_paged_kv *kv, const gcuda_paged_batch *b, 
     if (const int rc = on_current_device(kv->k, kv->v, kv->k_scale, kv->v_scale, b->row_start, b->length, b->pages, x->q, x->k, x->v, x->q_out,
                                          x->q_norm, x->k_norm, x->rope_dim > 0 ? x->inv_freq : nullptr))
         return rc;
-    // A row's warps: one where the rows alone make three CTAs an SM, else more, up to a turn for every warp
+    // A row's warps: one where the rows alone make three CTAs an SM, else more, up to a turn for every warp. For one warp a row,
+    // and warps for three, four and nine CTAs an SM: 1280 rows to int8 22, 16.0, 19.6 and 22 us, 1000 prompt rows 12.4, 10.0,
+    // 10.6 and 12.5, 320 rows 15.4, 10.3, 10 and 10.4, 9645 prompt rows 56 (57 with nine)
     const int per_turn = 256 / kv->head_dim;   // vectors
     const int turns = (x->n_heads + per_turn - 1) / per_turn + 2 * ((kv->n_kv_heads + per_turn - 1) / per_turn);
     const int warps = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(turns, (3ll * kAppendWarps * sm_count() + b->n_rows - 1) / b->n_rows)));

@@ -6,9 +6,10 @@
 // an id's bias entries the largest index wins). Then each row's slice is one round of 16-byte loads and stores, the next
 // row's loads in flight while one is finished, the first row's and the lists' while the counts are cleared.
 //
-// Measured: 64 x 5 rows of 248320 floats (641 MB) 129 us, 5.0 TB/s; 100 rows of 50257 bf16 (21 MB) 15 us, two waves of slices
-// that are each a chain lists -> atomics -> row; one row of 248320 floats 6.8 us, the same chain. A value at a time with 8 bytes
-// of counts read for each: 449, 25 and 13 us.
+// Measured: 64 x 5 rows of 248320 floats (641 MB) 130 us, 4.9 TB/s: 3904 slices in six to seven turns of four CTAs an SM, each
+// with its walk through the lists before the first store; 100 rows of 50257 bf16 (21 MB) 15.6 us, 1300 slices in one and a half
+// turns, each a chain lists -> atomics -> row; one row of 248320 floats 7.0 us, the same chain. A value at a time with 8 bytes of
+// counts read for each: 449, 25 and 13 us.
 #pragma once
 
 #include "paged.cuh"

@@ -3,7 +3,7 @@
 // An item is one (sequence, key head, block of query rows): the sequence's T rows times the G query heads that share the key
 // head, R = T * G rows in blocks of 8 (k_paged_attn), 16 or 40 (k_paged_attn_rows, paged_attn_rows.cuh). Items are cut into
 // tiles of positions and the tiles of all items, laid end to end with a few tiles' time for each item's beginning, are dealt
-// out evenly to the resident CTAs (each finds its share by a scan over the lengths on the device: whatever the lengths, every
+// out evenly to two CTAs an SM (each finds its share by a scan over the lengths on the device: whatever the lengths, every
 // CTA has the same work). What a CTA holds of an item that it does not finish goes to the scratch and k_paged_attn_join adds
 // the parts up. The copies run ahead of the products across tiles and items alike, so memory is not left idle while an item
 // ends and the next begins.
@@ -25,8 +25,8 @@
 // rows of any scale keep their bits. Scores, sums, maxima and outputs are float.
 //
 // Measured, main kernel and join (8 query rows a key head): 64 ragged conversations of up to 8192 positions over an int8
-// cache of 2 heads of 256 (278 MB) 61 us, each further 278 MB 41 us (6.8 TB/s); 2 x 131072 positions of bf16 73 us (5.2
-// TB/s); 128 of up to 1000 in f16, 8 heads of 128, 66 us (items of four tiles: their beginnings and ends); one conversation
+// cache of 2 heads of 256 (278 MB) 62 us, each further 278 MB 40 us (7 TB/s); 2 x 131072 positions of bf16 73 us (5.2
+// TB/s); 128 of up to 1000 in f16, 8 heads of 128, 69 us (items of four tiles: their beginnings and ends); one conversation
 // of 8192 positions 16 us (latency: the scan and the first copies 4.7, a tile 2.5, the join 5).
 #pragma once
 

@@ -7,9 +7,9 @@
 // maxima are the CTA's: a tile on which none grows far (nearly all but the first) costs one vote, folded into the barrier.
 //
 // Measured: 32 ragged verify batches of 5 rows (40 rows an item), up to 8192 positions of int8, 2 heads of 256, float
-// activations: 105 us (142 MB; 72 us for each further 142 MB). The tensor pipe is busy 41% of the time: a warp and tile has 280
+// activations: 106 us (142 MB; 68 us for each further 142 MB). The tensor pipe is busy 36% of the time: a warp and tile has 280
 // products (at the 8.2 cycles of mma.sync the pipe's floor is 35 us) among 1900 instructions in dependent phases, two warps a
-// scheduler.
+// scheduler, which wait for fixed latencies (2 warps an issue) and instruction fetches (1).
 #pragma once
 
 #include "paged_attn.cuh"

@@ -387,10 +387,10 @@ typedef struct {
 /* The step's rows: sequence s owns rows row_start[s] .. row_start[s+1]-1 (at most max_rows) of the step's buffers of
  * n_rows rows; its cache holds length[s] positions, its rows the last of them; position p lies on page
  * pages[s * pages_stride + p / page_size], p / page_size < max_pages (max_pages * page_size, n_seq and n_rows at most
- * 2^30). The three arrays are device memory (int32), so a captured step follows its plan from replay to replay. Rows of
- * no sequence (behind row_start[n_seq]) are not written. What is out of range on the device raises the status word's
- * flag 2 (gcuda_op_status): a sequence whose rows or length are out of range is left out whole; a position on a page id
- * outside [0, n_pages) is not stored and not attended to. */
+ * 2^30). The three arrays are device memory (int32), so a captured step follows its plan from replay to replay; they
+ * must not change while a call runs. Rows of no sequence (behind row_start[n_seq]) are not written. What is out of range
+ * on the device raises the status word's flag 2 (gcuda_op_status): a sequence whose rows or length are out of range is
+ * left out whole; a position on a page id outside [0, n_pages) is not stored and not attended to. */
 typedef struct {
     int n_seq, n_rows, max_rows, max_pages;
     const int *row_start, *length, *pages;
@@ -416,7 +416,9 @@ typedef struct {
     const float *q_norm, *k_norm, *inv_freq;
 } gcuda_append_rows;
 /* Appends the step's rows: row i of sequence s (i-th of T) at position length[s] - T + i. Two sequences must not
- * write one position's rows in the same call. */
+ * write one position's rows in the same call. A row before position 0 (T > length[s]) is not stored, its q_out is left as it
+ * was, and it raises flag 2; a row on a page id outside [0, n_pages) is not stored, its queries are normed and rotated. Rows with
+ * infinities or NaN hold no finite value in an int8 cache. */
 int gcuda_op_paged_append(const gcuda_paged_kv *kv, const gcuda_paged_batch *b, const gcuda_append_rows *x, void *stream);
 
 /* The rows of gcuda_op_paged_attn: q rows of n_heads heads (n_heads a multiple of n_kv_heads, query head h reads key
@@ -425,8 +427,9 @@ int gcuda_op_paged_append(const gcuda_paged_kv *kv, const gcuda_paged_batch *b, 
  * p = length[s] - T + i attends to the positions 0 .. p (the last `window` of them when window > 0):
  * out = sum softmax(scale * q . k) v, lse = log sum exp(scale * q . k). A row that sees no position (an empty
  * sequence, p < 0) gives zeros and lse -inf. Values at positions a row does not see do not touch it, whatever they
- * are; where a row does see a score that is no number, its outputs and lse are none. out must not overlap q (elsewhere, or
- * other columns of rows with one stride), lse neither. type: of q and out. */
+ * are. Where a row does see a score that is no number, its outputs and lse are none; where it sees an infinite value, that
+ * output is not finite (an infinity or no number). out must not overlap q (elsewhere, or other columns of rows with one
+ * stride), lse neither. type: of q and out. */
 typedef struct {
     int type, n_heads, window;
     float scale;
@@ -470,8 +473,9 @@ typedef struct {
 } gcuda_logit_rules;
 /* d_out row = the rules in this order (biases, penalties, mask) on d_in row, for S sequences of k+1 rows of V logits
  * (rows s * (k+1) + i, in_stride and out_stride values apart), computed in float and rounded once to `type`
- * (GCUDA_F32, GCUDA_BF16 or GCUDA_F16); k at most 64; V, history_stride and bias_stride at most 2^30. d_out may be d_in with the same stride; otherwise they
- * must not overlap. */
+ * (GCUDA_F32, GCUDA_BF16 or GCUDA_F16); k at most 64; V, history_stride and bias_stride at most 2^30. d_out may be d_in with
+ * the same stride; otherwise they must not overlap. (Rows that lie differently to 16 bytes in d_in and d_out go a value at a
+ * time.) */
 int gcuda_op_logits_adjust(const gcuda_logit_rules *r, const void *d_in, void *d_out, int type, int S, int k, int V,
                            int64_t in_stride, int64_t out_stride, void *stream);
 
