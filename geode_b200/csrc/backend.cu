@@ -212,6 +212,14 @@ int cuda_fail(gcuda *g, cudaError_t e, const char *what) {
                 std::string(what) + ": " + cudaGetErrorString(e));
 }
 
+// A copy in the order of the handle's stream, done on return. The handle's streams do not wait for the default stream nor it
+// for them: its cudaMemcpy could be overtaken by the zeroing that dalloc queued (a table of units left zeros: its null tile
+// addresses fault), and a small one returns before the bytes are in place.
+cudaError_t copy_now(gcuda *g, void *dst, const void *src, size_t bytes, cudaMemcpyKind kind) {
+    const cudaError_t e = cudaMemcpyAsync(dst, src, bytes, kind, g->st);
+    return e == cudaSuccess ? cudaStreamSynchronize(g->st) : e;
+}
+
 template <typename T>
 bool dalloc(gcuda *g, T **p, size_t count) {
     void *q = nullptr;
@@ -887,7 +895,7 @@ int gcuda_adopt_raw(gcuda *g, const void *data, size_t bytes) {
     void *dst = nullptr;
     cudaError_t e = cudaMalloc(&dst, bytes);
     if (e != cudaSuccess) return cuda_fail(g, e, "adopt_raw cudaMalloc");
-    e = cudaMemcpy(dst, data, bytes, cudaMemcpyHostToDevice);
+    e = copy_now(g, dst, data, bytes, cudaMemcpyHostToDevice);
     if (e != cudaSuccess) {
         cudaFree(dst);
         return cuda_fail(g, e, "adopt_raw");
@@ -921,13 +929,13 @@ int gcuda_adopt_experts(gcuda *g, const uint8_t *blocks, int n, size_t stride, c
     cudaError_t e = cudaMalloc(&X.d, static_cast<size_t>(n) * stride);
     if (e != cudaSuccess) return cuda_fail(g, e, "adopt_experts cudaMalloc");
     e = cudaMalloc(&X.scales, sizeof(float) * 2 * n);
-    if (e == cudaSuccess) e = cudaMemcpy(X.scales, scales, sizeof(float) * 2 * n, cudaMemcpyHostToDevice);
+    if (e == cudaSuccess) e = copy_now(g, X.scales, scales, sizeof(float) * 2 * n, cudaMemcpyHostToDevice);
     if (e != cudaSuccess) {
         cudaFree(X.d);
         return cuda_fail(g, e, "adopt_experts");
     }
     // the blocks stay raw until gcuda_setup knows hidden and ff (then each is relaid in place: see setup)
-    e = cudaMemcpy(X.d, blocks, static_cast<size_t>(n) * stride, cudaMemcpyHostToDevice);
+    e = copy_now(g, X.d, blocks, static_cast<size_t>(n) * stride, cudaMemcpyHostToDevice);
     if (e != cudaSuccess) return cuda_fail(g, e, "adopt_experts copy");
     g->experts.push_back(X);
     return static_cast<int>(g->experts.size()) - 1;
@@ -946,23 +954,21 @@ int ep_exchange_setup(gcuda *g, size_t slot_floats) {
         g->xbuf = nullptr;
         return fail(g, GCUDA_E_MEMORY, "ep exchange buffer: cudaMalloc");
     }
-    LAUNCH_OK(cudaMemset(g->xbuf, 0, bytes));
+    LAUNCH_OK(cudaMemsetAsync(g->xbuf, 0, bytes, g->st));
     g->xflags = static_cast<uint32_t *>(g->xbuf);
     g->eout = reinterpret_cast<float *>(static_cast<uint8_t *>(g->xbuf) + fbytes);
     if (!dalloc(g, &g->ep_epoch, 1) || !dalloc(g, &g->xcount, 1)) return GCUDA_E_MEMORY;
-    LAUNCH_OK(cudaMemset(g->ep_epoch, 0, sizeof(int)));
-    LAUNCH_OK(cudaMemset(g->xcount, 0, sizeof(unsigned int)));
     cudaIpcMemHandle_t mine;
     LAUNCH_OK(cudaIpcGetMemHandle(&mine, g->xbuf));
     void *d_h = nullptr;
     if (cudaMalloc(&d_h, sizeof(cudaIpcMemHandle_t) * (W + 1)) != cudaSuccess) return fail(g, GCUDA_E_MEMORY, "cudaMalloc");
     std::vector<cudaIpcMemHandle_t> all(static_cast<size_t>(W));
     uint8_t *d_mine = static_cast<uint8_t *>(d_h) + sizeof(cudaIpcMemHandle_t) * W;
-    cudaError_t e = cudaMemcpy(d_mine, &mine, sizeof mine, cudaMemcpyHostToDevice);
+    cudaError_t e = copy_now(g, d_mine, &mine, sizeof mine, cudaMemcpyHostToDevice);
     ncclResult_t nr = ncclSuccess;
     if (e == cudaSuccess) nr = nccl().all_gather(d_mine, d_h, sizeof mine, ncclUint8, g->comm, g->st);
     if (e == cudaSuccess && nr == ncclSuccess) e = cudaStreamSynchronize(g->st);
-    if (e == cudaSuccess && nr == ncclSuccess) e = cudaMemcpy(all.data(), d_h, sizeof(cudaIpcMemHandle_t) * W, cudaMemcpyDeviceToHost);
+    if (e == cudaSuccess && nr == ncclSuccess) e = copy_now(g, all.data(), d_h, sizeof(cudaIpcMemHandle_t) * W, cudaMemcpyDeviceToHost);
     cudaFree(d_h);
     if (nr != ncclSuccess) return fail(g, GCUDA_E_CUDA, std::string("ncclAllGather: ") + nccl().error_string(nr));
     LAUNCH_OK(e);
@@ -1117,7 +1123,7 @@ int gcuda_setup(gcuda *g, const gcuda_shape *shape, const gcuda_layer *layers, i
         std::vector<float> inv(static_cast<size_t>(std::max(1, s.rope_dim / 2)));
         for (int i = 0; i < s.rope_dim / 2; ++i)
             inv[static_cast<size_t>(i)] = 1.0f / std::pow(s.rope_theta, static_cast<float>(2 * i) / static_cast<float>(s.rope_dim));
-        cudaMemcpy(g->inv_freq, inv.data(), inv.size() * sizeof(float), cudaMemcpyHostToDevice);
+        LAUNCH_OK(copy_now(g, g->inv_freq, inv.data(), inv.size() * sizeof(float), cudaMemcpyHostToDevice));
     }
     // the unit tables and the small merged weight buffers
     std::vector<GemvUnit> U;
@@ -1143,8 +1149,8 @@ int gcuda_setup(gcuda *g, const gcuda_shape *shape, const gcuda_layer *layers, i
             plain_units(U, *out, g->x, H, kAccumulate);
             P.n_out = static_cast<int>(U.size()) - P.u_out;
             if (!dalloc(g, &P.ab_w, static_cast<size_t>(2 * s.gdn_v_heads) * H)) return GCUDA_E_MEMORY;
-            cudaMemcpy(P.ab_w, a->d, a->bytes, cudaMemcpyDeviceToDevice);
-            cudaMemcpy(P.ab_w + static_cast<size_t>(s.gdn_v_heads) * H, b->d, b->bytes, cudaMemcpyDeviceToDevice);
+            LAUNCH_OK(copy_now(g, P.ab_w, a->d, a->bytes, cudaMemcpyDeviceToDevice));
+            LAUNCH_OK(copy_now(g, P.ab_w + static_cast<size_t>(s.gdn_v_heads) * H, b->d, b->bytes, cudaMemcpyDeviceToDevice));
         } else {
             P.ai = ai++;
             const DevTensor *q = q4(L.q), *k = q4(L.k), *v = q4(L.v), *o = q4(L.o);
@@ -1176,8 +1182,8 @@ int gcuda_setup(gcuda *g, const gcuda_shape *shape, const gcuda_layer *layers, i
                 g->experts[static_cast<size_t>(L.experts)].n != s.n_experts)
                 return fail(g, GCUDA_E_ARG, "setup: MoE layer " + name + " tensors");
             if (!dalloc(g, &P.router_w, static_cast<size_t>(s.n_experts + 1) * H)) return GCUDA_E_MEMORY;
-            cudaMemcpy(P.router_w, r->d, r->bytes, cudaMemcpyDeviceToDevice);
-            cudaMemcpy(P.router_w + static_cast<size_t>(s.n_experts) * H, gt->d, gt->bytes, cudaMemcpyDeviceToDevice);
+            LAUNCH_OK(copy_now(g, P.router_w, r->d, r->bytes, cudaMemcpyDeviceToDevice));
+            LAUNCH_OK(copy_now(g, P.router_w + static_cast<size_t>(s.n_experts) * H, gt->d, gt->bytes, cudaMemcpyDeviceToDevice));
         }
         return GCUDA_OK;
     };
@@ -1216,7 +1222,7 @@ int gcuda_setup(gcuda *g, const gcuda_shape *shape, const gcuda_layer *layers, i
     }
     g->n_units = static_cast<int>(U.size());
     if (!dalloc(g, &g->units, U.size())) return GCUDA_E_MEMORY;
-    cudaMemcpy(g->units, U.data(), U.size() * sizeof(GemvUnit), cudaMemcpyHostToDevice);
+    LAUNCH_OK(copy_now(g, g->units, U.data(), U.size() * sizeof(GemvUnit), cudaMemcpyHostToDevice));
     RC_OK(set_attrs(g));
     LAUNCH_OK(cudaStreamSynchronize(g->st));
     RC_OK(record_graphs(g));
@@ -1248,7 +1254,7 @@ int gcuda_verify_device(gcuda *g, const int *d_toks, int n) {
     LAUNCH_OK(cudaStreamSynchronize(g->st));
     RC_OK(status_outcome(g, *g->h_status));
     cudaEventElapsedTime(&g->last_ms, g->ev0, g->ev1);
-    LAUNCH_OK(cudaMemcpy(g->last_toks, g->d_toks, sizeof(int) * n, cudaMemcpyDeviceToHost));
+    LAUNCH_OK(copy_now(g, g->last_toks, g->d_toks, sizeof(int) * n, cudaMemcpyDeviceToHost));
     g->pos += n;
     g->last_batch = n;
     g->hid_rows = n;
@@ -1534,10 +1540,10 @@ int gcuda_state_get(gcuda *g, float *conv, float *gdn, int8_t *kv, float *kv_sca
     cudaSetDevice(g->device);
     LAUNCH_OK(cudaStreamSynchronize(g->st));
     const gcuda_shape &s = g->sh;
-    if (conv && g->conv_n) LAUNCH_OK(cudaMemcpy(conv, g->conv, g->conv_n * sizeof(float), cudaMemcpyDeviceToHost));
+    if (conv && g->conv_n) LAUNCH_OK(copy_now(g, conv, g->conv, g->conv_n * sizeof(float), cudaMemcpyDeviceToHost));
     if (gdn && g->gdn_n) {
         std::vector<float> d(g->gdn_n);
-        LAUNCH_OK(cudaMemcpy(d.data(), g->gdn, g->gdn_n * sizeof(float), cudaMemcpyDeviceToHost));
+        LAUNCH_OK(copy_now(g, d.data(), g->gdn, g->gdn_n * sizeof(float), cudaMemcpyDeviceToHost));
         const int nv = s.gdn_v_heads, dv = s.gdn_v_dim, dk = s.gdn_k_dim;
         for (size_t l = 0; l < static_cast<size_t>(g->n_gdn); ++l)
             for (int h = 0; h < nv; ++h)
@@ -1554,12 +1560,12 @@ int gcuda_state_get(gcuda *g, float *conv, float *gdn, int8_t *kv, float *kv_sca
     for (int a = 0; a < g->n_attn + (g->has_mtp ? 1 : 0) && positions > 0; ++a) {
         const size_t base = static_cast<size_t>(a) * s.context;
         if (kv) {
-            LAUNCH_OK(cudaMemcpy(kv + (static_cast<size_t>(a) * 2 + 0) * positions * row, g->kc + base * row, positions * row, cudaMemcpyDeviceToHost));
-            LAUNCH_OK(cudaMemcpy(kv + (static_cast<size_t>(a) * 2 + 1) * positions * row, g->vc + base * row, positions * row, cudaMemcpyDeviceToHost));
+            LAUNCH_OK(copy_now(g, kv + (static_cast<size_t>(a) * 2 + 0) * positions * row, g->kc + base * row, positions * row, cudaMemcpyDeviceToHost));
+            LAUNCH_OK(copy_now(g, kv + (static_cast<size_t>(a) * 2 + 1) * positions * row, g->vc + base * row, positions * row, cudaMemcpyDeviceToHost));
         }
         if (kv_scale) {
-            LAUNCH_OK(cudaMemcpy(kv_scale + (static_cast<size_t>(a) * 2 + 0) * positions * nkv, g->ks + base * nkv, positions * nkv * 4, cudaMemcpyDeviceToHost));
-            LAUNCH_OK(cudaMemcpy(kv_scale + (static_cast<size_t>(a) * 2 + 1) * positions * nkv, g->vs + base * nkv, positions * nkv * 4, cudaMemcpyDeviceToHost));
+            LAUNCH_OK(copy_now(g, kv_scale + (static_cast<size_t>(a) * 2 + 0) * positions * nkv, g->ks + base * nkv, positions * nkv * 4, cudaMemcpyDeviceToHost));
+            LAUNCH_OK(copy_now(g, kv_scale + (static_cast<size_t>(a) * 2 + 1) * positions * nkv, g->vs + base * nkv, positions * nkv * 4, cudaMemcpyDeviceToHost));
         }
     }
     return GCUDA_OK;
@@ -1570,7 +1576,7 @@ int gcuda_state_put(gcuda *g, const float *conv, const float *gdn, const int8_t 
     cudaSetDevice(g->device);
     LAUNCH_OK(cudaStreamSynchronize(g->st));
     const gcuda_shape &s = g->sh;
-    if (conv && g->conv_n) LAUNCH_OK(cudaMemcpy(g->conv, conv, g->conv_n * sizeof(float), cudaMemcpyHostToDevice));
+    if (conv && g->conv_n) LAUNCH_OK(copy_now(g, g->conv, conv, g->conv_n * sizeof(float), cudaMemcpyHostToDevice));
     if (gdn && g->gdn_n) {
         std::vector<float> d(g->gdn_n);
         const int nv = s.gdn_v_heads, dv = s.gdn_v_dim, dk = s.gdn_k_dim;
@@ -1581,18 +1587,18 @@ int gcuda_state_put(gcuda *g, const float *conv, const float *gdn, const int8_t 
                         d[((l * nv + h) * dv + j) * dk + i] =
                             gdn[(l * nv + h) * static_cast<size_t>(dv) * dk + static_cast<size_t>(j / 16) * dk * 16 +
                                 static_cast<size_t>(i) * 16 + (j % 16)];
-        LAUNCH_OK(cudaMemcpy(g->gdn, d.data(), g->gdn_n * sizeof(float), cudaMemcpyHostToDevice));
+        LAUNCH_OK(copy_now(g, g->gdn, d.data(), g->gdn_n * sizeof(float), cudaMemcpyHostToDevice));
     }
     const size_t row = g->kvrow, nkv = s.n_kv_heads;
     for (int a = 0; a < g->n_attn + (g->has_mtp ? 1 : 0) && pos > 0; ++a) {
         const size_t base = static_cast<size_t>(a) * s.context;
         if (kv) {
-            LAUNCH_OK(cudaMemcpy(g->kc + base * row, kv + (static_cast<size_t>(a) * 2 + 0) * pos * row, pos * row, cudaMemcpyHostToDevice));
-            LAUNCH_OK(cudaMemcpy(g->vc + base * row, kv + (static_cast<size_t>(a) * 2 + 1) * pos * row, pos * row, cudaMemcpyHostToDevice));
+            LAUNCH_OK(copy_now(g, g->kc + base * row, kv + (static_cast<size_t>(a) * 2 + 0) * pos * row, pos * row, cudaMemcpyHostToDevice));
+            LAUNCH_OK(copy_now(g, g->vc + base * row, kv + (static_cast<size_t>(a) * 2 + 1) * pos * row, pos * row, cudaMemcpyHostToDevice));
         }
         if (kv_scale) {
-            LAUNCH_OK(cudaMemcpy(g->ks + base * nkv, kv_scale + (static_cast<size_t>(a) * 2 + 0) * pos * nkv, pos * nkv * 4, cudaMemcpyHostToDevice));
-            LAUNCH_OK(cudaMemcpy(g->vs + base * nkv, kv_scale + (static_cast<size_t>(a) * 2 + 1) * pos * nkv, pos * nkv * 4, cudaMemcpyHostToDevice));
+            LAUNCH_OK(copy_now(g, g->ks + base * nkv, kv_scale + (static_cast<size_t>(a) * 2 + 0) * pos * nkv, pos * nkv * 4, cudaMemcpyHostToDevice));
+            LAUNCH_OK(copy_now(g, g->vs + base * nkv, kv_scale + (static_cast<size_t>(a) * 2 + 1) * pos * nkv, pos * nkv * 4, cudaMemcpyHostToDevice));
         }
     }
     g->pos = pos;
@@ -1630,7 +1636,7 @@ int gcuda_debug_read(gcuda *g, int what, void *out, size_t bytes) {
     const void *src = what == 0 ? static_cast<const void *>(g->x) : what == 1 ? g->hf : what == 2 ? g->core_f
                       : what == 3 ? static_cast<const void *>(g->route) : what == 4 ? g->hid : what == 5 ? g->convd
                       : what == 6 ? g->ab : what == 7 ? g->zb : g->big;
-    LAUNCH_OK(cudaMemcpy(out, src, bytes, cudaMemcpyDeviceToHost));
+    LAUNCH_OK(copy_now(g, out, src, bytes, cudaMemcpyDeviceToHost));
     return GCUDA_OK;
 }
 
@@ -1682,9 +1688,9 @@ int gcuda_debug_trace(gcuda *g, const int *toks, int n, float *x, float *router_
     if (rc == GCUDA_OK) rc = enqueue_step(g, n);
     if (rc == GCUDA_OK) rc = check_status(g);
     std::vector<RouteOut> ro(moe ? L : 0);
-    if (rc == GCUDA_OK && (cudaMemcpy(x, bx, xbytes, cudaMemcpyDeviceToHost) != cudaSuccess ||
-                           (moe && cudaMemcpy(ro.data(), bt, L * sizeof(RouteOut), cudaMemcpyDeviceToHost) != cudaSuccess) ||
-                           (moe && router_logits && cudaMemcpy(router_logits, br, rbytes, cudaMemcpyDeviceToHost) != cudaSuccess)))
+    if (rc == GCUDA_OK && (copy_now(g, x, bx, xbytes, cudaMemcpyDeviceToHost) != cudaSuccess ||
+                           (moe && copy_now(g, ro.data(), bt, L * sizeof(RouteOut), cudaMemcpyDeviceToHost) != cudaSuccess) ||
+                           (moe && router_logits && copy_now(g, router_logits, br, rbytes, cudaMemcpyDeviceToHost) != cudaSuccess)))
         rc = GCUDA_E_CUDA;
     g->tr_x = nullptr;
     g->tr_rlog = nullptr;
@@ -1725,7 +1731,7 @@ int gcuda_debug_kernel_times(gcuda *g, const int *toks, int n, int reps, float *
     for (int k = 0; k < kKtKinds; ++k) ms[k] = 0.0f, launches[k] = 0;
     float total = 0.0f;
     int u0 = 0, u1 = 0;
-    LAUNCH_OK(cudaMemcpy(&u0, &g->step->n_union_sum, sizeof(int), cudaMemcpyDeviceToHost));
+    LAUNCH_OK(copy_now(g, &u0, &g->step->n_union_sum, sizeof(int), cudaMemcpyDeviceToHost));
     const bool keep_pdl = g->pdl;
     g->pdl = false;
     int rc = GCUDA_OK;
@@ -1754,7 +1760,7 @@ int gcuda_debug_kernel_times(gcuda *g, const int *toks, int n, int reps, float *
     }
     g->pdl = keep_pdl;
     if (rc == GCUDA_OK) rc = check_status(g);
-    if (rc == GCUDA_OK && cudaMemcpy(&u1, &g->step->n_union_sum, sizeof(int), cudaMemcpyDeviceToHost) != cudaSuccess)
+    if (rc == GCUDA_OK && copy_now(g, &u1, &g->step->n_union_sum, sizeof(int), cudaMemcpyDeviceToHost) != cudaSuccess)
         rc = GCUDA_E_CUDA;
     for (cudaEvent_t e : marks.pool) cudaEventDestroy(e);
     cudaEventDestroy(e0);
@@ -1841,7 +1847,7 @@ int gcuda_synth_experts(gcuda *g, int n, int hidden, int ff, float global, uint6
     cudaError_t e = cudaMalloc(&X.d, static_cast<size_t>(n) * X.stride);
     if (e != cudaSuccess) return cuda_fail(g, e, "synth_experts cudaMalloc");
     e = cudaMalloc(&X.scales, sizeof(float) * 2 * n);
-    if (e == cudaSuccess) e = cudaMemcpy(X.scales, X.host_scales.data(), sizeof(float) * 2 * n, cudaMemcpyHostToDevice);
+    if (e == cudaSuccess) e = copy_now(g, X.scales, X.host_scales.data(), sizeof(float) * 2 * n, cudaMemcpyHostToDevice);
     if (e != cudaSuccess) return cuda_fail(g, e, "synth_experts");
     k_synth_tiled<<<grid_for(static_cast<size_t>(n) * X.stride / 8), 256, 0, g->st>>>(X.d, static_cast<size_t>(n) * X.stride, seed);
     count_launch();
