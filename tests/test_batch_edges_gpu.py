@@ -514,3 +514,37 @@ def test_adjust_lists_in_a_wider_array(L):
     assert L.gcuda_op_logits_adjust(ref(r), src.data_ptr(), dst.data_ptr(), gb.F32, S, k, V, V, V, stream()) == 0
     torch.cuda.synchronize()
     check_adjust(x, dst.cpu(), "f32", S, k, V, h, 25, 9, True, True, (True, True, True))
+
+
+ALLOCATORS = """
+import sys
+sys.path[:0] = [{root!r}, {tests!r}]
+import torch
+import batch_helpers as bh
+from geode_b200 import batch as gb, cuda_lib
+from test_batch_gpu import append_inputs, attn_inputs, run_attn, check_attn, rules_for, stream
+L = cuda_lib()
+plan = bh.Plan([1, 2], [40, 70], 16, 2, 64, "i8")
+plan.randomize(1)
+x = attn_inputs(L, plan, "f32", 4, 2)
+assert run_attn(L, plan, x) == 0
+torch.cuda.synchronize()
+check_attn(plan, x, "f32", 4)
+y = append_inputs(plan, "f32", 4, 32, True, 1)
+assert L.gcuda_op_paged_append(bh.ref(plan.kv), bh.ref(plan.batch), bh.ref(y["desc"]), stream()) == 0
+h, t, r = rules_for(2, 2, 500, 3)
+src, dst = torch.zeros(6, 500, device="cuda"), torch.zeros(6, 500, device="cuda")
+assert L.gcuda_op_logits_adjust(bh.ref(r), src.data_ptr(), dst.data_ptr(), gb.F32, 2, 2, 500, 500, 500, stream()) == 0
+torch.cuda.synchronize()
+print("taken")
+"""
+
+
+@pytest.mark.parametrize("conf", ["expandable_segments:True", "backend:cudaMallocAsync"])
+def test_memory_of_other_allocators_is_taken(L, conf):
+    """Mapped segments and the stream-ordered pools are the device's memory too."""
+    here = os.path.dirname(os.path.abspath(__file__))
+    code = ALLOCATORS.format(root=os.path.dirname(here), tests=here)
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300,
+                       env={**os.environ, "PYTORCH_CUDA_ALLOC_CONF": conf})
+    assert r.returncode == 0 and "taken" in r.stdout, r.stderr[-2000:]
